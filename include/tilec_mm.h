@@ -42,7 +42,7 @@
 extern "C" {
 #endif
 
-#define TILEC_MM_ABI_VERSION 6
+#define TILEC_MM_ABI_VERSION 7
 
 #if defined(__GNUC__)
 #define TILEC_API __attribute__((visibility("default")))
@@ -190,6 +190,7 @@ TILEC_API int tilec_mm_set_table(const int32_t* rows, int32_t nrows);
 #define TILEC_DEV_STATUS_TIMEOUT 1    /* a bounded wait gave up (time limit); the kernel unwound */
 #define TILEC_DEV_STATUS_TMEM 2       /* TMEM allocation returned an unexpected address */
 #define TILEC_DEV_STATUS_BAD_LAUNCH 4 /* a kernel was launched with a block shape it was not built for */
+#define TILEC_DEV_STATUS_BAD_INDEX 8  /* ABI version 7: a class index outside the vocabulary (tilec_linear_ce_*) */
 
 /* Read and clear the device status word of the current device (0 = clean).
  * Synchronises `stream`. */
@@ -250,6 +251,58 @@ TILEC_API int tilec_mm_f32_splitk_noalloc(const float* A, const float* B, float*
                                           int64_t M, int64_t N, int64_t K,
                                           int64_t lda, int64_t ldb, int64_t ldc,
                                           int32_t split_k, void* stream);
+
+/* ---------------------------------------------------------------- language-model products
+ * ABI version 7; no counterpart in the reference.  The rules above hold: stream-ordered, no
+ * allocation, no synchronisation, status codes.  Workspaces are 256-byte aligned and belong
+ * to one call at a time (they hold nothing between calls). */
+
+/* Element types of 16- and 32-bit operands. */
+#define TILEC_DTYPE_F32 0
+#define TILEC_DTYPE_F16 1
+#define TILEC_DTYPE_BF16 2
+
+/* reduction of tilec_linear_ce_*: T losses, their sum, or their mean over the tokens whose
+ * target is not ignore_index. */
+#define TILEC_REDUCE_NONE 0
+#define TILEC_REDUCE_SUM 1
+#define TILEC_REDUCE_MEAN 2
+
+/* Softmax cross entropy of a linear layer's outputs, which are never stored as a whole:
+ *   logit[t, v] = sum_d x[t, d] * w[v, d]
+ *   loss[t]     = log(sum_v exp(logit[t, v])) - logit[t, target[t]]
+ * x [T, D] and w [V, D] of `dtype` with row strides ldx / ldw (elements), target [T] int64.
+ * Logits are fp32 (fp32 operands: the 3xTF32 product, a piece of the vocabulary at a time in
+ * the workspace; 16-bit operands: only in tensor memory).  A target equal to ignore_index
+ * gives a loss of 0 and no gradient.  Any other target outside [0, V) gives NaN (loss and
+ * gradients) and sets TILEC_DEV_STATUS_BAD_INDEX.  The mean over no target is NaN.
+ *   loss:  T floats (TILEC_REDUCE_NONE) or one float.
+ *   stats: 2 * T + 1 floats, 8-byte aligned, for the backward pass: per token (m, s) with
+ *          sum_v exp(logit) = s * 2^m, then (SUM / MEAN) the number of tokens with a target.
+ * Workspace: tilec_linear_ce_workspace_bytes(..., grads = 0). */
+TILEC_API int tilec_linear_ce_forward(const void* x, const void* w, const int64_t* target, int32_t dtype, int64_t T,
+                                      int64_t V, int64_t D, int64_t ldx, int64_t ldw, int64_t ignore_index,
+                                      int32_t reduction, float* loss, float* stats, void* workspace,
+                                      size_t ws_bytes, void* stream);
+
+/* Gradients of the above, from the same operands and the forward pass's stats:
+ *   dlogit[t, v] = g[t] * (softmax[t, v] - [v == target[t]])
+ *   dx = dlogit . w ([T, D], row-major, dense)    dw = dlogit^T . x ([V, D], row-major, dense)
+ * grad: the loss's gradient, T floats (TILEC_REDUCE_NONE) or one float.  dx or dw may be
+ * NULL.  dx and dw have the operands' dtype; sums are fp32, dlogit is rounded to the
+ * operands' dtype for the products (fp32: not rounded).  Logits are computed again, a piece
+ * of the vocabulary at a time (at most 512 MiB of dlogit, or 4096 entries).  Rows of x whose
+ * target is ignore_index get zeros in dx and never reach dw, whatever they hold.
+ * Workspace: tilec_linear_ce_workspace_bytes(..., grads = (dx ? 1 : 0) | (dw ? 2 : 0)). */
+TILEC_API int tilec_linear_ce_backward(const void* x, const void* w, const int64_t* target, int32_t dtype, int64_t T,
+                                       int64_t V, int64_t D, int64_t ldx, int64_t ldw, int64_t ignore_index,
+                                       int32_t reduction, const float* stats, const float* grad, void* dx, void* dw,
+                                       void* workspace, size_t ws_bytes, void* stream);
+
+/* Workspace bytes of the two calls above (NULL operands: assumed 16-byte aligned). */
+TILEC_API size_t tilec_linear_ce_workspace_bytes(const void* x, const void* w, int32_t dtype, int64_t T, int64_t V,
+                                                 int64_t D, int64_t ldx, int64_t ldw, int32_t reduction,
+                                                 int32_t grads);
 
 #ifdef __cplusplus
 }

@@ -26,11 +26,12 @@ EXPORTS = [
     "tilec_mm_f32", "tilec_mm_workspace_bytes", "tilec_mm_plan", "tilec_mm_set_table",
     "tilec_mm_device_status", "tilec_strerror", "tilec_mm_abi_version", "tilec_mm_built_arch",
     "tilec_mm_f32_splitk_noalloc", "tilec_mm_selftest_wait", "tilec_mm_f32_ex", "tilec_mm_workspace_bytes_ex",
-    "tilec_mm_set_wait_limit",
+    "tilec_mm_set_wait_limit", "tilec_linear_ce_forward", "tilec_linear_ce_backward",
+    "tilec_linear_ce_workspace_bytes",
 ]
 
 # Bits of the device status word (TILEC_DEV_STATUS_* in include/tilec_mm.h).
-DEV_STATUS_BITS = {1: "TIMEOUT", 2: "TMEM", 4: "BAD_LAUNCH"}
+DEV_STATUS_BITS = {1: "TIMEOUT", 2: "TMEM", 4: "BAD_LAUNCH", 8: "BAD_INDEX"}
 
 
 def status_bits(word):
@@ -121,6 +122,14 @@ def load():
         lib.tilec_mm_workspace_bytes_ex.argtypes = [vp, vp, vp, i64, i64, i64, i64, i64, i64, i64, i64, i64, i64,
                                                     cfgp]
         lib.tilec_mm_workspace_bytes_ex.restype = sz
+        i32 = ctypes.c_int32
+        lib.tilec_linear_ce_forward.argtypes = [vp, vp, vp, i32, i64, i64, i64, i64, i64, i64, i32, vp, vp, vp, sz, vp]
+        lib.tilec_linear_ce_forward.restype = ctypes.c_int
+        lib.tilec_linear_ce_backward.argtypes = [vp, vp, vp, i32, i64, i64, i64, i64, i64, i64, i32, vp, vp, vp, vp,
+                                                 vp, sz, vp]
+        lib.tilec_linear_ce_backward.restype = ctypes.c_int
+        lib.tilec_linear_ce_workspace_bytes.argtypes = [vp, vp, i32, i64, i64, i64, i64, i64, i32, i32]
+        lib.tilec_linear_ce_workspace_bytes.restype = sz
         _load_fast(lib)
         _lib = lib
         return _lib

@@ -16,6 +16,7 @@ enum : int {
   TILEC_DEV_TIMEOUT = 1,      // an mbarrier wait exceeded kWaitLimitNs
   TILEC_DEV_TMEM = 2,         // TMEM allocation returned an unexpected address
   TILEC_DEV_BAD_LAUNCH = 4,   // kernel launched with a block shape it was not built for
+  TILEC_DEV_BAD_INDEX = 8,    // a class index outside the vocabulary that is not the ignored one
 };
 
 // Defined here: the library is built as a single translation unit (tilec_mm.cu).

@@ -1,0 +1,539 @@
+// lm_ops.cuh -- host side and C ABI of the language-model operators (part of the library's
+// single translation unit, after tilec_mm.cu's own host code).
+#pragma once
+
+namespace tilec {
+namespace {
+
+// ---------------------------------------------------------------- 16-bit products
+struct LmInfo {
+  int f16_slots = 0;  // CTA pairs of tc2_f16_kernel resident at once
+  cudaError_t err = cudaSuccess;
+};
+LmInfo g_lm[kMaxDevices];
+std::once_flag g_lm_once[kMaxDevices];
+
+int lm_device(DeviceInfo** d, LmInfo** lm) {
+  const int rc = current_device(d);
+  if (rc) return rc;
+  const int dev = (*d)->dev;
+  std::call_once(g_lm_once[dev], [dev]() {
+    LmInfo& m = g_lm[dev];
+    auto acc = [&](cudaError_t e) {
+      if (m.err == cudaSuccess) m.err = e;
+    };
+    auto attr = [&](auto kern) {
+      acc(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, F16Cfg::kSmemBytes));
+    };
+    attr(tc2_f16_kernel<kEpiStats, false, true>);
+    attr(tc2_f16_kernel<kEpiProb, false, true>);
+    attr(tc2_f16_kernel<kEpiOut, false, false>);
+    attr(tc2_f16_kernel<kEpiAcc, false, false>);
+    attr(tc2_f16_kernel<kEpiOut, true, false>);
+    attr(tc2_f16_kernel<kEpiAcc, true, false>);
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim = dim3(2, 1, 1);
+    lc.blockDim = dim3(F16Cfg::kThreads);
+    lc.dynamicSmemBytes = F16Cfg::kSmemBytes;
+    cudaLaunchAttribute a;
+    a.id = cudaLaunchAttributeClusterDimension;
+    a.val.clusterDim.x = 2;
+    a.val.clusterDim.y = 1;
+    a.val.clusterDim.z = 1;
+    lc.attrs = &a;
+    lc.numAttrs = 1;
+    acc(cudaOccupancyMaxActiveClusters(&m.f16_slots, tc2_f16_kernel<kEpiOut, false, false>, &lc));
+    if (m.err == cudaSuccess && m.f16_slots < 1) m.err = cudaErrorLaunchOutOfResources;
+    cudaGetLastError();
+  });
+  if (g_lm[dev].err != cudaSuccess) return TILEC_ERR_NO_DEVICE;
+  *lm = &g_lm[dev];
+  return TILEC_OK;
+}
+
+// A 16-bit matrix of `outer` rows of `inner` elements, row stride ld (a multiple of 8, base
+// 16-byte aligned), read in boxes of 64 x box_out; out-of-range elements read as zero.
+int encode16(CUtensorMap* m, const void* base, int64_t inner, int64_t outer, int64_t ld, int box_out, bool bf16) {
+  PFN_cuTensorMapEncodeTiled_v12000 enc = get_encode();
+  if (!enc) return TILEC_ERR_NO_DEVICE;
+  cuuint64_t dims[2] = {cuuint64_t(inner), cuuint64_t(outer)};
+  cuuint64_t strides[1] = {cuuint64_t(ld) * 2};
+  cuuint32_t box[2] = {64, cuuint32_t(box_out)};
+  cuuint32_t estr[2] = {1, 1};
+  return enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+             const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+             ? TILEC_OK
+             : TILEC_ERR_BAD_ARG;
+}
+
+// One operand: M (or N) x K, stored row-major (mn = false) or as its transpose (mn = true).
+struct Op16 {
+  const void* p;
+  int64_t ld;
+  bool mn;
+};
+
+template <int EPI, bool A_MN, bool B_K>
+int launch_f16(const Op16& A, const Op16& B, int64_t M, int64_t N, int64_t K, F16Args p, const LmInfo& lm,
+               cudaStream_t s) {
+  CUtensorMap ma, mb;
+  const bool bf16 = p.bf16 != 0;
+  int rc = A_MN ? encode16(&ma, A.p, M, K, A.ld, 64, bf16) : encode16(&ma, A.p, K, M, A.ld, 128, bf16);
+  if (rc) return rc;
+  rc = B_K ? encode16(&mb, B.p, K, N, B.ld, 128, bf16) : encode16(&mb, B.p, N, K, B.ld, 64, bf16);
+  if (rc) return rc;
+  p.M = static_cast<int>(M);
+  p.N = static_cast<int>(N);
+  p.K = static_cast<int>(K);
+  p.n_tiles = static_cast<int>(cdiv(N, 256));
+  p.group_m = 8;
+  if (p.slices <= 1) {
+    p.slices = 1;
+    p.kb_per_slice = static_cast<int>(cdiv(K, F16Cfg::BK));
+  }
+  const int64_t total = cdiv(M, 256) * p.n_tiles * p.slices;
+  if (total >= (int64_t(1) << 30)) return TILEC_ERR_UNSUPPORTED;
+  const int pairs = static_cast<int>(total < lm.f16_slots ? total : lm.f16_slots);
+  return launch_k(tc2_f16_kernel<EPI, A_MN, B_K>, dim3(static_cast<unsigned>(2 * pairs)), dim3(F16Cfg::kThreads),
+                  F16Cfg::kSmemBytes, s, 2, ma, mb, p);
+}
+
+// K slices of a product of few tiles: as many as fill the CTA pairs once, each at least
+// eight stages deep.
+int f16_slices(int64_t M, int64_t N, int64_t K, const LmInfo& lm, int* kb_per_slice) {
+  const int64_t tiles = cdiv(M, 256) * cdiv(N, 256), nkb = cdiv(K, F16Cfg::BK);
+  int64_t n = lm.f16_slots / tiles;
+  if (n > nkb / 8) n = nkb / 8;
+  if (n < 1) n = 1;
+  const int64_t per = cdiv(nkb, n);
+  *kb_per_slice = static_cast<int>(per);
+  return static_cast<int>(cdiv(nkb, per));
+}
+
+// ---------------------------------------------------------------- linear cross entropy
+// Bytes of probabilities (16-bit) or logits (fp32) of one piece of the vocabulary.
+constexpr int64_t kCePieceBytes = int64_t(512) << 20;
+constexpr int64_t kCePieceMin = 4096;
+
+struct CeCall {
+  const void* x;
+  const void* w;
+  const int64_t* target;
+  int dtype;
+  int64_t T, V, D, ldx, ldw, ignore;
+  int reduction;
+};
+
+struct CePlan {
+  bool f32 = false, bf16 = false;
+  bool compact = false, pack_x = false, pack_w = false;
+  int64_t dp = 0;                // row stride of packed 16-bit operands
+  int64_t piece = 0, pieces = 0; // vocabulary entries per piece
+  int64_t ldp = 0;               // row stride of a piece's probabilities / logits
+  int64_t nblk = 0;              // partial statistics per row
+  int64_t ldacc = 0;             // row stride of fp32 sums of dx
+  int dx_slices = 1, dx_kb = 0, dw_slices = 1, dw_kb = 0;
+  size_t off_head = 0, off_rows = 0, off_x = 0, off_w = 0, off_part = 0, off_tlogit = 0, off_loss = 0, off_p = 0,
+         off_acc = 0, off_slabs = 0, off_mm = 0;
+  size_t mm_bytes = 0, bytes = 0;
+};
+
+inline bool rows_aligned16(const void* p, int64_t ld) { return aligned16(p) && ld % 8 == 0; }
+
+Problem ce_problem(const float* A, int64_t lda, const float* B, int64_t ldb, float* C, int64_t ldc, int64_t M,
+                   int64_t N, int64_t K) {
+  return single(A, B, C, M, N, K, lda, ldb, ldc);
+}
+
+size_t mm_bytes(const Problem& q, int flags) {
+  tilec_mm_cfg cfg = {};
+  cfg.flags = flags;
+  return workspace_for(q, &cfg);
+}
+
+int check_ce(const CeCall& c) {
+  if (c.dtype < TILEC_DTYPE_F32 || c.dtype > TILEC_DTYPE_BF16) return TILEC_ERR_BAD_ARG;
+  if (c.reduction < kReduceNone || c.reduction > kReduceMean) return TILEC_ERR_BAD_ARG;
+  if (c.T < 0 || c.V < 1 || c.D < 1 || c.ldx < c.D || c.ldw < c.D) return TILEC_ERR_BAD_ARG;
+  if (!c.w || (c.T > 0 && (!c.x || !c.target))) return TILEC_ERR_BAD_ARG;
+  const uintptr_t elem = c.dtype == TILEC_DTYPE_F32 ? 3 : 1;
+  if ((reinterpret_cast<uintptr_t>(c.x) & elem) || (reinterpret_cast<uintptr_t>(c.w) & elem)) return TILEC_ERR_BAD_ARG;
+  if (c.T >= (int64_t(1) << 30) || c.V >= (int64_t(1) << 30) || c.D >= (int64_t(1) << 30)) return TILEC_ERR_UNSUPPORTED;
+  return TILEC_OK;
+}
+
+// `grads`: bit 0 the gradient by x, bit 1 by w; 0 = forward.
+void plan_ce(const CeCall& c, int grads, const LmInfo& lm, CePlan* p) {
+  p->f32 = c.dtype == TILEC_DTYPE_F32;
+  p->bf16 = c.dtype == TILEC_DTYPE_BF16;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t o = at;
+    at = align256(at + bytes);
+    return o;
+  };
+  const bool bwd = grads != 0;
+  const int64_t elem = p->f32 ? 4 : 2;
+  p->piece = round_up(c.V, 256);
+  if (bwd || p->f32) {
+    int64_t fit = kCePieceBytes / (elem * c.T) / 256 * 256;
+    if (fit < kCePieceMin) fit = kCePieceMin;
+    if (p->piece > fit) {
+      p->pieces = cdiv(c.V, fit);
+      p->piece = round_up(cdiv(c.V, p->pieces), 256);
+    }
+  }
+  p->pieces = cdiv(c.V, p->piece);
+  if (p->piece > c.V) p->piece = c.V;
+  p->ldp = round_up(p->piece, 8);
+  if (!p->f32) {
+    p->dp = round_up(c.D, 8);
+    // Dropping tokens without a target pays where it can save whole 256-row tiles; the
+    // backward pass also needs their rows out of the sum over tokens.
+    p->compact = bwd || c.T > 256;
+    p->pack_x = p->compact || !rows_aligned16(c.x, c.ldx);
+    p->pack_w = !rows_aligned16(c.w, c.ldw);
+    p->off_head = take(16);
+    if (p->compact) p->off_rows = take(size_t(c.T) * 4);
+    if (p->pack_x) p->off_x = take(size_t(c.T) * p->dp * 2);
+    if (p->pack_w) p->off_w = take(size_t(c.V) * p->dp * 2);
+  }
+  if (!bwd) {
+    p->nblk = p->f32 ? p->pieces : 2 * cdiv(c.V, 256);
+    p->off_part = take(size_t(c.T) * p->nblk * 8);
+    p->off_tlogit = take(size_t(c.T) * 4);
+    if (c.reduction != kReduceNone) p->off_loss = take(size_t(c.T) * 4);
+  }
+  if (bwd || p->f32) p->off_p = take(size_t(c.T) * p->ldp * elem);
+  if (bwd && !p->f32) {
+    p->ldacc = round_up(c.D, 8);
+    size_t slabs = 0;
+    if (grads & 1) {
+      p->dx_slices = f16_slices(c.T, c.D, p->piece, lm, &p->dx_kb);
+      if (p->pieces > 1) p->off_acc = take(size_t(c.T) * p->ldacc * 4);
+      if (p->dx_slices > 1) slabs = size_t(p->dx_slices) * c.T * p->ldacc * 4;
+    }
+    if (grads & 2) {
+      p->dw_slices = f16_slices(p->piece, c.D, c.T, lm, &p->dw_kb);
+      if (p->dw_slices > 1) {
+        const size_t b = size_t(p->dw_slices) * p->piece * p->ldacc * 4;
+        if (b > slabs) slabs = b;
+      }
+    }
+    if (slabs) p->off_slabs = take(slabs);
+  }
+  if (p->f32) {
+    const float* x = static_cast<const float*>(c.x);
+    const float* w = static_cast<const float*>(c.w);
+    const int64_t dz = round_up(c.D, 4);
+    if (grads & 2) p->off_x = take(size_t(c.T) * dz * 4);
+    if ((grads & 1) && p->pieces > 1) p->off_acc = take(size_t(c.T) * c.D * 4);
+    const int64_t last = c.V - (p->pieces - 1) * p->piece;
+    for (int64_t n : {p->piece, last}) {
+      size_t b = mm_bytes(ce_problem(x, c.ldx, w, c.ldw, nullptr, p->ldp, c.T, n, c.D), TILEC_MM_TRANS_B);
+      if (b > p->mm_bytes) p->mm_bytes = b;
+      if (grads & 1) {
+        b = mm_bytes(ce_problem(nullptr, p->ldp, w, c.ldw, nullptr, c.D, c.T, c.D, n), 0);
+        if (b > p->mm_bytes) p->mm_bytes = b;
+      }
+      if (grads & 2) {
+        b = mm_bytes(ce_problem(nullptr, p->ldp, nullptr, dz, nullptr, c.D, n, c.D, c.T), TILEC_MM_TRANS_A);
+        if (b > p->mm_bytes) p->mm_bytes = b;
+      }
+    }
+    if (p->mm_bytes) p->off_mm = take(p->mm_bytes);
+  }
+  p->bytes = at;
+}
+
+int pack16(const void* src, int64_t lds, void* dst, int64_t ldd, int64_t nrows, int64_t cols, const int* rows,
+           const int* count, const int64_t* target, int64_t ignore, void* zero_rows, const DeviceInfo& d,
+           cudaStream_t s) {
+  int64_t blocks = cdiv(nrows, 8);
+  if (blocks > int64_t(d.sms) * 32) blocks = int64_t(d.sms) * 32;
+  return launch_k(pack16_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, 1,
+                  static_cast<const unsigned short*>(src), lds, static_cast<unsigned short*>(dst), ldd, nrows, cols,
+                  rows, count, rows_aligned16(src, lds) ? 1 : 0, target, ignore,
+                  static_cast<unsigned short*>(zero_rows));
+}
+
+int run_mm(const Problem& q, int flags, uint8_t* ws, const CePlan& p, cudaStream_t s) {
+  tilec_mm_cfg cfg = {};
+  cfg.flags = flags;
+  return run_problem(q, &cfg, p.mm_bytes ? ws + p.off_mm : nullptr, p.mm_bytes, s);
+}
+
+#define TILEC_TRY(expr)            \
+  do {                             \
+    const int rc_ = (expr);        \
+    if (rc_) return rc_;           \
+  } while (0)
+
+int check_ws(const CePlan& p, void* ws, size_t ws_bytes) {
+  return p.bytes > 0 && (!ws || ws_bytes < p.bytes || (reinterpret_cast<uintptr_t>(ws) & 255u) != 0)
+             ? TILEC_ERR_WORKSPACE
+             : TILEC_OK;
+}
+
+int ce_forward(const CeCall& c, float* loss, float* stats_buf, void* workspace, size_t ws_bytes, cudaStream_t s) {
+  DeviceInfo* d = nullptr;
+  LmInfo* lm = nullptr;
+  TILEC_TRY(lm_device(&d, &lm));
+  float2* stats = reinterpret_cast<float2*>(stats_buf);
+  float* count_out = stats_buf + 2 * c.T;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  if (c.T == 0) {
+    if (c.reduction == kReduceNone) return TILEC_OK;
+    return launch_k(ce_reduce_kernel, dim3(1), dim3(1024), 0, s, 1, static_cast<const float*>(nullptr), int64_t(0),
+                    c.target, c.ignore, c.reduction, loss, count_out);
+  }
+  CePlan p;
+  plan_ce(c, 0, *lm, &p);
+  TILEC_TRY(check_ws(p, workspace, ws_bytes));
+  float2* part = reinterpret_cast<float2*>(ws + p.off_part);
+  float* tlogit = reinterpret_cast<float*>(ws + p.off_tlogit);
+  float* losses = c.reduction == kReduceNone ? loss : reinterpret_cast<float*>(ws + p.off_loss);
+  int* head = reinterpret_cast<int*>(ws + p.off_head);
+  int* rows = p.compact ? reinterpret_cast<int*>(ws + p.off_rows) : nullptr;
+  const int* count = p.compact ? head : nullptr;
+  if (p.f32) {
+    float* l = reinterpret_cast<float*>(ws + p.off_p);
+    for (int64_t i = 0; i < p.pieces; ++i) {
+      const int64_t v0 = i * p.piece, n = c.V - v0 < p.piece ? c.V - v0 : p.piece;
+      TILEC_TRY(run_mm(ce_problem(static_cast<const float*>(c.x), c.ldx, static_cast<const float*>(c.w) + v0 * c.ldw,
+                                  c.ldw, l, p.ldp, c.T, n, c.D),
+                       TILEC_MM_TRANS_B, ws, p, s));
+      TILEC_TRY(launch_k(ce_stats_f32_kernel, dim3(static_cast<unsigned>(c.T)), dim3(256), 0, s, 1, l, p.ldp, n, v0,
+                         c.target, part, static_cast<int>(p.nblk), static_cast<int>(i), tlogit));
+    }
+  } else {
+    const void* x = c.x;
+    const void* w = c.w;
+    int64_t ldx = c.ldx, ldw = c.ldw;
+    if (p.compact)
+      TILEC_TRY(launch_k(ce_select_kernel, dim3(1), dim3(1024), 0, s, 1, c.target, c.T, c.ignore, rows,
+                         reinterpret_cast<float*>(head), static_cast<float*>(nullptr),
+                         static_cast<const float*>(nullptr), static_cast<const float*>(nullptr), c.reduction, 0));
+    if (p.pack_x) {
+      TILEC_TRY(pack16(c.x, c.ldx, ws + p.off_x, p.dp, c.T, c.D, rows, count, nullptr, 0, nullptr, *d, s));
+      x = ws + p.off_x;
+      ldx = p.dp;
+    }
+    if (p.pack_w) {
+      TILEC_TRY(pack16(c.w, c.ldw, ws + p.off_w, p.dp, c.V, c.D, nullptr, nullptr, nullptr, 0, nullptr, *d, s));
+      w = ws + p.off_w;
+      ldw = p.dp;
+    }
+    F16Args a = {};
+    a.bf16 = p.bf16;
+    a.count = count;
+    a.rows = rows;
+    a.part = part;
+    a.tlogit = tlogit;
+    a.target = c.target;
+    TILEC_TRY((launch_f16<kEpiStats, false, true>(Op16{x, ldx, false}, Op16{w, ldw, false}, c.T, c.V, c.D, a, *lm, s)));
+  }
+  TILEC_TRY(launch_k(ce_join_kernel, dim3(static_cast<unsigned>(cdiv(c.T, 8))), dim3(256), 0, s, 1, part,
+                     static_cast<int>(p.nblk), c.T, c.V, c.target, c.ignore, rows, count, tlogit, stats, losses));
+  if (c.reduction == kReduceNone) return TILEC_OK;
+  return launch_k(ce_reduce_kernel, dim3(1), dim3(1024), 0, s, 1, losses, c.T, c.target, c.ignore, c.reduction, loss,
+                  count_out);
+}
+
+int ce_backward_f32(const CeCall& c, const CePlan& p, const float* stats_buf, const float* grad, float* dx, float* dw,
+                    uint8_t* ws, const DeviceInfo& d, cudaStream_t s) {
+  const float2* stats = reinterpret_cast<const float2*>(stats_buf);
+  const float* count = stats_buf + 2 * c.T;
+  float* l = reinterpret_cast<float*>(ws + p.off_p);
+  float* xz = reinterpret_cast<float*>(ws + p.off_x);
+  float* sums = reinterpret_cast<float*>(ws + p.off_acc);
+  const int64_t dz = round_up(c.D, 4);
+  const unsigned row_blocks = static_cast<unsigned>(c.T < int64_t(d.sms) * 16 ? c.T : int64_t(d.sms) * 16);
+  const float* x = static_cast<const float*>(c.x);
+  if (dw)
+    TILEC_TRY(launch_k(ce_mask_rows_f32_kernel, dim3(row_blocks), dim3(256), 0, s, 1, x, c.ldx, xz, dz, c.T, c.D,
+                       c.target, c.ignore));
+  for (int64_t i = 0; i < p.pieces; ++i) {
+    const int64_t v0 = i * p.piece, n = c.V - v0 < p.piece ? c.V - v0 : p.piece;
+    const float* w = static_cast<const float*>(c.w) + v0 * c.ldw;
+    TILEC_TRY(run_mm(ce_problem(x, c.ldx, w, c.ldw, l, p.ldp, c.T, n, c.D), TILEC_MM_TRANS_B, ws, p, s));
+    TILEC_TRY(launch_k(ce_prob_f32_kernel, dim3(static_cast<unsigned>(c.T)), dim3(256), 0, s, 1, l, p.ldp, n, v0,
+                       c.target, c.ignore, stats, grad, count, c.reduction));
+    if (dx) {
+      TILEC_TRY(run_mm(ce_problem(l, p.ldp, w, c.ldw, i == 0 ? dx : sums, c.D, c.T, c.D, n), 0, ws, p, s));
+      const int last = i == p.pieces - 1;
+      if (i > 0 || last)
+        TILEC_TRY(launch_k(ce_finish_dx_f32_kernel, dim3(row_blocks), dim3(256), 0, s, 1, dx,
+                           static_cast<const float*>(i > 0 ? sums : nullptr), c.T, c.D, c.target, c.ignore, last));
+    }
+    if (dw)
+      TILEC_TRY(run_mm(ce_problem(l, p.ldp, xz, dz, dw + v0 * c.D, c.D, n, c.D, c.T), TILEC_MM_TRANS_A, ws, p, s));
+  }
+  return TILEC_OK;
+}
+
+// One gradient product of a piece: with K slices through slabs, and (dx over several pieces)
+// through fp32 sums of the earlier pieces.
+template <bool A_MN>
+int ce_grad_product(const Op16& A, const Op16& B, int64_t M, int64_t N, int64_t K, F16Args a, int slices, int kb,
+                    const float* acc_in, float* acc_out, void* out, float* slabs, const CePlan& p,
+                    const LmInfo& lm, const DeviceInfo& d, cudaStream_t s) {
+  const int vec = aligned16(out) && N % 8 == 0;
+  a.slices = slices;
+  a.kb_per_slice = kb;
+  if (slices > 1) {
+    F16Args b = a;
+    b.out = slabs;
+    b.ldo = p.ldacc;
+    b.slab = M * p.ldacc;
+    b.acc = nullptr;
+    TILEC_TRY((launch_f16<kEpiAcc, A_MN, false>(A, B, M, N, K, b, lm, s)));
+    int64_t blocks = cdiv(M * cdiv(N, 8), 256);
+    if (blocks > int64_t(d.sms) * 8) blocks = int64_t(d.sms) * 8;
+    return launch_k(f16_join_slabs_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, 1,
+                    static_cast<const float*>(slabs), slices, b.slab, p.ldacc, acc_in, acc_out,
+                    static_cast<unsigned short*>(out), N, M, N, a.count_is_k ? nullptr : a.count, a.rows, a.scale,
+                    a.scale2, a.bf16, vec);
+  }
+  a.acc = acc_in;
+  a.ldacc = p.ldacc;
+  if (out == nullptr) {
+    a.out = acc_out;
+    a.ldo = p.ldacc;
+    return launch_f16<kEpiAcc, A_MN, false>(A, B, M, N, K, a, lm, s);
+  }
+  a.out = out;
+  a.ldo = N;
+  a.vec_out = vec;
+  return launch_f16<kEpiOut, A_MN, false>(A, B, M, N, K, a, lm, s);
+}
+
+int ce_backward(const CeCall& c, const float* stats_buf, const float* grad, void* dx, void* dw, void* workspace,
+                size_t ws_bytes, cudaStream_t s) {
+  const int grads = (dx ? 1 : 0) | (dw ? 2 : 0);
+  if (grads == 0) return TILEC_OK;
+  DeviceInfo* d = nullptr;
+  LmInfo* lm = nullptr;
+  TILEC_TRY(lm_device(&d, &lm));
+  if (c.T == 0) {
+    if (!dw) return TILEC_OK;
+    return cudaMemsetAsync(dw, 0, size_t(c.V) * c.D * (c.dtype == TILEC_DTYPE_F32 ? 4 : 2), s) == cudaSuccess
+               ? TILEC_OK
+               : TILEC_ERR_LAUNCH;
+  }
+  CePlan p;
+  plan_ce(c, grads, *lm, &p);
+  TILEC_TRY(check_ws(p, workspace, ws_bytes));
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  if (p.f32)
+    return ce_backward_f32(c, p, stats_buf, grad, static_cast<float*>(dx), static_cast<float*>(dw), ws, *d, s);
+
+  float* head = reinterpret_cast<float*>(ws + p.off_head);
+  const int* count = reinterpret_cast<const int*>(head);
+  float* scale = head + 2;
+  int* rows = reinterpret_cast<int*>(ws + p.off_rows);
+  TILEC_TRY(launch_k(ce_select_kernel, dim3(1), dim3(1024), 0, s, 1, c.target, c.T, c.ignore, rows, head, scale, grad,
+                     stats_buf + 2 * c.T, c.reduction, p.bf16 ? 0 : 1));
+  void* xc = ws + p.off_x;
+  TILEC_TRY(pack16(c.x, c.ldx, xc, p.dp, c.T, c.D, rows, count, c.target, c.ignore, dx, *d, s));
+  const void* w = c.w;
+  int64_t ldw = c.ldw;
+  if (p.pack_w) {
+    TILEC_TRY(pack16(c.w, c.ldw, ws + p.off_w, p.dp, c.V, c.D, nullptr, nullptr, nullptr, 0, nullptr, *d, s));
+    w = ws + p.off_w;
+    ldw = p.dp;
+  }
+  // fp16 probabilities are held times 2^15 (the largest magnitude is then 2^15): a token's
+  // share 2^-24 of the probability would otherwise already be a subnormal.
+  const float pscale = p.bf16 ? 1.f : 32768.f;
+  for (int64_t i = 0; i < p.pieces; ++i) {
+    const int64_t v0 = i * p.piece, n = c.V - v0 < p.piece ? c.V - v0 : p.piece;
+    const void* wi = static_cast<const unsigned short*>(w) + v0 * ldw;
+    void* prob = ws + p.off_p;
+    F16Args a = {};
+    a.bf16 = p.bf16;
+    a.count = count;
+    a.rows = rows;
+    a.target = c.target;
+    a.stats = reinterpret_cast<const float2*>(stats_buf);
+    a.grad = c.reduction == kReduceNone ? grad : nullptr;
+    a.head = head;
+    a.pscale = pscale;
+    a.m_alloc = static_cast<int>(c.T);
+    a.col0 = static_cast<int>(v0);
+    a.out = prob;
+    a.ldo = p.ldp;
+    TILEC_TRY((launch_f16<kEpiProb, false, true>(Op16{xc, p.dp, false}, Op16{wi, ldw, false}, c.T, n, c.D, a, *lm, s)));
+    F16Args g = {};
+    g.bf16 = p.bf16;
+    g.count = count;
+    g.scale = scale;
+    g.scale2 = 1.f / pscale;
+    float* slabs = reinterpret_cast<float*>(ws + p.off_slabs);
+    if (dx) {
+      const bool last = i == p.pieces - 1;
+      float* acc = reinterpret_cast<float*>(ws + p.off_acc);
+      g.rows = rows;
+      TILEC_TRY((ce_grad_product<false>(Op16{prob, p.ldp, false}, Op16{wi, ldw, true}, c.T, c.D, n, g, p.dx_slices,
+                                        p.dx_kb, i > 0 ? acc : nullptr, acc, last ? dx : nullptr, slabs, p, *lm, *d,
+                                        s)));
+    }
+    if (dw) {
+      g.rows = nullptr;
+      g.count_is_k = 1;
+      TILEC_TRY((ce_grad_product<true>(Op16{prob, p.ldp, true}, Op16{xc, p.dp, true}, n, c.D, c.T, g, p.dw_slices,
+                                       p.dw_kb, nullptr, nullptr, static_cast<unsigned short*>(dw) + v0 * c.D, slabs,
+                                       p, *lm, *d, s)));
+    }
+  }
+  return TILEC_OK;
+}
+
+CeCall ce_call(const void* x, const void* w, const int64_t* target, int32_t dtype, int64_t T, int64_t V, int64_t D,
+               int64_t ldx, int64_t ldw, int64_t ignore, int32_t reduction) {
+  return CeCall{x, w, target, dtype, T, V, D, ldx, ldw, ignore, reduction};
+}
+
+}  // namespace
+}  // namespace tilec
+
+extern "C" {
+
+size_t tilec_linear_ce_workspace_bytes(const void* x, const void* w, int32_t dtype, int64_t T, int64_t V, int64_t D,
+                                       int64_t ldx, int64_t ldw, int32_t reduction, int32_t grads) {
+  static const int64_t kSome = 0;
+  const CeCall c = ce_call(x ? x : reinterpret_cast<const void*>(256), w ? w : reinterpret_cast<const void*>(256),
+                           &kSome, dtype, T, V, D, ldx, ldw, 0, reduction);
+  if (check_ce(c) || T == 0 || grads < 0 || grads > 3) return 0;
+  DeviceInfo* d = nullptr;
+  LmInfo* lm = nullptr;
+  if (lm_device(&d, &lm)) return 0;
+  CePlan p;
+  plan_ce(c, grads, *lm, &p);
+  return p.bytes;
+}
+
+int tilec_linear_ce_forward(const void* x, const void* w, const int64_t* target, int32_t dtype, int64_t T, int64_t V,
+                            int64_t D, int64_t ldx, int64_t ldw, int64_t ignore_index, int32_t reduction, float* loss,
+                            float* stats, void* workspace, size_t ws_bytes, void* stream) {
+  const CeCall c = ce_call(x, w, target, dtype, T, V, D, ldx, ldw, ignore_index, reduction);
+  const int rc = check_ce(c);
+  if (rc) return rc;
+  if (!stats || (!loss && (T > 0 || reduction != kReduceNone))) return TILEC_ERR_BAD_ARG;
+  return ce_forward(c, loss, stats, workspace, ws_bytes, static_cast<cudaStream_t>(stream));
+}
+
+int tilec_linear_ce_backward(const void* x, const void* w, const int64_t* target, int32_t dtype, int64_t T, int64_t V,
+                             int64_t D, int64_t ldx, int64_t ldw, int64_t ignore_index, int32_t reduction,
+                             const float* stats, const float* grad, void* dx, void* dw, void* workspace,
+                             size_t ws_bytes, void* stream) {
+  const CeCall c = ce_call(x, w, target, dtype, T, V, D, ldx, ldw, ignore_index, reduction);
+  const int rc = check_ce(c);
+  if (rc) return rc;
+  if (!stats || (!grad && (T > 0 || reduction != kReduceNone))) return TILEC_ERR_BAD_ARG;
+  return ce_backward(c, stats, grad, dx, dw, workspace, ws_bytes, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

@@ -26,9 +26,12 @@
 #include "tc2_gemm.cuh"
 #include "tc2_sk.cuh"
 #include "tc2_tf32p.cuh"
+#include "tc2_f16.cuh"
+#include "linear_ce.cuh"
 
 static_assert(TILEC_DEV_STATUS_TIMEOUT == tilec::TILEC_DEV_TIMEOUT && TILEC_DEV_STATUS_TMEM == tilec::TILEC_DEV_TMEM &&
-                  TILEC_DEV_STATUS_BAD_LAUNCH == tilec::TILEC_DEV_BAD_LAUNCH,
+                  TILEC_DEV_STATUS_BAD_LAUNCH == tilec::TILEC_DEV_BAD_LAUNCH &&
+                  TILEC_DEV_STATUS_BAD_INDEX == tilec::TILEC_DEV_BAD_INDEX,
               "status bits in include/tilec_mm.h match the device enum");
 static_assert(TILEC_MM_TRANS_A == tilec::kOpAMN && TILEC_MM_TRANS_B == tilec::kOpBK,
               "cfg->flags are passed to the kernels as their operand layout");
@@ -1501,3 +1504,6 @@ extern "C" int tilec_mm_f32_splitk_noalloc(const float* A, const float* B, float
   r.split = static_cast<int>(split);
   return launch_reduce(r, *d, s);
 }
+
+// ------------------------------------------------------------------ language-model operators
+#include "lm_ops.cuh"
