@@ -304,6 +304,28 @@ TILEC_API size_t tilec_linear_ce_workspace_bytes(const void* x, const void* w, i
                                                  int64_t D, int64_t ldx, int64_t ldw, int32_t reduction,
                                                  int32_t grads);
 
+/* Product with 4-bit weights:
+ *   out[m, n] = sum_k x[m, k] * (code[n, k] - zero[n, k / group]) * scale[n, k / group] + bias[n]
+ * x [M, K] (row stride ldx), bias [N] (or NULL) and out [M, N] (row stride ldo) of `dtype`,
+ * scale of scale_dtype, zero 0..15 (NULL: 8 everywhere).  group: 32, 64 or a multiple of 128.
+ * Layouts, with B = ceil(K / 128):
+ *   codes   [N][B][64 bytes], 16-byte aligned.  As 32-bit little-endian words, word 4t + j
+ *           (t, j = 0..3) of a block holds k = 32j + 8t + 0..7 of its 128: k = 2i in bits
+ *           4i..4i+3, k = 2i + 1 in bits 4i+16..4i+19 (i = 0..3).  k >= K: any code.
+ *   scales  [ceil(128 * B / group)][N], zeros likewise; groups past K: any finite scale.
+ * Codes, zero points and scales enter exactly and sums are fp32, except for more than 32
+ * rows (fp32: 10), where the weight (code - zero) * scale is rounded once to dtype and
+ * multiplied on the tensor cores (fp32: the 3xTF32 product).
+ * Workspace: tilec_mm_w4_workspace_bytes (at most 256 MiB of expanded weights or 256 rows). */
+TILEC_API int tilec_mm_w4(const void* x, int32_t dtype, int64_t M, int64_t ldx, const void* codes,
+                          const void* scales, int32_t scale_dtype, const uint8_t* zeros, int64_t N, int64_t K,
+                          int64_t group, const void* bias, void* out, int64_t ldo, void* workspace,
+                          size_t ws_bytes, void* stream);
+
+/* Workspace bytes of tilec_mm_w4 (NULL x or out: assumed 16-byte aligned). */
+TILEC_API size_t tilec_mm_w4_workspace_bytes(const void* x, int32_t dtype, int64_t M, int64_t ldx, int64_t N,
+                                             int64_t K, int64_t group, const void* out, int64_t ldo);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,364 @@
+"""4-bit weights: packing, quantising and refusals (CPU), matrix_mul_w4 against 64 bits (GPU).
+
+Element-wise bounds, u = half a unit in the last place (2^-8 bf16, 2^-11 fp16, 2^-24 fp32) and
+S = sum_k |x (code - zero) scale|:
+
+* up to 32 rows (fp32: 10): products of codes and x are exact; a 128-k block adds 8 groups of
+  16 products to an accumulator, each sum truncated at worst (16 * 2^-23 S), and the at most
+  64 blocks are added in fp32 (64 * 2^-24 S), the scale's product rounds once: below
+  2^-18 S; then one rounding, u |y|.
+* more rows: the weight is rounded to the type, u S more (fp32: the 3xTF32 product,
+  3 * 2^-20 S); sums over K <= 8192 in the tensor cores' fp32 stay below 2^-14 S (K / 16 sums,
+  each truncated by 2^-23).
+* fp16 results below 2^-14 are multiples of 2^-24: 2^-25 absolute.
+"""
+import pytest
+import torch
+
+from tilec_b200 import ext
+
+DT = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+U = {"bf16": 2.0 ** -8, "f16": 2.0 ** -11, "f32": 2.0 ** -24}
+
+
+def _make(m, n, k, group, dtype, zeros=True, bias=False, sdtype=None, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    groups = -(-k // group)
+    codes = torch.randint(0, 16, (n, k), generator=g, dtype=torch.uint8)
+    scales = ((torch.rand(n, groups, generator=g) + 0.1) * k ** -0.5 / 4).to(DT[sdtype or dtype])
+    z = torch.randint(0, 16, (n, groups), generator=g, dtype=torch.uint8) if zeros else None
+    x = torch.randn(m, k, generator=g).to(DT[dtype])
+    b = torch.randn(n, generator=g).to(DT[dtype]) if bias else None
+    return x, codes, scales, z, b
+
+
+def _weight64(codes, scales, zeros, group):
+    k = codes.shape[1]
+    s = scales.double().repeat_interleave(group, 1)[:, :k]
+    z = 8.0 if zeros is None else zeros.double().repeat_interleave(group, 1)[:, :k]
+    return (codes.double() - z) * s
+
+
+def _bound(x, w, y, dtype, rows):
+    s = x.double().abs() @ w.abs().t()
+    few = rows * (3 if dtype == "f32" else 1) <= 32
+    rel = 2.0 ** -18 if few else 2.0 ** -14 + (3 * 2.0 ** -20 if dtype == "f32" else U[dtype])
+    return rel * s + 1.001 * U[dtype] * y.abs() + (2.0 ** -25 if dtype == "f16" else 0.0)
+
+
+def _check(x, codes, scales, zeros, bias, group, dtype, call=None):
+    w = _weight64(codes, scales, zeros, group)
+    y = x.double() @ w.t()
+    tol = _bound(x, w, y, dtype, len(x))
+    if bias is not None:
+        y = y + bias.double()
+        tol = tol + U[dtype] * y.abs() + 2.0 ** -23 * bias.double().abs()
+    weight = ext.pack_w4(codes, scales, zeros, group).to("cuda")
+    got = (call or ext.matrix_mul_w4)(x.cuda(), weight, None if bias is None else bias.cuda())
+    assert got.dtype == x.dtype and got.shape == y.shape
+    err = (got.cpu().double() - y).abs()
+    assert torch.isfinite(got).all()
+    assert (err <= tol).all(), f"worst {(err / tol.clamp(min=1e-300)).max():.2f} of the bound"
+    ext.check_device()
+
+
+# ---------------------------------------------------------------- CPU
+@pytest.mark.parametrize("group", [32, 64, 128, 256])
+@pytest.mark.parametrize("n,k", [(1, 1), (5, 300), (3, 128), (16, 513)])
+def test_pack_keeps_codes_and_values(n, k, group):
+    _, codes, scales, zeros, _ = _make(1, n, k, group, "f32")
+    w = ext.pack_w4(codes, scales, zeros, group)
+    assert torch.equal(w.unpack(), codes)
+    assert torch.equal(w.dequantize().double(), _weight64(codes, scales, zeros, group).float().double())
+    # the layout of include/tilec_mm.h, word by word
+    words = w.codes.view(n, -1, 16, 4).long()
+    words = words[..., 0] | words[..., 1] << 8 | words[..., 2] << 16 | words[..., 3] << 24
+    blocks = -(-k // 128)
+    full = torch.nn.functional.pad(codes, (0, blocks * 128 - k)).view(n, blocks, 128).long()
+    for t in range(4):
+        for j in range(4):
+            for i in range(4):
+                for odd in range(2):
+                    assert torch.equal(words[:, :, 4 * t + j] >> (4 * i + 16 * odd) & 15,
+                                       full[:, :, 32 * j + 8 * t + 2 * i + odd])
+    assert w.scales.shape == (-(-blocks * 128 // group), n)
+    assert torch.isfinite(w.scales).all()
+
+
+@pytest.mark.parametrize("symmetric", [False, True])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("group", [32, 128])
+def test_quantize_error_is_half_a_step(group, dtype, symmetric):
+    g = torch.Generator().manual_seed(1)
+    w = torch.randn(24, 300, generator=g).to(DT[dtype])
+    w[3] = 0                       # a group of zeros
+    w[4] = w[4].abs() + 1          # all positive: the range is widened to hold zero
+    q = ext.quantize_w4(w, group, symmetric)
+    step = q.scales.t().float().repeat_interleave(group, 1)[:, :300]
+    err = (q.dequantize() - w.float()).abs()
+    # the rounded scale spans 15 (7) steps short by up to 15 u (7 u) of a step at the ends,
+    # and the zero point is rounded to a step
+    slack = 15 * U[dtype] + 2.0 ** -20
+    assert (err <= (0.5 + (0 if symmetric else 0.5) + slack) * step + 1e-30).all()
+    assert (q.dequantize()[3] == 0).all()
+    assert q.shape == (24, 300) and (q.zeros is None) == symmetric
+
+
+def test_refusals():
+    c, s = torch.zeros(4, 64, dtype=torch.uint8), torch.ones(4, 2)
+    for bad in (0, 16, 48, 96, 160, -128, 32.0):
+        with pytest.raises(ValueError, match="group_size"):
+            ext.pack_w4(c, s, group_size=bad)
+        with pytest.raises(ValueError, match="group_size"):
+            ext.quantize_w4(torch.ones(4, 64), bad)
+    with pytest.raises(TypeError, match="uint8"):
+        ext.pack_w4(c.int(), s, group_size=32)
+    with pytest.raises(ValueError, match="scales have shape"):
+        ext.pack_w4(c, s, group_size=64)
+    with pytest.raises(TypeError, match="scales must be"):
+        ext.pack_w4(c, s.double(), group_size=32)
+    with pytest.raises(ValueError, match="zeros have shape"):
+        ext.pack_w4(c, s, c[:, :1], group_size=32)
+    with pytest.raises(TypeError, match="zeros must be"):
+        ext.pack_w4(c, s, s, group_size=32)
+    with pytest.raises(ValueError, match="0..15"):
+        ext.pack_w4(c + 16, s, group_size=32)
+    with pytest.raises(ValueError, match="K >= 1"):
+        ext.pack_w4(c[:, :0], s, group_size=32)
+    with pytest.raises(TypeError, match="weight must be"):
+        ext.quantize_w4(torch.ones(4, 64, dtype=torch.float64))
+    w = ext.pack_w4(c, s, group_size=32)
+    x = torch.ones(2, 64)
+    with pytest.raises(TypeError, match="W4Weight"):
+        ext.matrix_mul_w4(x, c)
+    with pytest.raises(ValueError, match="don't match"):
+        ext.matrix_mul_w4(x[:, :63], w)
+    with pytest.raises(TypeError, match="x must be"):
+        ext.matrix_mul_w4(x.double(), w)
+    with pytest.raises(ValueError, match="CUDA"):
+        ext.matrix_mul_w4(x, w)
+
+
+def test_abi_refusals():
+    from tilec_b200 import _native
+    lib = _native.load()
+    ok = dict(x=256, dtype=2, M=2, ldx=64, codes=256, scales=256, sdt=2, zeros=None, N=8, K=64, group=32, bias=None,
+              out=256, ldo=8)
+
+    def call(**kw):
+        return lib.tilec_mm_w4(*{**ok, **kw}.values(), None, 0, None)
+
+    for bad in (dict(dtype=3), dict(sdt=-1), dict(M=-1), dict(N=-1), dict(K=0), dict(ldx=63), dict(group=16),
+                dict(group=0), dict(group=192), dict(x=None), dict(codes=None), dict(scales=None), dict(out=None),
+                dict(ldo=7), dict(codes=264), dict(x=257), dict(out=257), dict(bias=257), dict(scales=257),
+                dict(sdt=0, scales=258)):
+        assert call(**bad) == 1, bad
+    assert call(M=1 << 31) == 7
+    assert call(M=0, x=None, out=None) == 0 and call(N=0, codes=None, scales=None, ldo=0) == 0
+    assert lib.tilec_mm_w4_workspace_bytes(None, 9, 2, 64, 8, 64, 32, None, 8) == 0
+
+
+# ---------------------------------------------------------------- GPU
+gpu = pytest.mark.gpu
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("group", [32, 64, 128, 256])
+@pytest.mark.parametrize("n,k", [(1, 1), (7, 31), (16, 128), (33, 300), (100, 1024), (130, 4100)])
+def test_one_token(n, k, group, dtype):
+    _check(*_make(1, n, k, group, dtype), group, dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("m", [2, 3, 8, 9, 10, 11, 16, 17, 32, 33, 65, 257])
+def test_rows(m, dtype):
+    """Either side of each variant's row count, with bias, symmetric and with zero points."""
+    for zeros, group, n, k in ((True, 32, 90, 640), (False, 128, 259, 1157)):
+        _check(*_make(m, n, k, group, dtype, zeros=zeros, bias=True, seed=m), group, dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("sdtype", ["bf16", "f16", "f32"])
+def test_scale_types(sdtype, dtype):
+    for m in (1, 40):
+        _check(*_make(m, 70, 384, 64, dtype, sdtype=sdtype), 64, dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("m,n,k", [(1, 16, 8192), (5, 4096, 512), (1, 300, 8190), (40, 520, 8192), (300, 700, 2048)])
+def test_long_sums_and_many_tiles(m, n, k, dtype):
+    _check(*_make(m, n, k, 128, dtype), 128, dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+def test_exact_values(dtype):
+    """Small whole numbers: every product and sum is exact, so the result is too."""
+    g = torch.Generator().manual_seed(3)
+    for m in (1, 6, 50):
+        codes = torch.randint(0, 16, (75, 384), generator=g, dtype=torch.uint8)
+        scales = torch.randint(1, 3, (75, 12), generator=g).to(DT[dtype])
+        zeros = torch.randint(0, 16, (75, 12), generator=g, dtype=torch.uint8)
+        x = torch.zeros(m, 384)
+        x[:, torch.randperm(384, generator=g)[:8]] = torch.randint(-2, 3, (m, 8), generator=g).float()
+        w = ext.pack_w4(codes, scales, zeros, 32).to("cuda")
+        got = ext.matrix_mul_w4(x.to(DT[dtype]).cuda(), w).cpu().double()
+        want = x.double() @ _weight64(codes, scales, zeros, 32).t()
+        assert torch.equal(got, want.to(DT[dtype]).double())
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("m", [3, 40])
+def test_strides_out_and_shapes(m, dtype):
+    x, codes, scales, zeros, bias = _make(m, 200, 320, 64, dtype, bias=True)
+    w = ext.pack_w4(codes, scales, zeros, 64).to("cuda")
+    x, bias = x.cuda(), bias.cuda()
+    base = ext.matrix_mul_w4(x, w, bias)
+    for off in (0, 1, 8):   # row views, off a 16-byte boundary too; what lies beside them is NaN
+        wide = torch.full((m, 400), float("nan"), dtype=x.dtype, device="cuda")
+        wide[:, off:off + 320] = x
+        got = ext.matrix_mul_w4(wide[:, off:off + 320], w, bias)
+        if dtype == "f32" and m > 10:   # the fp32 product picks its kernel by alignment
+            torch.testing.assert_close(got, base, rtol=1e-5, atol=1e-4)
+        else:
+            assert torch.equal(got, base)
+    assert torch.equal(ext.matrix_mul_w4(x.t().contiguous().t(), w, bias), base)
+    assert torch.equal(ext.matrix_mul_w4(x.view(1, m, 320), w, bias), base.view(1, m, 200))
+    assert ext.matrix_mul_w4(x[0], w, bias).shape == (200,)
+    for off in (0, 3):      # a wider out: its other columns stay as they were
+        buf = torch.full((m, 260), 7.0, dtype=x.dtype, device="cuda")
+        view = buf[:, off:off + 200]
+        assert ext.matrix_mul_w4(x, w, bias, out=view) is view
+        if dtype == "f32" and m > 10:
+            torch.testing.assert_close(view, base, rtol=1e-5, atol=1e-4)
+        else:
+            assert torch.equal(view, base)
+        assert (buf[:, :off] == 7).all() and (buf[:, off + 200:] == 7).all()
+    for bad in (base.float() if dtype != "f32" else base.half(), base[:, :-1], base.t().contiguous().t(), base.cpu()):
+        with pytest.raises(ValueError, match="out must"):
+            ext.matrix_mul_w4(x, w, bias, out=bad)
+    with pytest.raises(ValueError, match="bias must"):
+        ext.matrix_mul_w4(x, w, bias[:-1])
+    with pytest.raises(ValueError, match="not differentiable"):
+        ext.matrix_mul_w4(x.clone().requires_grad_(True), w)
+    with pytest.raises(ValueError, match="one CUDA device"):
+        ext.matrix_mul_w4(x, w.to("cpu"))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_empty(dtype):
+    x, codes, scales, zeros, _ = _make(0, 20, 64, 32, dtype)
+    w = ext.pack_w4(codes, scales, zeros, 32).to("cuda")
+    assert ext.matrix_mul_w4(x.cuda(), w).shape == (0, 20)
+    w = ext.pack_w4(codes[:0], scales[:0], zeros[:0], 32).to("cuda")
+    assert ext.matrix_mul_w4(torch.ones(3, 64, dtype=DT[dtype], device="cuda"), w).shape == (3, 0)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("m", [2, 9, 40])
+def test_not_finite_values_stay_in_their_row(m, dtype):
+    x, codes, scales, zeros, _ = _make(m, 150, 256, 64, dtype)
+    w = ext.pack_w4(codes, scales, zeros, 64).to("cuda")
+    x = x.cuda()
+    base = ext.matrix_mul_w4(x, w)
+    bad = x.clone()
+    bad[0, 17], bad[1, 40] = float("inf"), float("nan")
+    got = ext.matrix_mul_w4(bad, w)
+    assert not torch.isfinite(got[0]).any() or (codes[:, 17] == zeros[:, 0]).any()
+    value = codes[:, 17].int() - zeros[:, 0].int()
+    assert torch.isnan(got[1]).all()
+    assert (~torch.isfinite(got[0].cpu()))[value != 0].all()
+    assert torch.equal(got[2:], base[2:])
+
+
+@gpu
+@pytest.mark.parametrize("m", [1, 40])
+def test_streams_and_graphs(m):
+    """Two graphs replayed at once on two streams with new inputs; repeats give the same bits."""
+    sets = []
+    for seed in (1, 2):
+        x, codes, scales, zeros, _ = _make(m, 500, 3001, 32, "f32" if m == 1 else "bf16", seed=seed)
+        w = ext.pack_w4(codes, scales, zeros, 32).to("cuda")
+        x = x.cuda()
+        ext.matrix_mul_w4(x, w)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = ext.matrix_mul_w4(x, w)
+        sets.append((g, x, w, y))
+    want = []
+    for _, x, w, _ in sets:
+        x.mul_(-0.5)
+        want.append(ext.matrix_mul_w4(x, w))
+        assert torch.equal(want[-1], ext.matrix_mul_w4(x, w))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(4):
+        for (g, _, _, _), st in zip(sets, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+    torch.cuda.synchronize()
+    for (_, _, _, y), ref in zip(sets, want):
+        assert torch.equal(y, ref)
+
+
+@gpu
+def test_offsets_past_32_bits():
+    """Codes of 2.2 GB: rows past 2^31 bytes are read from where they are."""
+    n, k = 140000, 32768
+    g = torch.Generator(device="cuda").manual_seed(5)
+    codes = torch.randint(0, 256, (n, k // 2), device="cuda", generator=g, dtype=torch.uint8)
+    scales = torch.rand(k // 128, n, device="cuda", generator=g).half()
+    w = ext.W4Weight((n, k), 128, codes, scales, None)
+    x = torch.zeros(1, k, device="cuda", dtype=torch.float16)
+    x[0, ::97] = 1.0
+    got = ext.matrix_mul_w4(x, w)[0]
+    for rows in (slice(0, 64), slice(n - 64, n)):
+        part = ext.W4Weight((64, k), 128, codes[rows], scales[:, rows], None)
+        want = x.double() @ part.dequantize().double().t()
+        assert ((got[rows].double() - want[0]).abs() <= 2.0 ** -10 * want[0].abs() + 2.0 ** -14 * 400).all()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_train_quantise_serve(dtype):
+    """The operators together: train a small head with linear_cross_entropy, quantise it, and
+    serve its logits in 4 bits; they equal the dequantised head's, and the loss over them is
+    the loss linear_cross_entropy gives for the dequantised head."""
+    g = torch.Generator(device="cuda").manual_seed(9)
+    v, d, t = 1000, 256, 24
+    head = (torch.randn(v, d, device="cuda", generator=g) * d ** -0.5).to(DT[dtype]).requires_grad_(True)
+    x = torch.randn(t, d, device="cuda", generator=g).to(DT[dtype])
+    y = torch.randint(0, v, (t,), device="cuda", generator=g)
+    for _ in range(3):
+        loss = ext.linear_cross_entropy(x, head, y)
+        loss.backward()
+        with torch.no_grad():
+            head -= head.grad
+            head.grad = None
+    q = ext.quantize_w4(head, 64)
+    per_token = []
+    with torch.no_grad():
+        whole = ext.matrix_mul_w4(x, q)            # a batch at once (24 rows)
+        for i in range(t):                          # and one token after another
+            step = ext.matrix_mul_w4(x[i], q)
+            per_token.append(step)
+    w = q.dequantize().double()
+    ref = x.double() @ w.t()
+    bound = 2.0 ** -18 * (x.double().abs() @ w.abs().t()) + 1.001 * U[dtype] * ref.abs()
+    if dtype == "f32":   # 24 rows of fp32 go through the 3xTF32 product
+        bound = bound + (2.0 ** -14) * (x.double().abs() @ w.abs().t())
+    assert ((whole.double() - ref).abs() <= bound).all()
+    assert ((torch.stack(per_token).double() - ref).abs() <= bound).all()
+    if dtype == "f32":
+        got = ext.linear_cross_entropy(x, q.dequantize(), y, reduction="none").double()
+        want = torch.logsumexp(ref, 1) - ref.gather(1, y[:, None])[:, 0]
+        e = 1e-5 + 2e-6 * (x.double().norm(dim=1).max() * w.norm(dim=1).max()).item()
+        assert ((got - want).abs() <= e + 1e-5 * want).all()

@@ -27,7 +27,7 @@ EXPORTS = [
     "tilec_mm_device_status", "tilec_strerror", "tilec_mm_abi_version", "tilec_mm_built_arch",
     "tilec_mm_f32_splitk_noalloc", "tilec_mm_selftest_wait", "tilec_mm_f32_ex", "tilec_mm_workspace_bytes_ex",
     "tilec_mm_set_wait_limit", "tilec_linear_ce_forward", "tilec_linear_ce_backward",
-    "tilec_linear_ce_workspace_bytes",
+    "tilec_linear_ce_workspace_bytes", "tilec_mm_w4", "tilec_mm_w4_workspace_bytes",
 ]
 
 # Bits of the device status word (TILEC_DEV_STATUS_* in include/tilec_mm.h).
@@ -130,6 +130,10 @@ def load():
         lib.tilec_linear_ce_backward.restype = ctypes.c_int
         lib.tilec_linear_ce_workspace_bytes.argtypes = [vp, vp, i32, i64, i64, i64, i64, i64, i32, i32]
         lib.tilec_linear_ce_workspace_bytes.restype = sz
+        lib.tilec_mm_w4.argtypes = [vp, i32, i64, i64, vp, vp, i32, vp, i64, i64, i64, vp, vp, i64, vp, sz, vp]
+        lib.tilec_mm_w4.restype = ctypes.c_int
+        lib.tilec_mm_w4_workspace_bytes.argtypes = [vp, i32, i64, i64, i64, i64, i64, vp, i64]
+        lib.tilec_mm_w4_workspace_bytes.restype = sz
         _load_fast(lib)
         _lib = lib
         return _lib

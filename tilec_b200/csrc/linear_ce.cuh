@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(256) f16_join_slabs_kernel(const float* __rest
                                                              unsigned short* out, int64_t ldo, int64_t M, int64_t N,
                                                              const int* __restrict__ count,
                                                              const int* __restrict__ rows, const float* scale,
-                                                             float scale2, int bf16, int vec_out) {
+                                                             float scale2, const void* bias, int bf16, int vec_out) {
   pdl_wait();
   pdl_launch_dependents();
   if (count != nullptr) M = *count;
@@ -247,9 +247,14 @@ __global__ void __launch_bounds__(256) f16_join_slabs_kernel(const float* __rest
       continue;
     }
     const float f = (scale != nullptr ? *scale : 1.f) * scale2;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      x[j] *= f;
+      if (bias != nullptr && c + j < N) x[j] += load_16(bias, c + j, bf16);
+    }
     uint32_t w[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) w[j] = pack_16x2(x[2 * j] * f, x[2 * j + 1] * f, bf16);
+    for (int j = 0; j < 4; ++j) w[j] = pack_16x2(x[2 * j], x[2 * j + 1], bf16);
     unsigned short* d = out + (rows != nullptr ? int64_t(rows[r]) : r) * ldo + c;
     if (vec_out && c + 8 <= N) {
       *reinterpret_cast<uint4*>(d) = make_uint4(w[0], w[1], w[2], w[3]);

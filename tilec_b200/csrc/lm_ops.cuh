@@ -31,6 +31,8 @@ int lm_device(DeviceInfo** d, LmInfo** lm) {
     attr(tc2_f16_kernel<kEpiAcc, false, false>);
     attr(tc2_f16_kernel<kEpiOut, true, false>);
     attr(tc2_f16_kernel<kEpiAcc, true, false>);
+    attr(tc2_f16_kernel<kEpiOut, false, true>);
+    attr(tc2_f16_kernel<kEpiAcc, false, true>);
     cudaLaunchConfig_t lc = {};
     lc.gridDim = dim3(2, 1, 1);
     lc.blockDim = dim3(F16Cfg::kThreads);
@@ -110,6 +112,49 @@ int f16_slices(int64_t M, int64_t N, int64_t K, const LmInfo& lm, int* kb_per_sl
   const int64_t per = cdiv(nkb, n);
   *kb_per_slice = static_cast<int>(per);
   return static_cast<int>(cdiv(nkb, per));
+}
+
+#define TILEC_TRY(expr)            \
+  do {                             \
+    const int rc_ = (expr);        \
+    if (rc_) return rc_;           \
+  } while (0)
+
+// A 16-bit product with its sums in fp32: K slices go through slabs ([slices][M][lda] floats),
+// a sum over several products (dx over pieces of the vocabulary) through acc_in / acc_out
+// ([M][lda] floats).  out == nullptr: the sums stay in acc_out.
+template <bool A_MN, bool B_K>
+int product16(const Op16& A, const Op16& B, int64_t M, int64_t N, int64_t K, F16Args a, int slices, int kb,
+              int64_t lda, const float* acc_in, float* acc_out, void* out, int64_t ldo, float* slabs,
+              const LmInfo& lm, const DeviceInfo& d, cudaStream_t s) {
+  const int vec = aligned16(out) && ldo % 8 == 0;
+  a.slices = slices;
+  a.kb_per_slice = kb;
+  if (slices > 1) {
+    F16Args b = a;
+    b.out = slabs;
+    b.ldo = lda;
+    b.slab = M * lda;
+    b.acc = nullptr;
+    TILEC_TRY((launch_f16<kEpiAcc, A_MN, B_K>(A, B, M, N, K, b, lm, s)));
+    int64_t blocks = cdiv(M * cdiv(N, 8), 256);
+    if (blocks > int64_t(d.sms) * 8) blocks = int64_t(d.sms) * 8;
+    return launch_k(f16_join_slabs_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, 1,
+                    static_cast<const float*>(slabs), slices, b.slab, lda, acc_in, acc_out,
+                    static_cast<unsigned short*>(out), ldo, M, N, a.count_is_k ? nullptr : a.count, a.rows, a.scale,
+                    a.scale2, a.bias, a.bf16, vec);
+  }
+  a.acc = acc_in;
+  a.ldacc = lda;
+  if (out == nullptr) {
+    a.out = acc_out;
+    a.ldo = lda;
+    return launch_f16<kEpiAcc, A_MN, B_K>(A, B, M, N, K, a, lm, s);
+  }
+  a.out = out;
+  a.ldo = ldo;
+  a.vec_out = vec;
+  return launch_f16<kEpiOut, A_MN, B_K>(A, B, M, N, K, a, lm, s);
 }
 
 // ---------------------------------------------------------------- linear cross entropy
@@ -265,12 +310,6 @@ int run_mm(const Problem& q, int flags, uint8_t* ws, const CePlan& p, cudaStream
   return run_problem(q, &cfg, p.mm_bytes ? ws + p.off_mm : nullptr, p.mm_bytes, s);
 }
 
-#define TILEC_TRY(expr)            \
-  do {                             \
-    const int rc_ = (expr);        \
-    if (rc_) return rc_;           \
-  } while (0)
-
 int check_ws(const CePlan& p, void* ws, size_t ws_bytes) {
   return p.bytes > 0 && (!ws || ws_bytes < p.bytes || (reinterpret_cast<uintptr_t>(ws) & 255u) != 0)
              ? TILEC_ERR_WORKSPACE
@@ -374,42 +413,6 @@ int ce_backward_f32(const CeCall& c, const CePlan& p, const float* stats_buf, co
   return TILEC_OK;
 }
 
-// One gradient product of a piece: with K slices through slabs, and (dx over several pieces)
-// through fp32 sums of the earlier pieces.
-template <bool A_MN>
-int ce_grad_product(const Op16& A, const Op16& B, int64_t M, int64_t N, int64_t K, F16Args a, int slices, int kb,
-                    const float* acc_in, float* acc_out, void* out, float* slabs, const CePlan& p,
-                    const LmInfo& lm, const DeviceInfo& d, cudaStream_t s) {
-  const int vec = aligned16(out) && N % 8 == 0;
-  a.slices = slices;
-  a.kb_per_slice = kb;
-  if (slices > 1) {
-    F16Args b = a;
-    b.out = slabs;
-    b.ldo = p.ldacc;
-    b.slab = M * p.ldacc;
-    b.acc = nullptr;
-    TILEC_TRY((launch_f16<kEpiAcc, A_MN, false>(A, B, M, N, K, b, lm, s)));
-    int64_t blocks = cdiv(M * cdiv(N, 8), 256);
-    if (blocks > int64_t(d.sms) * 8) blocks = int64_t(d.sms) * 8;
-    return launch_k(f16_join_slabs_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, 1,
-                    static_cast<const float*>(slabs), slices, b.slab, p.ldacc, acc_in, acc_out,
-                    static_cast<unsigned short*>(out), N, M, N, a.count_is_k ? nullptr : a.count, a.rows, a.scale,
-                    a.scale2, a.bf16, vec);
-  }
-  a.acc = acc_in;
-  a.ldacc = p.ldacc;
-  if (out == nullptr) {
-    a.out = acc_out;
-    a.ldo = p.ldacc;
-    return launch_f16<kEpiAcc, A_MN, false>(A, B, M, N, K, a, lm, s);
-  }
-  a.out = out;
-  a.ldo = N;
-  a.vec_out = vec;
-  return launch_f16<kEpiOut, A_MN, false>(A, B, M, N, K, a, lm, s);
-}
-
 int ce_backward(const CeCall& c, const float* stats_buf, const float* grad, void* dx, void* dw, void* workspace,
                 size_t ws_bytes, cudaStream_t s) {
   const int grads = (dx ? 1 : 0) | (dw ? 2 : 0);
@@ -476,16 +479,16 @@ int ce_backward(const CeCall& c, const float* stats_buf, const float* grad, void
       const bool last = i == p.pieces - 1;
       float* acc = reinterpret_cast<float*>(ws + p.off_acc);
       g.rows = rows;
-      TILEC_TRY((ce_grad_product<false>(Op16{prob, p.ldp, false}, Op16{wi, ldw, true}, c.T, c.D, n, g, p.dx_slices,
-                                        p.dx_kb, i > 0 ? acc : nullptr, acc, last ? dx : nullptr, slabs, p, *lm, *d,
-                                        s)));
+      TILEC_TRY((product16<false, false>(Op16{prob, p.ldp, false}, Op16{wi, ldw, true}, c.T, c.D, n, g, p.dx_slices,
+                                         p.dx_kb, p.ldacc, i > 0 ? acc : nullptr, acc, last ? dx : nullptr, c.D, slabs,
+                                         *lm, *d, s)));
     }
     if (dw) {
       g.rows = nullptr;
       g.count_is_k = 1;
-      TILEC_TRY((ce_grad_product<true>(Op16{prob, p.ldp, true}, Op16{xc, p.dp, true}, n, c.D, c.T, g, p.dw_slices,
-                                       p.dw_kb, nullptr, nullptr, static_cast<unsigned short*>(dw) + v0 * c.D, slabs,
-                                       p, *lm, *d, s)));
+      TILEC_TRY((product16<true, false>(Op16{prob, p.ldp, true}, Op16{xc, p.dp, true}, n, c.D, c.T, g, p.dw_slices,
+                                        p.dw_kb, p.ldacc, nullptr, nullptr,
+                                        static_cast<unsigned short*>(dw) + v0 * c.D, c.D, slabs, *lm, *d, s)));
     }
   }
   return TILEC_OK;
@@ -494,6 +497,200 @@ int ce_backward(const CeCall& c, const float* stats_buf, const float* grad, void
 CeCall ce_call(const void* x, const void* w, const int64_t* target, int32_t dtype, int64_t T, int64_t V, int64_t D,
                int64_t ldx, int64_t ldw, int64_t ignore, int32_t reduction) {
   return CeCall{x, w, target, dtype, T, V, D, ldx, ldw, ignore, reduction};
+}
+
+// ---------------------------------------------------------------- 4-bit weights
+// Bytes of expanded weights held at a time where x has many rows.
+constexpr int64_t kW4ExpandBytes = int64_t(256) << 20;
+
+struct W4Call {
+  const void* x;
+  int dtype;
+  int64_t M, ldx;
+  const void* codes;
+  const void* scales;
+  int sdt;
+  const uint8_t* zeros;
+  int64_t N, K, group;
+  const void* bias;
+  void* out;
+  int64_t ldo;
+};
+
+struct W4Plan {
+  bool stream = false;   // w4_mma_kernel; otherwise expanded weights and a plain product
+  bool columns = false;  // x goes through w4_columns_kernel (stream) or pack16 first
+  int parts = 1, nt = 1, mt = 1, splits = 1;
+  int64_t blocks = 0, kp = 0, piece = 0;
+  int slices = 1, kb = 0;
+  int64_t ldslab = 0;
+  size_t off_x = 0, off_w = 0, off_slabs = 0, off_mm = 0, mm_bytes = 0, bytes = 0;
+};
+
+int check_w4(const W4Call& c) {
+  if (c.dtype < TILEC_DTYPE_F32 || c.dtype > TILEC_DTYPE_BF16 || c.sdt < TILEC_DTYPE_F32 || c.sdt > TILEC_DTYPE_BF16)
+    return TILEC_ERR_BAD_ARG;
+  if (c.M < 0 || c.N < 0 || c.K < 1 || c.ldx < c.K) return TILEC_ERR_BAD_ARG;
+  if (c.group != 32 && c.group != 64 && (c.group < 128 || c.group % 128 != 0)) return TILEC_ERR_BAD_ARG;
+  if (c.M >= (int64_t(1) << 30) || c.N >= (int64_t(1) << 30) || c.K >= (int64_t(1) << 30) ||
+      c.group >= (int64_t(1) << 31))
+    return TILEC_ERR_UNSUPPORTED;
+  return TILEC_OK;
+}
+
+int check_w4_pointers(const W4Call& c) {
+  if (c.M == 0 || c.N == 0) return TILEC_OK;
+  if (!c.x || !c.codes || !c.scales || !c.out || c.ldo < c.N) return TILEC_ERR_BAD_ARG;
+  const uintptr_t elem = c.dtype == TILEC_DTYPE_F32 ? 3 : 1, selem = c.sdt == TILEC_DTYPE_F32 ? 3 : 1;
+  auto off = [](const void* p, uintptr_t mask) { return (reinterpret_cast<uintptr_t>(p) & mask) != 0; };
+  if (off(c.codes, 15) || off(c.x, elem) || off(c.out, elem) || off(c.bias, elem) || off(c.scales, selem))
+    return TILEC_ERR_BAD_ARG;
+  return TILEC_OK;
+}
+
+// Up to 32 columns (x rows, three columns each in fp32) the codes are streamed through the
+// mma kernel; above, W is expanded once into the workspace and multiplied on the tcgen05
+// kernels (fp32: 3xTF32).
+constexpr int64_t kW4MaxCols = 32;
+
+void plan_w4(const W4Call& c, const DeviceInfo& d, const LmInfo& lm, W4Plan* p) {
+  const bool f32 = c.dtype == TILEC_DTYPE_F32;
+  p->blocks = cdiv(c.K, kW4Block);
+  p->kp = p->blocks * kW4Block;
+  p->parts = f32 ? 3 : 1;
+  const int64_t cols = c.M * p->parts;
+  size_t at = 0;
+  auto take = [&](size_t bytes) {
+    const size_t o = at;
+    at = align256(at + bytes);
+    return o;
+  };
+  if (cols <= kW4MaxCols) {
+    p->stream = true;
+    p->nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
+    p->mt = p->nt == 1 ? 1 : 2;
+    p->columns = f32 || c.K % kW4Block != 0 || !rows_aligned16(c.x, c.ldx);
+    if (p->columns) p->off_x = take(size_t(cols) * p->kp * 2);
+    // CTAs of 8 warps: three per SM keep enough loads in flight; every warp has a block.
+    const int64_t tiles = cdiv(c.N, 16 * p->mt);
+    while (p->splits < 8 && tiles * p->splits < int64_t(d.sms) * 3 && p->blocks >= 2 * p->splits * kW4Warps)
+      p->splits *= 2;
+  } else {
+    int64_t piece = kW4ExpandBytes / (p->kp * (f32 ? 4 : 2)) / 256 * 256;
+    if (piece < 256) piece = 256;
+    p->piece = c.N < piece ? c.N : piece;
+    p->off_w = take(size_t(p->piece) * p->kp * (f32 ? 4 : 2));
+    if (f32) {
+      const int64_t last = c.N - (cdiv(c.N, p->piece) - 1) * p->piece;
+      for (int64_t n : {p->piece, last}) {
+        Problem q = single(static_cast<const float*>(c.x), nullptr, static_cast<float*>(c.out), c.M, n, c.K, c.ldx,
+                           p->kp, c.ldo > 0 ? c.ldo : c.N);
+        const size_t b = mm_bytes(q, TILEC_MM_TRANS_B);
+        if (b > p->mm_bytes) p->mm_bytes = b;
+      }
+      if (p->mm_bytes) p->off_mm = take(p->mm_bytes);
+    } else {
+      p->columns = !rows_aligned16(c.x, c.ldx);
+      if (p->columns) p->off_x = take(size_t(c.M) * p->kp * 2);
+      p->slices = f16_slices(c.M, p->piece, c.K, lm, &p->kb);
+      p->ldslab = round_up(p->piece, 8);
+      if (p->slices > 1) p->off_slabs = take(size_t(p->slices) * c.M * p->ldslab * 4);
+    }
+  }
+  p->bytes = at;
+}
+
+template <bool BF16, int GPB>
+int launch_w4(const W4Args& a, int nt, int mt, cudaStream_t s) {
+  const int64_t tiles = cdiv(a.N, 16 * mt);
+  const dim3 grid(static_cast<unsigned>(tiles * a.splits));
+  auto go = [&](auto kern) { return launch_k(kern, grid, dim3(32 * kW4Warps), 0, s, a.splits, a); };
+  if (nt == 1) return go(w4_mma_kernel<BF16, 1, 1, GPB>);
+  if (nt == 2) return go(w4_mma_kernel<BF16, 2, 2, GPB>);
+  return go(w4_mma_kernel<BF16, 4, 2, GPB>);
+}
+
+int run_w4(const W4Call& c, void* workspace, size_t ws_bytes, cudaStream_t s) {
+  DeviceInfo* d = nullptr;
+  LmInfo* lm = nullptr;
+  TILEC_TRY(lm_device(&d, &lm));
+  W4Plan p;
+  plan_w4(c, *d, *lm, &p);
+  if (p.bytes > 0 && (!workspace || ws_bytes < p.bytes || (reinterpret_cast<uintptr_t>(workspace) & 255u) != 0))
+    return TILEC_ERR_WORKSPACE;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const bool f32 = c.dtype == TILEC_DTYPE_F32;
+  W4Args a = {};
+  a.codes = static_cast<const uint4*>(c.codes);
+  a.scales = c.scales;
+  a.zeros = c.zeros;
+  a.sdt = c.sdt;
+  a.N = static_cast<int>(c.N);
+  a.blocks = static_cast<int>(p.blocks);
+  a.group_blocks = c.group >= kW4Block ? static_cast<int>(c.group / kW4Block) : 1;
+  const int gpb = c.group == 32 ? 4 : c.group == 64 ? 2 : 1;
+  if (p.stream) {
+    a.x = static_cast<const unsigned short*>(c.x);
+    a.ldx = c.ldx;
+    a.parts = p.parts;
+    a.cols = static_cast<int>(c.M * p.parts);
+    a.M = static_cast<int>(c.M);
+    a.out = c.out;
+    a.ldo = c.ldo;
+    a.odt = c.dtype;
+    a.bias = c.bias;
+    a.splits = p.splits;
+    if (p.columns) {
+      unsigned short* xc = reinterpret_cast<unsigned short*>(ws + p.off_x);
+      TILEC_TRY(launch_k(w4_columns_kernel, dim3(static_cast<unsigned>(cdiv(p.kp, 2048)), static_cast<unsigned>(c.M)),
+                         dim3(256), 0, s, 1, c.x, c.ldx, static_cast<int>(c.K), f32 ? 1 : 0, xc, p.kp));
+      a.x = xc;
+      a.ldx = p.kp;
+    }
+    const bool bf16 = c.dtype != TILEC_DTYPE_F16;
+    if (bf16)
+      return gpb == 4   ? launch_w4<true, 4>(a, p.nt, p.mt, s)
+             : gpb == 2 ? launch_w4<true, 2>(a, p.nt, p.mt, s)
+                        : launch_w4<true, 1>(a, p.nt, p.mt, s);
+    return gpb == 4   ? launch_w4<false, 4>(a, p.nt, p.mt, s)
+           : gpb == 2 ? launch_w4<false, 2>(a, p.nt, p.mt, s)
+                      : launch_w4<false, 1>(a, p.nt, p.mt, s);
+  }
+  const void* x = c.x;
+  int64_t ldx = c.ldx;
+  if (p.columns) {
+    TILEC_TRY(pack16(c.x, c.ldx, ws + p.off_x, p.kp, c.M, c.K, nullptr, nullptr, nullptr, 0, nullptr, *d, s));
+    x = ws + p.off_x;
+    ldx = p.kp;
+  }
+  void* wd = ws + p.off_w;
+  const int64_t elem = f32 ? 4 : 2;
+  for (int64_t n0 = 0; n0 < c.N; n0 += p.piece) {
+    const int64_t n = c.N - n0 < p.piece ? c.N - n0 : p.piece;
+    int64_t blocks = cdiv(n * p.blocks * 16, 256);
+    if (blocks > int64_t(d->sms) * 16) blocks = int64_t(d->sms) * 16;
+    TILEC_TRY(launch_k(w4_expand_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, 1, a,
+                       static_cast<int>(n0), static_cast<int>(n), gpb, c.dtype, wd, p.kp));
+    uint8_t* out = static_cast<uint8_t*>(c.out) + n0 * elem;
+    const uint8_t* bias = c.bias ? static_cast<const uint8_t*>(c.bias) + n0 * elem : nullptr;
+    if (f32) {
+      Problem q = single(static_cast<const float*>(x), static_cast<const float*>(wd), reinterpret_cast<float*>(out),
+                         c.M, n, c.K, ldx, p.kp, c.ldo);
+      q.bias = reinterpret_cast<const float*>(bias);
+      tilec_mm_cfg cfg = {};
+      cfg.flags = TILEC_MM_TRANS_B;
+      TILEC_TRY(run_problem(q, &cfg, p.mm_bytes ? ws + p.off_mm : nullptr, p.mm_bytes, s));
+    } else {
+      F16Args f = {};
+      f.bf16 = c.dtype == TILEC_DTYPE_BF16;
+      f.scale2 = 1.f;
+      f.bias = bias;
+      TILEC_TRY((product16<false, true>(Op16{x, ldx, false}, Op16{wd, p.kp, false}, c.M, n, c.K, f, p.slices, p.kb,
+                                        p.ldslab, nullptr, nullptr, out, c.ldo,
+                                        reinterpret_cast<float*>(ws + p.off_slabs), *lm, *d, s)));
+    }
+  }
+  return TILEC_OK;
 }
 
 }  // namespace
@@ -534,6 +731,38 @@ int tilec_linear_ce_backward(const void* x, const void* w, const int64_t* target
   if (rc) return rc;
   if (!stats || (!grad && (T > 0 || reduction != kReduceNone))) return TILEC_ERR_BAD_ARG;
   return ce_backward(c, stats, grad, dx, dw, workspace, ws_bytes, static_cast<cudaStream_t>(stream));
+}
+
+size_t tilec_mm_w4_workspace_bytes(const void* x, int32_t dtype, int64_t M, int64_t ldx, int64_t N, int64_t K,
+                                   int64_t group, const void* out, int64_t ldo) {
+  W4Call c = {};
+  c.x = x ? x : reinterpret_cast<const void*>(256);
+  c.dtype = dtype;
+  c.M = M;
+  c.ldx = ldx;
+  c.N = N;
+  c.K = K;
+  c.group = group;
+  c.out = const_cast<void*>(out);
+  c.ldo = ldo;
+  if (check_w4(c) || M == 0 || N == 0 || ldo < N) return 0;
+  DeviceInfo* d = nullptr;
+  LmInfo* lm = nullptr;
+  if (lm_device(&d, &lm)) return 0;
+  W4Plan p;
+  plan_w4(c, *d, *lm, &p);
+  return p.bytes;
+}
+
+int tilec_mm_w4(const void* x, int32_t dtype, int64_t M, int64_t ldx, const void* codes, const void* scales,
+                int32_t scale_dtype, const uint8_t* zeros, int64_t N, int64_t K, int64_t group, const void* bias,
+                void* out, int64_t ldo, void* workspace, size_t ws_bytes, void* stream) {
+  const W4Call c{x, dtype, M, ldx, codes, scales, scale_dtype, zeros, N, K, group, bias, out, ldo};
+  int rc = check_w4(c);
+  if (rc) return rc;
+  rc = check_w4_pointers(c);
+  if (rc || M == 0 || N == 0) return rc;
+  return run_w4(c, workspace, ws_bytes, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

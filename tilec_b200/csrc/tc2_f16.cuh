@@ -17,6 +17,9 @@
 // Where time goes (B200): see launch_f16 in lm_ops.cuh.
 #pragma once
 
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
 #include "common.cuh"
 #include "tc_gemm.cuh"
 
@@ -37,6 +40,11 @@ __device__ __forceinline__ uint32_t pack_16x2(float lo, float hi, bool bf16) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
+}
+
+__device__ __forceinline__ float load_16(const void* p, int64_t i, bool bf16) {
+  return bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i])
+              : __half2float(static_cast<const __half*>(p)[i]);
 }
 
 // What becomes of a finished tile.
@@ -73,6 +81,7 @@ struct F16Args {
   int64_t ldacc;
   const float* scale;     // kEpiOut: *scale * scale2 multiplies the sums (nullptr: scale2 alone)
   float scale2;
+  const void* bias;       // kEpiOut: 16-bit values added per column, or nullptr
 };
 
 struct F16Cfg {
@@ -136,6 +145,11 @@ __device__ __forceinline__ void f16_store_rows(const F16Args& p, const float* st
       if constexpr (EPI == kEpiOut) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] *= scale;
+        if (p.bias != nullptr) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (j < n) x[j] += load_16(p.bias, col + j, p.bf16);
+        }
       }
       uint4 h;
       h.x = pack_16x2(x[0], x[1], p.bf16);

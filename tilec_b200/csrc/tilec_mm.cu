@@ -28,6 +28,7 @@
 #include "tc2_tf32p.cuh"
 #include "tc2_f16.cuh"
 #include "linear_ce.cuh"
+#include "w4.cuh"
 
 static_assert(TILEC_DEV_STATUS_TIMEOUT == tilec::TILEC_DEV_TIMEOUT && TILEC_DEV_STATUS_TMEM == tilec::TILEC_DEV_TMEM &&
                   TILEC_DEV_STATUS_BAD_LAUNCH == tilec::TILEC_DEV_BAD_LAUNCH &&

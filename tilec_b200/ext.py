@@ -24,7 +24,7 @@ import torch
 
 from . import _native
 from .language import cdiv  # noqa: F401  (re-exported like tilec/ext.py:3)
-from .lm import linear_cross_entropy  # noqa: F401
+from .lm import W4Weight, linear_cross_entropy, matrix_mul_w4, pack_w4, quantize_w4  # noqa: F401
 
 # Kernel tile shapes (for callers that size work around them; the library picks per call).
 SIMT_TILE = (128, 128, 16)     # BM, BN, BK of the SIMT kernel

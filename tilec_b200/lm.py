@@ -2,9 +2,12 @@
 
 * ``linear_cross_entropy``: the output projection fused with its loss and gradients; the
   [tokens, vocabulary] logits are never kept.
+* ``matrix_mul_w4``: x @ W.T with W in 4-bit codes and a scale per group; ``pack_w4`` lays
+  out given codes, ``quantize_w4`` makes them from a weight matrix.
 
-The kernels are behind the C ABI (tilec_linear_ce_* in include/tilec_mm.h).  Like the rest
-of the package there is no CPU path: CPU tensors raise, and a missing kernel library raises.
+The kernels are behind the C ABI (tilec_linear_ce_*, tilec_mm_w4 in include/tilec_mm.h).
+Like the rest of the package there is no CPU path for the products: CPU tensors raise, and a
+missing kernel library raises.  (Packing and quantising are plain torch and run anywhere.)
 """
 import torch
 from torch.autograd.function import once_differentiable
@@ -135,3 +138,194 @@ def linear_cross_entropy(x, weight, target, ignore_index=-100, reduction="mean")
     loss = _LinearCrossEntropy.apply(x.reshape(-1, x.shape[-1]), weight, target.reshape(-1).contiguous(),
                                      int(ignore_index), reduction)
     return loss.view(target.shape) if reduction == "none" else loss
+
+
+# ---------------------------------------------------------------- 4-bit weights
+_BLOCK = 128   # k per 64-byte block of codes (tilec_mm_w4 in include/tilec_mm.h)
+
+
+def _check_group(group_size, where):
+    if not isinstance(group_size, int) or not (group_size in (32, 64) or (group_size > 0 and group_size % _BLOCK == 0)):
+        raise ValueError(f"{where}: group_size must be 32, 64 or a multiple of 128, got {group_size!r}")
+
+
+class W4Weight:
+    """A weight [N, K] in 4-bit codes, laid out for matrix_mul_w4 (see pack_w4).
+
+    shape (N, K); group_size; codes uint8 [N, blocks * 64]; scales [groups, N]; zeros uint8
+    [groups, N] or None (every zero point is 8).  The tensors may be moved together with
+    to(device); matrix_mul_w4 reads them in place."""
+
+    def __init__(self, shape, group_size, codes, scales, zeros):
+        self.shape, self.group_size = tuple(shape), group_size
+        self.codes, self.scales, self.zeros = codes, scales, zeros
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def to(self, device):
+        zeros = None if self.zeros is None else self.zeros.to(device)
+        return W4Weight(self.shape, self.group_size, self.codes.to(device), self.scales.to(device), zeros)
+
+    def unpack(self):
+        """The codes as uint8 [N, K], one per byte, in k order."""
+        n, k = self.shape
+        w = self.codes.view(n, -1, 4, 4, 4)                        # block, t, j, byte of the word
+        nib = torch.stack((w & 15, w >> 4), -1).flatten(-2)        # nibbles 0..7 of the word
+        nib = nib.view(*nib.shape[:-1], 2, 4).transpose(-1, -2)    # (i, parity): k = 2i + parity
+        return nib.flatten(-2).transpose(2, 3).reshape(n, -1)[:, :k]
+
+    def dequantize(self):
+        """(code - zero) * scale as float32 [N, K]."""
+        n, k = self.shape
+        scales = self.scales.float().t().repeat_interleave(self.group_size, 1)[:, :k]
+        zeros = 8.0 if self.zeros is None else self.zeros.float().t().repeat_interleave(self.group_size, 1)[:, :k]
+        return (self.unpack().float() - zeros) * scales
+
+    def __repr__(self):
+        return (f"W4Weight(shape={self.shape}, group_size={self.group_size}, scales={self.scales.dtype}, "
+                f"zeros={self.zeros is not None}, device={self.device})")
+
+
+def pack_w4(codes, scales, zeros=None, group_size=128):
+    """Lays 4-bit codes out for matrix_mul_w4, once per weight.
+
+    codes uint8 [N, K], one code 0..15 per byte; scales [N, ceil(K / group_size)] float32,
+    float16 or bfloat16; zeros: None (zero point 8 everywhere) or uint8 of scales' shape,
+    0..15.  The weight is (code - zero) * scale.  group_size: consecutive k that share a
+    scale: 32, 64 or a multiple of 128 (the last group may be short)."""
+    _check_group(group_size, "pack_w4")
+    if codes.dim() != 2 or codes.shape[1] == 0:
+        raise ValueError(f"pack_w4: codes must be [N, K] with K >= 1, got shape {tuple(codes.shape)}")
+    if codes.dtype != torch.uint8:
+        raise TypeError(f"pack_w4: codes must be uint8, got {codes.dtype}")
+    n, k = codes.shape
+    groups = -(-k // group_size)
+    if tuple(scales.shape) != (n, groups):
+        raise ValueError(f"pack_w4: scales have shape {tuple(scales.shape)}, expected {(n, groups)}")
+    if scales.dtype not in _DTYPES:
+        raise TypeError(f"pack_w4: scales must be float32, float16 or bfloat16, got {scales.dtype}")
+    if zeros is not None:
+        if tuple(zeros.shape) != (n, groups):
+            raise ValueError(f"pack_w4: zeros have shape {tuple(zeros.shape)}, expected {(n, groups)}")
+        if zeros.dtype != torch.uint8:
+            raise TypeError(f"pack_w4: zeros must be uint8, got {zeros.dtype}")
+    if scales.device != codes.device or (zeros is not None and zeros.device != codes.device):
+        raise ValueError("pack_w4: codes, scales and zeros must be on one device")
+    if n and (int(codes.max()) > 15 or (zeros is not None and int(zeros.max()) > 15)):
+        raise ValueError("pack_w4: codes and zeros must be 0..15")
+    blocks = -(-k // _BLOCK)
+    if k % _BLOCK:
+        codes = torch.nn.functional.pad(codes, (0, blocks * _BLOCK - k))
+    c = codes.reshape(n, blocks, 4, 4, 4, 2)           # j, t, i, parity: k = 32j + 8t + 2i + parity
+    c = c.permute(0, 1, 3, 2, 5, 4).reshape(n, blocks, 4, 4, 4, 2)   # t, j, then nibbles 4 * parity + i
+    packed = (c[..., 0] | c[..., 1] << 4).reshape(n, blocks * 64)
+    rows = -(-blocks * _BLOCK // group_size)
+
+    def by_group(t):
+        out = torch.zeros(rows, n, dtype=t.dtype, device=t.device)
+        out[:groups] = t.t()
+        return out
+
+    return W4Weight((n, k), group_size, packed, by_group(scales), None if zeros is None else by_group(zeros))
+
+
+def quantize_w4(weight, group_size=128, symmetric=False):
+    """A W4Weight whose values are the nearest of 16 steps to weight [N, K], group by group.
+
+    symmetric: steps of max|w| / 7 around zero (zero point 8).  Otherwise 15 steps over the
+    group's range, widened to hold zero, which stays exact.  Scales have weight's dtype
+    (float32, float16 or bfloat16); codes are chosen for the rounded scale, so an error is at
+    most half a step plus what the scale's rounding cuts off the ends of the range."""
+    _check_group(group_size, "quantize_w4")
+    if weight.dim() != 2 or weight.shape[1] == 0:
+        raise ValueError(f"quantize_w4: weight must be [N, K] with K >= 1, got shape {tuple(weight.shape)}")
+    if weight.dtype not in _DTYPES:
+        raise TypeError(f"quantize_w4: weight must be float32, float16 or bfloat16, got {weight.dtype}")
+    weight = weight.detach()
+    n, k = weight.shape
+    groups = -(-k // group_size)
+    w = torch.nn.functional.pad(weight.float(), (0, groups * group_size - k)).view(n, groups, group_size)
+    if symmetric:
+        scales = w.abs().amax(2) / 7
+    else:
+        low, high = w.amin(2).clamp(max=0), w.amax(2).clamp(min=0)
+        scales = (high - low) / 15
+    scales = scales.to(weight.dtype)
+    step = torch.where(scales > 0, scales.float(), 1.0)
+    if symmetric:
+        zeros, zf = None, torch.full_like(step, 8)
+    else:
+        zf = torch.round(-low / step).clamp(0, 15)
+        zeros = zf.to(torch.uint8)
+    codes = (torch.round(w / step[:, :, None]) + zf[:, :, None]).clamp(0, 15).to(torch.uint8)
+    return pack_w4(codes.view(n, -1)[:, :k], scales, zeros, group_size)
+
+
+def matrix_mul_w4(x, weight, bias=None, out=None):
+    """x @ W.T (+ bias) with W a W4Weight of shape (N, K); x [..., K] float32, float16 or
+    bfloat16 on the weight's device; bias None or [N] of x's dtype.  Returns (or writes into
+    `out`, [..., N] with unit column stride) x's dtype.
+
+    Up to 32 rows of x (float32: 10), the decoding case, the codes are read once and enter
+    exactly: products are exact, sums fp32, one rounding at the end.  More rows: the weight is
+    expanded into the workspace, rounded to x's dtype (float32: exact), at most 256 MiB (or
+    256 rows of it) at a time, and multiplied on the tensor cores (float32: the 3xTF32 product
+    of matrix_mul).  Not differentiable."""
+    if not isinstance(weight, W4Weight):
+        raise TypeError(f"matrix_mul_w4: weight must be a W4Weight (pack_w4, quantize_w4), got {type(weight).__name__}")
+    n, k = weight.shape
+    if x.dim() < 1 or x.shape[-1] != k:
+        raise ValueError(f"matrix_mul_w4: shapes {tuple(x.shape)} and {weight.shape} don't match (x [..., K], "
+                         "weight [N, K])")
+    dt = _DTYPES.get(x.dtype)
+    if dt is None:
+        raise TypeError(f"matrix_mul_w4: x must be float32, float16 or bfloat16, got {x.dtype}")
+    codes, scales, zeros, dev = weight.codes, weight.scales, weight.zeros, x.device
+    if not (x.is_cuda and codes.device == dev):
+        raise ValueError(f"matrix_mul_w4: x and weight must be on one CUDA device (got {dev} and {codes.device}); "
+                         "tilec_b200 has no CPU path")
+    if bias is not None and (bias.dtype != x.dtype or bias.dim() != 1 or bias.shape[0] != n or bias.device != dev):
+        raise ValueError(f"matrix_mul_w4: bias must be a {x.dtype} [{n}] tensor on {dev}")
+    if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
+        raise ValueError("matrix_mul_w4: not differentiable; call it under torch.no_grad() or detach the inputs")
+    xr, ldx = _rows(x if x.dim() == 2 else x.reshape(-1, k))
+    m = xr.shape[0]
+    shape = x.shape[:-1] + (n,)
+    if out is None:
+        out = torch.empty(shape, dtype=x.dtype, device=dev)
+        out2, ldo = out, n
+    else:
+        if out.dtype != x.dtype or out.shape != shape or out.device != dev:
+            raise ValueError(f"matrix_mul_w4: out must be a {x.dtype} {tuple(shape)} tensor on {dev}")
+        try:
+            out2 = out.view(m, n)
+        except RuntimeError:
+            raise ValueError("matrix_mul_w4: the rows of out must lie at one stride") from None
+        s0, s1 = out2.stride()
+        if not ((n <= 1 or s1 == 1) and (m <= 1 or s0 >= n)):
+            raise ValueError("matrix_mul_w4: out must have unit column stride and non-overlapping rows")
+        ldo = s0 if m > 1 else n
+    if m == 0 or n == 0:
+        return out
+    if bias is not None:
+        bias = bias.contiguous()
+    lib = _native.load()
+    prev = torch.cuda.current_device()
+    switch = prev != dev.index
+    if switch:
+        torch.cuda.set_device(dev.index)
+    try:
+        stream = _stream(dev)
+        px, po = xr.data_ptr(), out2.data_ptr()
+        nbytes = lib.tilec_mm_w4_workspace_bytes(px, dt, m, ldx, n, k, weight.group_size, po, ldo)
+        ws = _workspace(nbytes, dev)
+        rc = lib.tilec_mm_w4(px, dt, m, ldx, codes.data_ptr(), scales.data_ptr(), _DTYPES[scales.dtype], _ptr(zeros),
+                             n, k, weight.group_size, _ptr(bias), po, ldo, _ptr(ws), nbytes, stream)
+        _native.check(rc, "tilec_mm_w4")
+        _check_device(stream)
+    finally:
+        if switch:
+            torch.cuda.set_device(prev)
+    return out
