@@ -307,24 +307,29 @@ TILEC_API size_t tilec_linear_ce_workspace_bytes(const void* x, const void* w, i
 /* Product with 4-bit weights:
  *   out[m, n] = sum_k x[m, k] * (code[n, k] - zero[n, k / group]) * scale[n, k / group] + bias[n]
  * x [M, K] (row stride ldx), bias [N] (or NULL) and out [M, N] (row stride ldo) of `dtype`,
- * scale of scale_dtype, zero 0..15 (NULL: 8 everywhere).  group: 32, 64 or a multiple of 128.
- * Layouts, with B = ceil(K / 128):
- *   codes   [N][B][64 bytes], 16-byte aligned.  As 32-bit little-endian words, word 4t + j
- *           (t, j = 0..3) of a block holds k = 32j + 8t + 0..7 of its 128: k = 2i in bits
- *           4i..4i+3, k = 2i + 1 in bits 4i+16..4i+19 (i = 0..3).  k >= K: any code.
- *   scales  [ceil(128 * B / group)][N], zeros likewise; groups past K: any finite scale.
+ * scale of scale_dtype, zero 0..15.  group: 32, 64 or a multiple of 128.
+ * weight: [ceil(N / 16)][ceil(K / 128)] pieces of 16 rows x 128 k, 16-byte aligned.  A piece is
+ * the group words of its 16 rows, then 64 bytes of codes for each of them.
+ *   Group words of a row: one 32-bit word per group of the block (4 for groups of 32, 2 for 64,
+ *   else 1: longer groups have theirs in each block), zero + (the scale's 16 bits << 16), or for
+ *   fp32 scales pairs of words (zero, scale).
+ *   Codes of a row as 32-bit little-endian words: word 4t + j (t, j = 0..3) holds k = 32j + 8t +
+ *   0..7 of the block, k = 2i in bits 4i..4i+3 and k = 2i + 1 in bits 4i+16..4i+19 (i = 0..3).
+ *   Rows past N and k past K: any codes, finite scales.
  * Codes, zero points and scales enter exactly and sums are fp32, except for more than 32
- * rows (fp32: 10), where the weight (code - zero) * scale is rounded once to dtype and
- * multiplied on the tensor cores (fp32: the 3xTF32 product).
+ * rows (fp32: 8), where the weight (code - zero) * scale is rounded once to dtype and
+ * multiplied on the tensor cores (fp32: the 3xTF32 product).  Up to 8 rows, x enters
+ * as whole multiples of 2^-29 of the power of two at or below the largest magnitude of its
+ * block of 128 k.
  * Workspace: tilec_mm_w4_workspace_bytes (at most 256 MiB of expanded weights or 256 rows). */
-TILEC_API int tilec_mm_w4(const void* x, int32_t dtype, int64_t M, int64_t ldx, const void* codes,
-                          const void* scales, int32_t scale_dtype, const uint8_t* zeros, int64_t N, int64_t K,
-                          int64_t group, const void* bias, void* out, int64_t ldo, void* workspace,
-                          size_t ws_bytes, void* stream);
+TILEC_API int tilec_mm_w4(const void* x, int32_t dtype, int64_t M, int64_t ldx, const void* weight,
+                          int32_t scale_dtype, int64_t N, int64_t K, int64_t group, const void* bias, void* out,
+                          int64_t ldo, void* workspace, size_t ws_bytes, void* stream);
 
 /* Workspace bytes of tilec_mm_w4 (NULL x or out: assumed 16-byte aligned). */
-TILEC_API size_t tilec_mm_w4_workspace_bytes(const void* x, int32_t dtype, int64_t M, int64_t ldx, int64_t N,
-                                             int64_t K, int64_t group, const void* out, int64_t ldo);
+TILEC_API size_t tilec_mm_w4_workspace_bytes(const void* x, int32_t dtype, int64_t M, int64_t ldx,
+                                             int32_t scale_dtype, int64_t N, int64_t K, int64_t group,
+                                             const void* out, int64_t ldo);
 
 #ifdef __cplusplus
 }

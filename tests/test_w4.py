@@ -3,10 +3,14 @@
 Element-wise bounds, u = half a unit in the last place (2^-8 bf16, 2^-11 fp16, 2^-24 fp32) and
 S = sum_k |x (code - zero) scale|:
 
-* up to 32 rows (fp32: 10): products of codes and x are exact; a 128-k block adds 8 groups of
-  16 products to an accumulator, each sum truncated at worst (16 * 2^-23 S), and the at most
-  64 blocks are added in fp32 (64 * 2^-24 S), the scale's product rounds once: below
-  2^-18 S; then one rounding, u |y|.
+* up to 8 rows: x is rounded to a whole number of steps of 2^-29 of its 128-k block's largest
+  magnitude, far below what follows; group sums are exact, the at most 64 blocks' (in up to 24
+  parts) and four digits' sums are added in fp32, (64 + 4) * 2^-24 S for the upper digit, which
+  holds all but 2^-7 of S: below 2^-17.8 S at worst, and the roundings are independent: 2^-18 S
+  is held to; then one rounding, u |y|.
+* up to 32 rows: products of codes and x are exact; a 128-k block adds 8 groups of 16 products
+  to an accumulator, each sum truncated at worst (16 * 2^-23 S), and the at most 64 blocks are
+  added in fp32 (64 * 2^-24 S), the scale's product rounds once: below 2^-18 S.
 * more rows: the weight is rounded to the type, u S more (fp32: the 3xTF32 product,
   3 * 2^-20 S); sums over K <= 8192 in the tensor cores' fp32 stay below 2^-14 S (K / 16 sums,
   each truncated by 2^-23).
@@ -41,7 +45,7 @@ def _weight64(codes, scales, zeros, group):
 
 def _bound(x, w, y, dtype, rows):
     s = x.double().abs() @ w.abs().t()
-    few = rows * (3 if dtype == "f32" else 1) <= 32
+    few = rows <= (8 if dtype == "f32" else 32)
     rel = 2.0 ** -18 if few else 2.0 ** -14 + (3 * 2.0 ** -20 if dtype == "f32" else U[dtype])
     return rel * s + 1.001 * U[dtype] * y.abs() + (2.0 ** -25 if dtype == "f16" else 0.0)
 
@@ -70,19 +74,33 @@ def test_pack_keeps_codes_and_values(n, k, group):
     w = ext.pack_w4(codes, scales, zeros, group)
     assert torch.equal(w.unpack(), codes)
     assert torch.equal(w.dequantize().double(), _weight64(codes, scales, zeros, group).float().double())
+    assert torch.equal(w.scales(), scales) and torch.equal(w.zeros(), zeros)
     # the layout of include/tilec_mm.h, word by word
-    words = w.codes.view(n, -1, 16, 4).long()
-    words = words[..., 0] | words[..., 1] << 8 | words[..., 2] << 16 | words[..., 3] << 24
-    blocks = -(-k // 128)
-    full = torch.nn.functional.pad(codes, (0, blocks * 128 - k)).view(n, blocks, 128).long()
-    for t in range(4):
-        for j in range(4):
-            for i in range(4):
-                for odd in range(2):
-                    assert torch.equal(words[:, :, 4 * t + j] >> (4 * i + 16 * odd) & 15,
-                                       full[:, :, 32 * j + 8 * t + 2 * i + odd])
-    assert w.scales.shape == (-(-blocks * 128 // group), n)
-    assert torch.isfinite(w.scales).all()
+    blocks, per_block = -(-k // 128), max(1, 128 // group)
+    for dtype in (torch.float32, torch.float16, torch.bfloat16):
+        half = ext.pack_w4(codes, scales.to(dtype), zeros, group)
+        assert torch.equal(half.scales(), scales.to(dtype)) and torch.equal(half.zeros(), zeros)
+        assert (ext.pack_w4(codes, scales.to(dtype), None, group).zeros() == 8).all()
+        wide = 2 if dtype == torch.float32 else 1
+        assert half.data.shape == (-(-n // 16), blocks, 64 * per_block * wide + 1024)
+        for row in range(n):
+            for b in range(blocks):
+                piece = half.data[row // 16, b]
+                words = piece[:-1024].clone().view(torch.int32).view(16, per_block, wide)[row % 16]
+                for i in range(per_block):
+                    at = (b * 128 + i * (128 // per_block)) // group
+                    if b * 128 + i * (128 // per_block) >= k:
+                        continue
+                    s = scales.to(dtype)[row, at:at + 1].contiguous()
+                    bits = int(s.view(torch.int32) if wide == 2 else s.view(torch.int16).int() << 16)
+                    z = int(zeros[row, at])
+                    assert words[i].tolist() == ([z, bits] if wide == 2 else [z | bits])
+                word = piece[-1024:].reshape(16, 16, 4)[row % 16].long()
+                word = word[:, 0] | word[:, 1] << 8 | word[:, 2] << 16 | word[:, 3] << 24
+                full = torch.nn.functional.pad(codes[row, b * 128:b * 128 + 128], (0, max(0, b * 128 + 128 - k)))
+                e = torch.arange(128)
+                j, t, i, odd = e // 32, e % 32 // 8, e % 8 // 2, e % 2
+                assert torch.equal(word[4 * t + j] >> (4 * i + 16 * odd) & 15, full.long())
 
 
 @pytest.mark.parametrize("symmetric", [False, True])
@@ -94,14 +112,14 @@ def test_quantize_error_is_half_a_step(group, dtype, symmetric):
     w[3] = 0                       # a group of zeros
     w[4] = w[4].abs() + 1          # all positive: the range is widened to hold zero
     q = ext.quantize_w4(w, group, symmetric)
-    step = q.scales.t().float().repeat_interleave(group, 1)[:, :300]
+    step = q.scales().float().repeat_interleave(group, 1)[:, :300]
     err = (q.dequantize() - w.float()).abs()
     # the rounded scale spans 15 (7) steps short by up to 15 u (7 u) of a step at the ends,
     # and the zero point is rounded to a step
     slack = 15 * U[dtype] + 2.0 ** -20
     assert (err <= (0.5 + (0 if symmetric else 0.5) + slack) * step + 1e-30).all()
     assert (q.dequantize()[3] == 0).all()
-    assert q.shape == (24, 300) and (q.zeros is None) == symmetric
+    assert q.shape == (24, 300) and (q.zeros() == 8).all() >= symmetric
 
 
 def test_refusals():
@@ -142,20 +160,18 @@ def test_refusals():
 def test_abi_refusals():
     from tilec_b200 import _native
     lib = _native.load()
-    ok = dict(x=256, dtype=2, M=2, ldx=64, codes=256, scales=256, sdt=2, zeros=None, N=8, K=64, group=32, bias=None,
-              out=256, ldo=8)
+    ok = dict(x=256, dtype=2, M=2, ldx=64, weight=256, sdt=2, N=8, K=64, group=32, bias=None, out=256, ldo=8)
 
     def call(**kw):
         return lib.tilec_mm_w4(*{**ok, **kw}.values(), None, 0, None)
 
     for bad in (dict(dtype=3), dict(sdt=-1), dict(M=-1), dict(N=-1), dict(K=0), dict(ldx=63), dict(group=16),
-                dict(group=0), dict(group=192), dict(x=None), dict(codes=None), dict(scales=None), dict(out=None),
-                dict(ldo=7), dict(codes=264), dict(x=257), dict(out=257), dict(bias=257), dict(scales=257),
-                dict(sdt=0, scales=258)):
+                dict(group=0), dict(group=192), dict(x=None), dict(weight=None), dict(out=None),
+                dict(ldo=7), dict(weight=264), dict(x=257), dict(out=257), dict(bias=257)):
         assert call(**bad) == 1, bad
     assert call(M=1 << 31) == 7
-    assert call(M=0, x=None, out=None) == 0 and call(N=0, codes=None, scales=None, ldo=0) == 0
-    assert lib.tilec_mm_w4_workspace_bytes(None, 9, 2, 64, 8, 64, 32, None, 8) == 0
+    assert call(M=0, x=None, out=None) == 0 and call(N=0, weight=None, ldo=0) == 0
+    assert lib.tilec_mm_w4_workspace_bytes(None, 9, 2, 64, 2, 8, 64, 32, None, 8) == 0
 
 
 # ---------------------------------------------------------------- GPU
@@ -223,7 +239,7 @@ def test_strides_out_and_shapes(m, dtype):
         wide = torch.full((m, 400), float("nan"), dtype=x.dtype, device="cuda")
         wide[:, off:off + 320] = x
         got = ext.matrix_mul_w4(wide[:, off:off + 320], w, bias)
-        if dtype == "f32" and m > 10:   # the fp32 product picks its kernel by alignment
+        if dtype == "f32" and m > 8:   # the fp32 product picks its kernel by alignment
             torch.testing.assert_close(got, base, rtol=1e-5, atol=1e-4)
         else:
             assert torch.equal(got, base)
@@ -234,7 +250,7 @@ def test_strides_out_and_shapes(m, dtype):
         buf = torch.full((m, 260), 7.0, dtype=x.dtype, device="cuda")
         view = buf[:, off:off + 200]
         assert ext.matrix_mul_w4(x, w, bias, out=view) is view
-        if dtype == "f32" and m > 10:
+        if dtype == "f32" and m > 8:
             torch.testing.assert_close(view, base, rtol=1e-5, atol=1e-4)
         else:
             assert torch.equal(view, base)
@@ -314,14 +330,15 @@ def test_offsets_past_32_bits():
     """Codes of 2.2 GB: rows past 2^31 bytes are read from where they are."""
     n, k = 140000, 32768
     g = torch.Generator(device="cuda").manual_seed(5)
-    codes = torch.randint(0, 256, (n, k // 2), device="cuda", generator=g, dtype=torch.uint8)
-    scales = torch.rand(k // 128, n, device="cuda", generator=g).half()
-    w = ext.W4Weight((n, k), 128, codes, scales, None)
+    data = torch.randint(0, 256, (n // 16, k // 128, 64 + 1024), device="cuda", generator=g, dtype=torch.uint8)
+    words = torch.rand(n // 16, k // 128, 16, device="cuda", generator=g).half().view(torch.int16).int() << 16 | 8
+    data[:, :, :64] = words.view(torch.uint8)
+    w = ext.W4Weight((n, k), 128, torch.float16, data)
     x = torch.zeros(1, k, device="cuda", dtype=torch.float16)
     x[0, ::97] = 1.0
     got = ext.matrix_mul_w4(x, w)[0]
     for rows in (slice(0, 64), slice(n - 64, n)):
-        part = ext.W4Weight((64, k), 128, codes[rows], scales[:, rows], None)
+        part = ext.W4Weight((64, k), 128, torch.float16, data[rows.start // 16:rows.stop // 16])
         want = x.double() @ part.dequantize().double().t()
         assert ((got[rows].double() - want[0]).abs() <= 2.0 ** -10 * want[0].abs() + 2.0 ** -14 * 400).all()
 

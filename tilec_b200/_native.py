@@ -130,9 +130,9 @@ def load():
         lib.tilec_linear_ce_backward.restype = ctypes.c_int
         lib.tilec_linear_ce_workspace_bytes.argtypes = [vp, vp, i32, i64, i64, i64, i64, i64, i32, i32]
         lib.tilec_linear_ce_workspace_bytes.restype = sz
-        lib.tilec_mm_w4.argtypes = [vp, i32, i64, i64, vp, vp, i32, vp, i64, i64, i64, vp, vp, i64, vp, sz, vp]
+        lib.tilec_mm_w4.argtypes = [vp, i32, i64, i64, vp, i32, i64, i64, i64, vp, vp, i64, vp, sz, vp]
         lib.tilec_mm_w4.restype = ctypes.c_int
-        lib.tilec_mm_w4_workspace_bytes.argtypes = [vp, i32, i64, i64, i64, i64, i64, vp, i64]
+        lib.tilec_mm_w4_workspace_bytes.argtypes = [vp, i32, i64, i64, i32, i64, i64, i64, vp, i64]
         lib.tilec_mm_w4_workspace_bytes.restype = sz
         _load_fast(lib)
         _lib = lib

@@ -5,6 +5,9 @@
 namespace tilec {
 namespace {
 
+constexpr int64_t kW4MmaSlabBytes = 32768; // w4_mma_kernel: x in shared memory at a time
+constexpr int64_t kW4MaxSmem = 232448;    // shared memory a CTA may have, and an SM's for all of them
+
 // ---------------------------------------------------------------- 16-bit products
 struct LmInfo {
   int f16_slots = 0;  // CTA pairs of tc2_f16_kernel resident at once
@@ -33,6 +36,38 @@ int lm_device(DeviceInfo** d, LmInfo** lm) {
     attr(tc2_f16_kernel<kEpiAcc, true, false>);
     attr(tc2_f16_kernel<kEpiOut, false, true>);
     attr(tc2_f16_kernel<kEpiAcc, false, true>);
+    auto w4_attr = [&](auto kern) {
+      acc(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, int(kW4MaxSmem)));
+    };
+    auto w4_attrs = [&](auto gpb, auto wide) {
+      constexpr int G = decltype(gpb)::value;
+      constexpr bool W = decltype(wide)::value;
+      auto stream = [&](auto sc) {
+        constexpr int C = decltype(sc)::value;
+        w4_attr(w4_stream_kernel<1, G, C>);
+        w4_attr(w4_stream_kernel<2, G, C>);
+        w4_attr(w4_stream_kernel<4, G, C>);
+      };
+      if constexpr (W) {
+        stream(std::integral_constant<int, TILEC_DTYPE_F32>{});
+      } else {
+        stream(std::integral_constant<int, TILEC_DTYPE_F16>{});
+        stream(std::integral_constant<int, TILEC_DTYPE_BF16>{});
+      }
+      w4_attr(w4_mma_kernel<true, 1, 1, G, W>);
+      w4_attr(w4_mma_kernel<false, 1, 1, G, W>);
+      w4_attr(w4_mma_kernel<true, 2, 2, G, W>);
+      w4_attr(w4_mma_kernel<true, 4, 2, G, W>);
+      w4_attr(w4_mma_kernel<false, 2, 2, G, W>);
+      w4_attr(w4_mma_kernel<false, 4, 2, G, W>);
+    };
+    auto w4_all = [&](auto gpb) {
+      w4_attrs(gpb, std::true_type{});
+      w4_attrs(gpb, std::false_type{});
+    };
+    w4_all(std::integral_constant<int, 1>{});
+    w4_all(std::integral_constant<int, 2>{});
+    w4_all(std::integral_constant<int, 4>{});
     cudaLaunchConfig_t lc = {};
     lc.gridDim = dim3(2, 1, 1);
     lc.blockDim = dim3(F16Cfg::kThreads);
@@ -507,20 +542,33 @@ struct W4Call {
   const void* x;
   int dtype;
   int64_t M, ldx;
-  const void* codes;
-  const void* scales;
+  const void* weight;
   int sdt;
-  const uint8_t* zeros;
   int64_t N, K, group;
   const void* bias;
   void* out;
   int64_t ldo;
 };
 
+template <int NT>
+int64_t w4_stream_fixed_nt(int gpb, bool wide) {
+  return gpb == 4   ? (wide ? W4StreamCfg<NT, 4, true>::kFixed : W4StreamCfg<NT, 4, false>::kFixed)
+         : gpb == 2 ? (wide ? W4StreamCfg<NT, 2, true>::kFixed : W4StreamCfg<NT, 2, false>::kFixed)
+                    : (wide ? W4StreamCfg<NT, 1, true>::kFixed : W4StreamCfg<NT, 1, false>::kFixed);
+}
+int64_t w4_stream_fixed(int nt, int gpb, bool wide) {
+  return nt == 1   ? w4_stream_fixed_nt<1>(gpb, wide)
+         : nt == 2 ? w4_stream_fixed_nt<2>(gpb, wide)
+                   : w4_stream_fixed_nt<4>(gpb, wide);
+}
+
 struct W4Plan {
-  bool stream = false;   // w4_mma_kernel; otherwise expanded weights and a plain product
-  bool columns = false;  // x goes through w4_columns_kernel (stream) or pack16 first
-  int parts = 1, nt = 1, mt = 1, splits = 1;
+  bool stream = false;   // w4_stream_kernel
+  bool mma = false;      // w4_mma_kernel; otherwise expanded weights and a plain product
+  bool pack_x = false;   // x is copied to aligned rows first (expanded weights)
+  int nt = 1, mt = 1, splits = 1, row_warps = 1, slab = 1, per_cta = 0, ctas = 0;
+  bool cut_before = false;
+  size_t off_digits = 0, off_sums = 0, off_scale = 0;
   int64_t blocks = 0, kp = 0, piece = 0;
   int slices = 1, kb = 0;
   int64_t ldslab = 0;
@@ -540,41 +588,71 @@ int check_w4(const W4Call& c) {
 
 int check_w4_pointers(const W4Call& c) {
   if (c.M == 0 || c.N == 0) return TILEC_OK;
-  if (!c.x || !c.codes || !c.scales || !c.out || c.ldo < c.N) return TILEC_ERR_BAD_ARG;
-  const uintptr_t elem = c.dtype == TILEC_DTYPE_F32 ? 3 : 1, selem = c.sdt == TILEC_DTYPE_F32 ? 3 : 1;
+  if (!c.x || !c.weight || !c.out || c.ldo < c.N) return TILEC_ERR_BAD_ARG;
+  const uintptr_t elem = c.dtype == TILEC_DTYPE_F32 ? 3 : 1;
   auto off = [](const void* p, uintptr_t mask) { return (reinterpret_cast<uintptr_t>(p) & mask) != 0; };
-  if (off(c.codes, 15) || off(c.x, elem) || off(c.out, elem) || off(c.bias, elem) || off(c.scales, selem))
+  if (off(c.weight, 15) || off(c.x, elem) || off(c.out, elem) || off(c.bias, elem))
     return TILEC_ERR_BAD_ARG;
   return TILEC_OK;
 }
 
-// Up to 32 columns (x rows, three columns each in fp32) the codes are streamed through the
-// mma kernel; above, W is expanded once into the workspace and multiplied on the tcgen05
-// kernels (fp32: 3xTF32).
+// How many rows of x run where: one or two (a tile of 8 columns of digits; fp32: up to 8, four
+// tiles) on w4_stream_kernel, up to 32 rows of 16-bit x on w4_mma_kernel; above, W is expanded once into the workspace and
+// multiplied on the tcgen05 kernels (fp32: 3xTF32).
 constexpr int64_t kW4MaxCols = 32;
 
 void plan_w4(const W4Call& c, const DeviceInfo& d, const LmInfo& lm, W4Plan* p) {
   const bool f32 = c.dtype == TILEC_DTYPE_F32;
   p->blocks = cdiv(c.K, kW4Block);
   p->kp = p->blocks * kW4Block;
-  p->parts = f32 ? 3 : 1;
-  const int64_t cols = c.M * p->parts;
+  const int digits = kW4Digits;
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t o = at;
     at = align256(at + bytes);
     return o;
   };
-  if (cols <= kW4MaxCols) {
+  if (c.M * digits <= (f32 ? kW4MaxCols : 8)) {
     p->stream = true;
+    const int cols = static_cast<int>(c.M * digits);
     p->nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
-    p->mt = p->nt == 1 ? 1 : 2;
-    p->columns = f32 || c.K % kW4Block != 0 || !rows_aligned16(c.x, c.ldx);
-    if (p->columns) p->off_x = take(size_t(cols) * p->kp * 2);
-    // CTAs of 8 warps: three per SM keep enough loads in flight; every warp has a block.
-    const int64_t tiles = cdiv(c.N, 16 * p->mt);
-    while (p->splits < 8 && tiles * p->splits < int64_t(d.sms) * 3 && p->blocks >= 2 * p->splits * kW4Warps)
-      p->splits *= 2;
+    const int gpb = c.group == 32 ? 4 : c.group == 64 ? 2 : 1;
+    const int pad = 8 * p->nt;
+    // One CTA per SM.  With fewer 16-row tiles than SMs, a cluster of CTAs shares each tile's K.
+    const int64_t tiles = cdiv(c.N, 16);
+    int64_t splits = d.sms / tiles;
+    if (splits > 8) splits = 8;
+    if (splits > p->blocks / 4) splits = p->blocks / 4;
+    if (splits < 1) splits = 1;
+    p->per_cta = static_cast<int>(cdiv(p->blocks, splits));
+    p->splits = static_cast<int>(cdiv(p->blocks, p->per_cta));
+    const int64_t clusters = d.sms / p->splits;
+    p->ctas = static_cast<int>((tiles < clusters ? tiles : clusters) * p->splits);
+    // Two rows are cut in every CTA (a round of some 150 instructions per row and 48 blocks),
+    // more once for all.
+    p->cut_before = c.M > 2;
+    const bool wide = c.sdt == TILEC_DTYPE_F32;
+    const int64_t room = kW4MaxSmem - w4_stream_fixed(p->nt, gpb, wide);
+    int64_t slab = p->per_cta;
+    while (slab > 1 && w4_slab_bytes(slab, cols, pad, gpb) > room) --slab;
+    p->slab = static_cast<int>(slab);
+    if (p->cut_before) {
+      p->off_digits = take(size_t(cols) * p->blocks * kW4Block);
+      p->off_sums = take(size_t(p->blocks) * gpb * pad * 4);
+      p->off_scale = take(size_t(p->blocks) * pad * 4);
+    }
+  } else if (!f32 && c.M <= kW4MaxCols) {
+    p->mma = true;
+    p->nt = c.M <= 8 ? 1 : c.M <= 16 ? 2 : 4;
+    p->mt = c.M <= 8 ? 1 : 2;
+    p->row_warps = 8;
+    const int64_t tiles = cdiv(c.N, 16 * p->mt * p->row_warps), slots = int64_t(d.sms) * (p->mt == 1 ? 3 : 2);
+    while (p->splits < 8 && tiles * p->splits * 2 <= slots && p->blocks >= 4 * p->splits) p->splits *= 2;
+    const int64_t per_cta = cdiv(p->blocks, p->splits);
+    int64_t slab = kW4MmaSlabBytes / (c.M * kW4Block * 2);
+    if (slab < 1) slab = 1;
+    if (slab > per_cta) slab = per_cta;
+    p->slab = static_cast<int>(slab);
   } else {
     int64_t piece = kW4ExpandBytes / (p->kp * (f32 ? 4 : 2)) / 256 * 256;
     if (piece < 256) piece = 256;
@@ -590,8 +668,8 @@ void plan_w4(const W4Call& c, const DeviceInfo& d, const LmInfo& lm, W4Plan* p) 
       }
       if (p->mm_bytes) p->off_mm = take(p->mm_bytes);
     } else {
-      p->columns = !rows_aligned16(c.x, c.ldx);
-      if (p->columns) p->off_x = take(size_t(c.M) * p->kp * 2);
+      p->pack_x = !rows_aligned16(c.x, c.ldx);
+      if (p->pack_x) p->off_x = take(size_t(c.M) * p->kp * 2);
       p->slices = f16_slices(c.M, p->piece, c.K, lm, &p->kb);
       p->ldslab = round_up(p->piece, 8);
       if (p->slices > 1) p->off_slabs = take(size_t(p->slices) * c.M * p->ldslab * 4);
@@ -600,14 +678,81 @@ void plan_w4(const W4Call& c, const DeviceInfo& d, const LmInfo& lm, W4Plan* p) 
   p->bytes = at;
 }
 
-template <bool BF16, int GPB>
-int launch_w4(const W4Args& a, int nt, int mt, cudaStream_t s) {
-  const int64_t tiles = cdiv(a.N, 16 * mt);
-  const dim3 grid(static_cast<unsigned>(tiles * a.splits));
-  auto go = [&](auto kern) { return launch_k(kern, grid, dim3(32 * kW4Warps), 0, s, a.splits, a); };
-  if (nt == 1) return go(w4_mma_kernel<BF16, 1, 1, GPB>);
-  if (nt == 2) return go(w4_mma_kernel<BF16, 2, 2, GPB>);
-  return go(w4_mma_kernel<BF16, 4, 2, GPB>);
+int w4_per_sm(size_t smem, int most) {
+  const int64_t n = kW4MaxSmem / (int64_t(smem) + 1024);  // 1 KB of each CTA's goes to the system
+  return static_cast<int>(n < 1 ? 1 : n > most ? most : n);
+}
+
+template <typename Kernel>
+int launch_w4_grid(Kernel kern, W4Args a, int rows, size_t smem, int most, int sms, cudaStream_t s) {
+  if (int64_t(smem) > kW4MaxSmem) return TILEC_ERR_UNSUPPORTED;
+  a.tiles = static_cast<int>(cdiv(a.N, rows));
+  int64_t clusters = int64_t(sms) * w4_per_sm(smem, most) / a.splits;
+  if (clusters > a.tiles) clusters = a.tiles;
+  return launch_k(kern, dim3(static_cast<unsigned>(clusters * a.splits)), dim3(32 * kW4Warps), smem, s, a.splits, a);
+}
+
+template <int NT, int GPB, int SC>
+int launch_w4_stream(const W4Args& w, const W4Plan& p, uint8_t* ws, cudaStream_t s) {
+  W4StreamArgs a;
+  a.w = w;
+  a.d.digits = p.cut_before ? ws + p.off_digits : nullptr;
+  a.d.pitch = p.blocks * kW4Block;
+  a.d.sums = reinterpret_cast<int*>(ws + p.off_sums);
+  a.d.scale = reinterpret_cast<float*>(ws + p.off_scale);
+  a.d.cols_pad = 8 * NT;
+  a.d.gpb = GPB;
+  a.row_tiles = static_cast<int>(cdiv(w.N, 16));
+  a.per_cta = p.per_cta;
+  a.slab = p.slab;
+  using Cfg = W4StreamCfg<NT, GPB, SC == 0>;
+  const size_t smem = size_t(Cfg::kFixed + w4_slab_bytes(p.slab, w.cols, 8 * NT, GPB));
+  if (int64_t(smem) > kW4MaxSmem) return TILEC_ERR_UNSUPPORTED;
+  if (p.cut_before)
+    TILEC_TRY(launch_k(w4_digits_kernel, dim3(static_cast<unsigned>(cdiv(int64_t(w.M) * p.blocks, 8))), dim3(128), 0, s,
+                       1, w, a.d, static_cast<int>(p.blocks)));
+  return launch_k(w4_stream_kernel<NT, GPB, SC>, dim3(static_cast<unsigned>(p.ctas)), dim3(Cfg::kThreads), smem, s,
+                  w.splits, a);
+}
+
+template <bool BF16, int NT, int MT, int GPB, bool WIDE>
+int launch_w4_mma(const W4Args& a, int sms, cudaStream_t s) {
+  using Cfg = W4Cfg<MT, GPB, WIDE>;
+  const size_t smem = size_t(Cfg::kRingBytes) + size_t(kW4Warps) * 16 * MT * 8 * NT * 4 +
+                      size_t(a.cols) * (a.slab * kW4Block + 32) * 2;
+  static_assert(Cfg::kRingBytes + kW4Warps * 16 * MT * 8 * NT * 4 + kW4MmaSlabBytes + 8 * NT * 64 <= kW4MaxSmem,
+                "shared memory");
+  return launch_w4_grid(w4_mma_kernel<BF16, NT, MT, GPB, WIDE>, a, 16 * MT * a.row_warps, smem, Cfg::kPerSm, sms, s);
+}
+
+// The kernels' variants: by columns, groups per block, type of x and scales.
+template <int GPB, bool WIDE>
+int launch_w4(const W4Args& a, const W4Plan& p, bool bf16, int sms, uint8_t* ws, cudaStream_t s) {
+  if (p.stream) {
+    auto by_columns = [&](auto sc) {
+      constexpr int SC = decltype(sc)::value;
+      return p.nt == 1   ? launch_w4_stream<1, GPB, SC>(a, p, ws, s)
+             : p.nt == 2 ? launch_w4_stream<2, GPB, SC>(a, p, ws, s)
+                         : launch_w4_stream<4, GPB, SC>(a, p, ws, s);
+    };
+    if constexpr (WIDE)
+      return by_columns(std::integral_constant<int, TILEC_DTYPE_F32>{});
+    else
+      return a.scale_bf16 ? by_columns(std::integral_constant<int, TILEC_DTYPE_BF16>{})
+                          : by_columns(std::integral_constant<int, TILEC_DTYPE_F16>{});
+  }
+  if (p.nt == 1)
+    return bf16 ? launch_w4_mma<true, 1, 1, GPB, WIDE>(a, sms, s) : launch_w4_mma<false, 1, 1, GPB, WIDE>(a, sms, s);
+  if (p.nt == 2)
+    return bf16 ? launch_w4_mma<true, 2, 2, GPB, WIDE>(a, sms, s) : launch_w4_mma<false, 2, 2, GPB, WIDE>(a, sms, s);
+  return bf16 ? launch_w4_mma<true, 4, 2, GPB, WIDE>(a, sms, s) : launch_w4_mma<false, 4, 2, GPB, WIDE>(a, sms, s);
+}
+
+template <bool WIDE>
+int launch_w4(const W4Args& a, const W4Plan& p, int gpb, bool bf16, int sms, uint8_t* ws, cudaStream_t s) {
+  return gpb == 4   ? launch_w4<4, WIDE>(a, p, bf16, sms, ws, s)
+         : gpb == 2 ? launch_w4<2, WIDE>(a, p, bf16, sms, ws, s)
+                    : launch_w4<1, WIDE>(a, p, bf16, sms, ws, s);
 }
 
 int run_w4(const W4Call& c, void* workspace, size_t ws_bytes, cudaStream_t s) {
@@ -621,44 +766,32 @@ int run_w4(const W4Call& c, void* workspace, size_t ws_bytes, cudaStream_t s) {
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const bool f32 = c.dtype == TILEC_DTYPE_F32;
   W4Args a = {};
-  a.codes = static_cast<const uint4*>(c.codes);
-  a.scales = c.scales;
-  a.zeros = c.zeros;
-  a.sdt = c.sdt;
+  a.data = static_cast<const uint8_t*>(c.weight);
+  a.wide = c.sdt == TILEC_DTYPE_F32;
+  a.scale_bf16 = c.sdt == TILEC_DTYPE_BF16;
   a.N = static_cast<int>(c.N);
+  a.K = static_cast<int>(c.K);
   a.blocks = static_cast<int>(p.blocks);
-  a.group_blocks = c.group >= kW4Block ? static_cast<int>(c.group / kW4Block) : 1;
   const int gpb = c.group == 32 ? 4 : c.group == 64 ? 2 : 1;
-  if (p.stream) {
-    a.x = static_cast<const unsigned short*>(c.x);
+  if (p.stream || p.mma) {
+    a.x = c.x;
     a.ldx = c.ldx;
-    a.parts = p.parts;
-    a.cols = static_cast<int>(c.M * p.parts);
+    a.dtype = c.dtype;
     a.M = static_cast<int>(c.M);
+    a.cols = static_cast<int>(c.M * (p.stream ? kW4Digits : 1));
+    a.vec_x = !f32 && rows_aligned16(c.x, c.ldx);
     a.out = c.out;
     a.ldo = c.ldo;
-    a.odt = c.dtype;
     a.bias = c.bias;
     a.splits = p.splits;
-    if (p.columns) {
-      unsigned short* xc = reinterpret_cast<unsigned short*>(ws + p.off_x);
-      TILEC_TRY(launch_k(w4_columns_kernel, dim3(static_cast<unsigned>(cdiv(p.kp, 2048)), static_cast<unsigned>(c.M)),
-                         dim3(256), 0, s, 1, c.x, c.ldx, static_cast<int>(c.K), f32 ? 1 : 0, xc, p.kp));
-      a.x = xc;
-      a.ldx = p.kp;
-    }
-    const bool bf16 = c.dtype != TILEC_DTYPE_F16;
-    if (bf16)
-      return gpb == 4   ? launch_w4<true, 4>(a, p.nt, p.mt, s)
-             : gpb == 2 ? launch_w4<true, 2>(a, p.nt, p.mt, s)
-                        : launch_w4<true, 1>(a, p.nt, p.mt, s);
-    return gpb == 4   ? launch_w4<false, 4>(a, p.nt, p.mt, s)
-           : gpb == 2 ? launch_w4<false, 2>(a, p.nt, p.mt, s)
-                      : launch_w4<false, 1>(a, p.nt, p.mt, s);
+    a.row_warps = p.row_warps;
+    a.slab = p.slab;
+    const bool bf16 = c.dtype == TILEC_DTYPE_BF16;
+    return a.wide ? launch_w4<true>(a, p, gpb, bf16, d->sms, ws, s) : launch_w4<false>(a, p, gpb, bf16, d->sms, ws, s);
   }
   const void* x = c.x;
   int64_t ldx = c.ldx;
-  if (p.columns) {
+  if (p.pack_x) {
     TILEC_TRY(pack16(c.x, c.ldx, ws + p.off_x, p.kp, c.M, c.K, nullptr, nullptr, nullptr, 0, nullptr, *d, s));
     x = ws + p.off_x;
     ldx = p.kp;
@@ -733,9 +866,10 @@ int tilec_linear_ce_backward(const void* x, const void* w, const int64_t* target
   return ce_backward(c, stats, grad, dx, dw, workspace, ws_bytes, static_cast<cudaStream_t>(stream));
 }
 
-size_t tilec_mm_w4_workspace_bytes(const void* x, int32_t dtype, int64_t M, int64_t ldx, int64_t N, int64_t K,
-                                   int64_t group, const void* out, int64_t ldo) {
+size_t tilec_mm_w4_workspace_bytes(const void* x, int32_t dtype, int64_t M, int64_t ldx, int32_t scale_dtype,
+                                   int64_t N, int64_t K, int64_t group, const void* out, int64_t ldo) {
   W4Call c = {};
+  c.sdt = scale_dtype;
   c.x = x ? x : reinterpret_cast<const void*>(256);
   c.dtype = dtype;
   c.M = M;
@@ -754,10 +888,10 @@ size_t tilec_mm_w4_workspace_bytes(const void* x, int32_t dtype, int64_t M, int6
   return p.bytes;
 }
 
-int tilec_mm_w4(const void* x, int32_t dtype, int64_t M, int64_t ldx, const void* codes, const void* scales,
-                int32_t scale_dtype, const uint8_t* zeros, int64_t N, int64_t K, int64_t group, const void* bias,
-                void* out, int64_t ldo, void* workspace, size_t ws_bytes, void* stream) {
-  const W4Call c{x, dtype, M, ldx, codes, scales, scale_dtype, zeros, N, K, group, bias, out, ldo};
+int tilec_mm_w4(const void* x, int32_t dtype, int64_t M, int64_t ldx, const void* weight,
+                int32_t scale_dtype, int64_t N, int64_t K, int64_t group, const void* bias, void* out, int64_t ldo,
+                void* workspace, size_t ws_bytes, void* stream) {
+  const W4Call c{x, dtype, M, ldx, weight, scale_dtype, N, K, group, bias, out, ldo};
   int rc = check_w4(c);
   if (rc) return rc;
   rc = check_w4_pointers(c);

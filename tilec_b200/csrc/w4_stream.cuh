@@ -1,0 +1,494 @@
+// w4_stream.cuh -- the few-rows product with 4-bit weights on the integer tensor path.
+//
+// One token's product reads N * K / 2 bytes of codes and is bound by memory, if only the
+// arithmetic keeps up: at 6.5 TB/s a quarter SM has about 180 cycles per 1 KB of codes (16
+// rows x 128 k).  On the 16-bit path (w4_mma_kernel) a code costs 1.4 instructions to become
+// a 16-bit float, most of them on the half-rate integer pipe: 28672 x 8192 took 40 us.  An
+// 8-bit operand needs 3 for 8 codes, and m16n8k32 takes twice the k at the same rate:
+//
+//   * per 128-k block and row, x becomes whole numbers X = round(x * 2^(29 - e)), 2^e <= the
+//     block's largest magnitude < 2^(e + 1), in four signed 8-bit digits: x is off by at most
+//     2^-30 of 2^e, which is exact for 16-bit types wherever the magnitude is within 2^-22
+//     (bf16) or 2^-19 (fp16) of that, and below the rounding of an fp32 sum;
+//   * each digit is one column of the tensor-core product, so sums over a group are exact
+//     32-bit integers: sum code * X - zero * sum X;
+//   * that times scale * 2^(e - 29) * 256^digit is added in fp32.
+//
+// The sums start at 0x4B400000 - zero * sum X: read as a float that is 1.5 * 2^23 + the sum
+// (|sum| < 2^22), which saves the conversions.
+//
+// One CTA per SM, persistent, with 24 warps that share one copy of x.  A CTA takes an equal
+// run of 16-row tiles, and its warps equal runs of their pieces (16 rows x 128 k): a warp's
+// run is one run of memory too, streamed through a ring of its own in shared memory by bulk
+// copies of two pieces each, so that 150 KB are on their way to an SM at any time.  Where a
+// tile is shared by several warps their sums meet in shared memory, in the order of K.
+//
+// x is cut by the CTAs themselves where that is little work (one or two rows), otherwise once,
+// by w4_digits_kernel; w4_stream_kernel then starts its first copies of the weight while x is
+// still being cut: it is launched with programmatic serialisation, and w4_digits_kernel lets
+// it go only after everything before has completed.
+//
+// Measured, 28672 x 8192, one token (125 MB): 27.8 us, 4.5 TB/s; loads alone take 25 in the
+// best of the forms tried.  On the way: rows of codes with the group words apart 35 to 40 us
+// (the words alone cost 6); 24 warps with copies of two pieces 30.5; 12 warps 30.3; CTAs of
+// 128 rows, two waves of them for want of one slot, 40.
+#pragma once
+
+#include "w4.cuh"
+
+namespace tilec {
+
+constexpr int kW4StreamWarps = 16;
+constexpr int kW4Digits = 4;      // columns per row of x
+constexpr int kW4GroupTiles = 16; // row tiles whose sums a CTA holds at a time
+
+// The digits of x, in the workspace or (same layout) in shared memory; zeros past K.
+struct W4Digits {
+  uint8_t* digits;   // [col][pitch], 128 bytes a block, [t][j][8]: 8 consecutive k in the order 0 4 1 5 2 6 3 7
+  int64_t pitch;
+  int* sums;         // [block][group][8 NT]: minus the sum of a column's digits over a group
+  float* scale;      // [block][8 NT]: 2^(e - 29) * 256^digit
+  int cols_pad;      // 8 NT; columns are 4 * row + digit, the smallest first
+  int gpb;           // groups per block
+};
+
+struct W4StreamArgs {
+  W4Args w;          // the weight, x (to be cut, and for outputs that are not finite), bias and out
+  W4Digits d;        // workspace; digits == nullptr: the CTAs cut x themselves
+  int row_tiles;
+  int per_cta;       // blocks of K a CTA takes; a cluster's CTAs follow one another along K
+  int slab;          // blocks of x in shared memory at a time
+};
+
+template <int NT, int GPB, bool WIDE>
+struct W4StreamCfg {
+  static constexpr int kThreads = 32 * kW4StreamWarps;
+  static constexpr int kPiece = w4_piece_bytes(GPB, WIDE);
+  // Pieces a copy.  An SM's bulk copies start some 60 ns apart, so few large ones keep up with
+  // HBM; with more columns x needs the room.
+  static constexpr int kRun = NT == 1 && kPiece <= 1152 ? 4 : 2;
+  static constexpr int kStage = kRun * kPiece;
+  static constexpr int kStages = 2;
+  static constexpr int kRingBytes = kW4StreamWarps * kStages * kStage;
+  static constexpr int kPart = 2 * NT * 16;  // floats: the sums of a row tile, [row of x][16]
+  static constexpr int kSumBytes = kW4GroupTiles * kPart * 4;
+  static constexpr int kPartBytes = 2 * kW4StreamWarps * kPart * 4;
+  static constexpr int kBarBytes = 1024;     // a barrier per warp and stage, the abort flag
+  static constexpr int kFixed = kRingBytes + kSumBytes + kPartBytes + kBarBytes;
+  static_assert(kStage % 128 == 0 && (kW4StreamWarps * kStages + 1) * 8 <= kBarBytes, "shared memory layout");
+};
+// Bytes of `slab` blocks of x: digits (16 bytes more a column: conflict-free reads), sums, scales.
+__host__ __device__ inline int64_t w4_slab_bytes(int64_t slab, int cols, int cols_pad, int gpb) {
+  return cols * (slab * kW4Block + 16) + slab * cols_pad * 4 * (gpb + 1);
+}
+
+// Sixteen lanes (l = 0 .. 15) cut one 128-k block of one row of x; all lanes of a warp call.
+// `at`: where the block goes in d.
+__device__ __forceinline__ void w4_cut(const W4Args& p, const W4Digits& d, bool live, int m, int blk, int at, int l) {
+  constexpr int shift = 29;
+  const int j = l >> 2, t = l & 3;
+  const int k0 = blk * kW4Block + 8 * l;
+  float v[8];
+  if (p.dtype == 0) {
+    const float* s = static_cast<const float*>(p.x) + m * p.ldx + k0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = live && k0 + i < p.K ? s[i] : 0.f;
+  } else {
+    const unsigned short* s = static_cast<const unsigned short*>(p.x) + m * p.ldx + k0;
+    uint32_t w[4] = {0, 0, 0, 0};
+    if (live && p.vec_x && k0 + 8 <= p.K) {
+      const uint4 h = *reinterpret_cast<const uint4*>(s);
+      w[0] = h.x; w[1] = h.y; w[2] = h.z; w[3] = h.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (live && k0 + i < p.K) w[i >> 1] |= uint32_t(s[i]) << (16 * (i & 1));
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (p.dtype == 2) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+      } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+      }
+    }
+  }
+  uint32_t top = 0;  // the largest magnitude, as bits: infinities and NaN come out on top
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+  // 2^-90 and below share one step (2^(shift + 90) still is a float).
+  const int e = max(static_cast<int>(top >> 23) - 127, -90);
+  const float up = __uint_as_float(static_cast<uint32_t>(127 + shift - e) << 23);
+  uint32_t y[8];  // X + 0x80 in every byte: bytes, less 0x80 each, are the digits
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float s = v[i] * up;
+    y[i] = static_cast<uint32_t>(__float2int_rn(s)) + 0x80808080u;
+  }
+  // 2^(e - shift) * 256^part; a block with anything not finite makes its sums NaN, and the
+  // outputs are then computed one by one (w4_output).
+  const float down = top >= 0x7F800000u ? __int_as_float(0x7fc00000)
+                                        : __uint_as_float(static_cast<uint32_t>(127 + e - shift) << 23);
+#pragma unroll
+  for (int part = 0; part < kW4Digits; ++part) {
+    const uint32_t sel = part | (4 + part) << 4;
+    auto gather = [&](int a, int b, int c, int e) {
+      return __byte_perm(__byte_perm(y[a], y[b], sel), __byte_perm(y[c], y[e], sel), 0x5410) ^ 0x80808080u;
+    };
+    const uint32_t d0 = gather(0, 4, 1, 5), d1 = gather(2, 6, 3, 7);
+    int sum = __dp4a(static_cast<int>(d0), 0x01010101, __dp4a(static_cast<int>(d1), 0x01010101, 0));
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    int other = __shfl_xor_sync(0xffffffffu, sum, 4);
+    if (d.gpb <= 2) sum += other;
+    other = __shfl_xor_sync(0xffffffffu, sum, 8);
+    if (d.gpb == 1) sum += other;
+    if (!live) continue;
+    const int col = m * kW4Digits + part;
+    *reinterpret_cast<uint2*>(d.digits + col * d.pitch + at * kW4Block + t * 32 + j * 8) = make_uint2(d0, d1);
+    if (t == 0 && j % (4 / d.gpb) == 0)
+      d.sums[(at * d.gpb + j / (4 / d.gpb)) * d.cols_pad + col] = -sum;
+    if (l == 0) d.scale[at * d.cols_pad + col] = down * __uint_as_float(static_cast<uint32_t>(127 + 8 * part) << 23);
+  }
+}
+
+// Cuts all of x, 8 blocks a CTA.
+__global__ void __launch_bounds__(128) w4_digits_kernel(const __grid_constant__ W4Args p,
+                                                        const __grid_constant__ W4Digits d, int nblocks) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int task = static_cast<int>(blockIdx.x) * 8 + (threadIdx.x >> 4);
+  const bool live = task < p.M * nblocks;
+  const int m = live ? task / nblocks : 0, blk = live ? task - m * nblocks : 0;
+  w4_cut(p, d, live, m, blk, blk, threadIdx.x & 15);
+}
+
+// One output from its definition, in fp32 and k order.
+__device__ __noinline__ float w4_output(const W4Args& p, int gpb, int n, int m) {
+  float v = 0.f;
+  const int wb = w4_word_bytes(gpb, p.wide);
+  for (int k = 0; k < p.K; ++k) {
+    const int b = k / kW4Block, kk = k % kW4Block;
+    const uint8_t* piece = p.data + (int64_t(n >> 4) * p.blocks + b) * w4_piece_bytes(gpb, p.wide);
+    const uint32_t code =
+        reinterpret_cast<const uint32_t*>(piece + 16 * wb + (n & 15) * 64)[(kk >> 3 & 3) * 4 + (kk >> 5)];
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(piece + (n & 15) * wb) + (kk * gpb / kW4Block) * (p.wide ? 2 : 1);
+    const float s = p.wide ? __uint_as_float(w[1]) : w4_scale16(w[0], p.scale_bf16);
+    const float q = float((code >> (4 * (kk >> 1 & 3) + 16 * (kk & 1))) & 15u) - float(w[0] & 15u);
+    v += load_as_float(p.x, m * p.ldx + k, p.dtype) * (q * s);
+  }
+  return v;
+}
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                   smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+
+// Shared memory by its 32-bit address: one register and an immediate where generic pointers
+// cost two registers and their arithmetic.
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  return v;
+}
+template <int WORDS>
+__device__ __forceinline__ void lds_words(uint32_t (&w)[WORDS], uint32_t a) {
+  if constexpr (WORDS == 1) {
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(a));
+  } else if constexpr (WORDS == 2) {
+    const uint2 v = lds64(a);
+    w[0] = v.x; w[1] = v.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < WORDS; i += 4) {
+      const uint4 v = lds128(a + 4 * i);
+      w[i] = v.x; w[i + 1] = v.y; w[i + 2] = v.z; w[i + 3] = v.w;
+    }
+  }
+}
+
+// SC: type of the scales (TILEC_DTYPE_*).
+// Grid: x = CTAs (clusters of `splits`, whose CTAs share their row tiles and split K).
+template <int NT, int GPB, int SC>
+__global__ void __launch_bounds__(32 * kW4StreamWarps, 1) w4_stream_kernel(const __grid_constant__ W4StreamArgs a) {
+  constexpr bool WIDE = SC == 0;
+  using Cfg = W4StreamCfg<NT, GPB, WIDE>;
+  constexpr int COLS = 8 * NT, WB = w4_word_bytes(GPB, WIDE), T = Cfg::kThreads, S = Cfg::kStages, W = kW4StreamWarps;
+  extern __shared__ __align__(128) uint8_t w4_smem[];
+  const W4Args& p = a.w;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint8_t* ring = w4_smem + warp * (S * Cfg::kStage);
+  float* tile_sums = reinterpret_cast<float*>(w4_smem + Cfg::kRingBytes);                  // [tile of the group][kPart]
+  float* parts = reinterpret_cast<float*>(w4_smem + Cfg::kRingBytes + Cfg::kSumBytes);     // [warp][first, last][kPart]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(w4_smem + Cfg::kFixed - Cfg::kBarBytes) + warp * S;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(w4_smem + Cfg::kFixed - 8);
+  const int pitch = a.slab * kW4Block + 16;
+  W4Digits d = a.d;                                // the slab in shared memory
+  d.digits = w4_smem + Cfg::kFixed;
+  d.pitch = pitch;
+  d.sums = reinterpret_cast<int*>(d.digits + p.cols * pitch);
+  d.scale = reinterpret_cast<float*>(d.sums + a.slab * GPB * COLS);
+  const int g = lane >> 2, t = lane & 3;
+  const int rank = p.splits > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  const int cluster = static_cast<int>(blockIdx.x) / p.splits, clusters = static_cast<int>(gridDim.x) / p.splits;
+  const int b_begin = min(p.blocks, rank * a.per_cta), b_end = min(p.blocks, b_begin + a.per_cta);
+  const int tile_begin = static_cast<int>(int64_t(a.row_tiles) * cluster / clusters);
+  const int tile_end = static_cast<int>(int64_t(a.row_tiles) * (cluster + 1) / clusters);
+  const bool cut_here = a.d.digits == nullptr;
+  if (lane == 0) {
+    for (int i = 0; i < S; ++i) mbar_init(&bars[i], 1);
+    if (warp == 0) *abort_flag = 0;
+    fence_barrier_init();
+  }
+  __syncthreads();
+  if (cut_here) pdl_wait();  // otherwise w4_digits_kernel has: what came before it is complete
+
+  float total[NT][4];
+  // 32-bit shared addresses; columns past the last one repeat it, their sums are never read.
+  const uint32_t ring_at = smem_u32(ring), lane_codes = 16 * WB + lane * 16, lane_words = g * WB;
+  uint32_t x_col[NT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i) x_col[i] = smem_u32(d.digits) + min(8 * i + g, p.cols - 1) * pitch + 32 * t;
+  const uint32_t sums_at = smem_u32(d.sums) + 8 * t, scale_at = smem_u32(d.scale) + 8 * t;
+
+  auto multiply = [&](uint32_t piece, int blk) {  // `blk`: the piece's block within the slab
+    const uint4 qa = lds128(piece + lane_codes), qb = lds128(piece + lane_codes + 512);
+    uint32_t wa[WB / 4], wb[WB / 4];
+    lds_words(wa, piece + lane_words);
+    lds_words(wb, piece + lane_words + 8 * WB);
+    uint4 x[NT][2];
+    uint2 xs[NT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      x[i][0] = lds128(x_col[i] + blk * kW4Block);
+      x[i][1] = lds128(x_col[i] + blk * kW4Block + 16);
+      xs[i] = lds64(scale_at + blk * (COLS * 4) + 32 * i);
+    }
+    int acc[NT][4];
+    float sa = 0.f, sb = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      constexpr int kSteps = 4 / GPB;  // words of codes per group
+      if (j % kSteps == 0) {
+        const int k = j / kSteps;
+        const uint32_t ga = wa[WIDE ? 2 * k : k], gb = wb[WIDE ? 2 * k : k];
+        const int za = static_cast<int>(ga & 15u), zb = static_cast<int>(gb & 15u);
+        if constexpr (WIDE) {
+          sa = __uint_as_float(wa[2 * k + 1]);
+          sb = __uint_as_float(wb[2 * k + 1]);
+        } else {
+          sa = w4_scale16(ga, SC == 2);
+          sb = w4_scale16(gb, SC == 2);
+        }
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          const uint2 sx = lds64(sums_at + (blk * GPB + k) * (COLS * 4) + 32 * i);
+          acc[i][0] = 0x4B400000 + za * static_cast<int>(sx.x);
+          acc[i][1] = 0x4B400000 + za * static_cast<int>(sx.y);
+          acc[i][2] = 0x4B400000 + zb * static_cast<int>(sx.x);
+          acc[i][3] = 0x4B400000 + zb * static_cast<int>(sx.y);
+        }
+      }
+      const uint32_t ca = j == 0 ? qa.x : j == 1 ? qa.y : j == 2 ? qa.z : qa.w;
+      const uint32_t cb = j == 0 ? qb.x : j == 1 ? qb.y : j == 2 ? qb.z : qb.w;
+      const uint32_t a0 = ca & 0x0F0F0F0Fu, a2 = (ca >> 4) & 0x0F0F0F0Fu;
+      const uint32_t a1 = cb & 0x0F0F0F0Fu, a3 = (cb >> 4) & 0x0F0F0F0Fu;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        const uint4 xv = x[i][j >> 1];
+        const uint32_t b_lo = j & 1 ? xv.z : xv.x, b_hi = j & 1 ? xv.w : xv.y;
+        asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+            "{%0, %1, %2, %3};"
+            : "+r"(acc[i][0]), "+r"(acc[i][1]), "+r"(acc[i][2]), "+r"(acc[i][3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b_lo), "r"(b_hi));
+      }
+      if ((j + 1) % kSteps == 0) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          const float x0 = __uint_as_float(xs[i].x), x1 = __uint_as_float(xs[i].y);
+          total[i][0] = fmaf(__int_as_float(acc[i][0]) - 12582912.f, sa * x0, total[i][0]);
+          total[i][1] = fmaf(__int_as_float(acc[i][1]) - 12582912.f, sa * x1, total[i][1]);
+          total[i][2] = fmaf(__int_as_float(acc[i][2]) - 12582912.f, sb * x0, total[i][2]);
+          total[i][3] = fmaf(__int_as_float(acc[i][3]) - 12582912.f, sb * x1, total[i][3]);
+        }
+      }
+    }
+  };
+
+  int stage = 0;
+  uint32_t phase = 0;
+  bool ok = true, waited = false;
+  const bool whole_x = b_end - b_begin <= a.slab;
+  for (int group = tile_begin; group < tile_end; group += kW4GroupTiles) {
+    const int ntiles = min(kW4GroupTiles, tile_end - group);
+    for (int s0 = b_begin; s0 == b_begin || s0 < b_end; s0 += a.slab) {
+      const int n = max(0, min(a.slab, b_end - s0));  // blocks of K in work
+      // This warp's run of the slab's pieces, tile by tile.
+      const int pieces = ntiles * n, share = (pieces + W - 1) / W;
+      const int first = min(pieces, warp * share), last = min(pieces, first + share);
+      const int first_tile = n > 0 ? first / n : 0, first_blk = first - first_tile * n;
+      // Up to kRun pieces of one tile follow one another in memory and go out in one copy.
+      int f_left = last - first, f_blk = first_blk, fill = stage;
+      const uint8_t* f_src =
+          p.data + (static_cast<int64_t>(group + first_tile) * p.blocks + s0 + f_blk) * Cfg::kPiece;
+      const int64_t skip = static_cast<int64_t>(p.blocks - n) * Cfg::kPiece;  // from a tile's slab to the next one's
+      auto fetch = [&]() {
+        if (f_left <= 0) return;
+        const int run = min(Cfg::kRun, min(f_left, n - f_blk));
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&bars[fill], run * Cfg::kPiece);
+          bulk_load(ring + fill * Cfg::kStage, f_src, run * Cfg::kPiece, &bars[fill]);
+        }
+        fill = fill == S - 1 ? 0 : fill + 1;
+        f_left -= run;
+        f_blk += run;
+        f_src += run * Cfg::kPiece;
+        if (f_blk == n) {
+          f_blk = 0;
+          f_src += skip;
+        }
+      };
+#pragma unroll
+      for (int i = 0; i < S; ++i) fetch();
+      if (!waited) {
+        pdl_wait();
+        pdl_launch_dependents();
+        waited = true;
+      }
+      if (!whole_x || (group == tile_begin && s0 == b_begin)) {
+        if (cut_here) {
+          for (int base = 0; base < p.M * n; base += T / 16) {
+            const int task = base + (threadIdx.x >> 4);
+            const bool live = task < p.M * n;
+            const int m = live ? task / n : 0, at = live ? task - m * n : 0;
+            w4_cut(p, d, live, m, s0 + at, at, threadIdx.x & 15);
+          }
+        } else {
+          for (int c = warp; c < p.cols; c += W) {
+            const uint8_t* src = a.d.digits + c * a.d.pitch + static_cast<int64_t>(s0) * kW4Block;
+            for (int k = lane * 16; k < n * kW4Block; k += 512) cp_async_16(d.digits + c * pitch + k, src + k, 16);
+          }
+          const int* src_sums = a.d.sums + static_cast<int64_t>(s0) * GPB * COLS;
+          for (int i = threadIdx.x * 4; i < n * GPB * COLS; i += T * 4) cp_async_16(d.sums + i, src_sums + i, 16);
+          const float* src_scale = a.d.scale + static_cast<int64_t>(s0) * COLS;
+          for (int i = threadIdx.x * 4; i < n * COLS; i += T * 4) cp_async_16(d.scale + i, src_scale + i, 16);
+          cp_async_commit();
+          cp_async_wait<0>();
+        }
+      }
+      if (s0 == b_begin)
+        for (int i = threadIdx.x; i < ntiles * Cfg::kPart; i += T) tile_sums[i] = 0.f;
+      __syncthreads();
+
+      // A row tile's sums are complete, or as far as this warp goes.
+      auto leave = [&](int tile, bool whole, int which) {
+        float* dst = whole ? tile_sums + tile * Cfg::kPart : parts + (2 * warp + which) * Cfg::kPart;
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          // Digits of one row of x: two columns here, two in the neighbouring lane.
+          float v0 = total[i][0] + total[i][1], v1 = total[i][2] + total[i][3];
+          v0 += __shfl_xor_sync(0xffffffffu, v0, 1);
+          v1 += __shfl_xor_sync(0xffffffffu, v1, 1);
+          if ((t & 1) == 0) {
+            float* r = dst + (2 * i + (t >> 1)) * 16 + g;
+            r[0] = whole ? r[0] + v0 : v0;
+            r[8] = whole ? r[8] + v1 : v1;
+          }
+          total[i][0] = total[i][1] = total[i][2] = total[i][3] = 0.f;
+        }
+      };
+#pragma unroll
+      for (int i = 0; i < NT; ++i) total[i][0] = total[i][1] = total[i][2] = total[i][3] = 0.f;
+      int tile = first_tile, blk = first_blk;
+      bool from_start = blk == 0;   // this warp has the tile's first block
+      for (int at = first; at < last && ok;) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&bars[stage], phase, abort_flag));
+        if (!ok) break;
+        const uint32_t piece = ring_at + stage * Cfg::kStage;
+        const int run = min(Cfg::kRun, min(last - at, n - blk));
+#pragma unroll
+        for (int i = 0; i < Cfg::kRun; ++i)
+          if (i < run) multiply(piece + i * Cfg::kPiece, blk + i);
+        __syncwarp();  // every lane has read the stage
+        fetch();
+        if (++stage == S) {
+          stage = 0;
+          phase ^= 1;
+        }
+        at += run;
+        blk += run;
+        if (blk == n) {
+          leave(tile, from_start, tile == first_tile ? 0 : 1);
+          ++tile;
+          blk = 0;
+          from_start = true;
+        }
+      }
+      if (ok && first < last && blk > 0) leave(tile, false, tile == first_tile ? 0 : 1);
+      if (!ok) {  // gave up: let what is on its way land, and leave NaN
+        for (int i = 0; i < S; ++i) mbar_drain(&bars[i], i >= stage ? phase : phase ^ 1);
+        for (int i = lane; i < 2 * Cfg::kPart; i += 32) parts[2 * warp * Cfg::kPart + i] = __int_as_float(0x7fc00000);
+        for (int k = first; k < last; k = (k / n + 1) * n)
+          for (int i = lane; i < Cfg::kPart; i += 32) tile_sums[k / n * Cfg::kPart + i] = __int_as_float(0x7fc00000);
+      }
+      __syncthreads();
+      // Tiles that several warps share: the first of them adds the parts, in the order of K.
+      if (first < last) {
+        auto gather = [&](int tl) {
+          const int lo = tl * n, hi = lo + n;
+          if (first > lo || last >= hi) return;  // an earlier warp leads, or this one had it whole
+          for (int i = lane; i < Cfg::kPart; i += 32) {
+            float v = tile_sums[tl * Cfg::kPart + i];
+            for (int w = warp; w < W && w * share < hi; ++w)  // w's first tile, unless it starts before
+              v += parts[(2 * w + (w * share >= lo ? 0 : 1)) * Cfg::kPart + i];
+            tile_sums[tl * Cfg::kPart + i] = v;
+          }
+        };
+        gather(first_tile);
+        const int last_tile = (last - 1) / n;
+        if (last_tile != first_tile) gather(last_tile);
+      }
+      __syncthreads();
+    }
+
+    // Outputs of the group's tiles, from all CTAs' sums of a cluster.
+    if (p.splits > 1) cluster_sync();
+    const int count = ntiles * 16 * p.M;
+    for (int i = rank * T + threadIdx.x; i < count; i += p.splits * T) {
+      const int r = i & 15, m = (i >> 4) % p.M, tl = (i >> 4) / p.M, at = tl * Cfg::kPart + m * 16 + r;
+      const int row = (group + tl) * 16 + r;
+      if (row >= p.N) continue;
+      float v = 0.f;
+      if (p.splits == 1) {
+        v = tile_sums[at];
+      } else {
+        const uint32_t addr = smem_u32(tile_sums + at);
+        for (int c = 0; c < p.splits; ++c) {
+          float u;
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(u) : "r"(mapa_shared(addr, c)) : "memory");
+          v += u;
+        }
+      }
+      if (v != v) v = w4_output(p, GPB, row, m);
+      if (p.bias != nullptr) v += load_as_float(p.bias, row, p.dtype);
+      store_from_float(p.out, int64_t(m) * p.ldo + row, p.dtype, v);
+    }
+    if (p.splits > 1) cluster_sync();  // every CTA's sums have been read
+    else __syncthreads();
+  }
+}
+
+}  // namespace tilec

@@ -152,40 +152,59 @@ def _check_group(group_size, where):
 class W4Weight:
     """A weight [N, K] in 4-bit codes, laid out for matrix_mul_w4 (see pack_w4).
 
-    shape (N, K); group_size; codes uint8 [N, blocks * 64]; scales [groups, N]; zeros uint8
-    [groups, N] or None (every zero point is 8).  The tensors may be moved together with
-    to(device); matrix_mul_w4 reads them in place."""
+    shape (N, K); group_size; scale_dtype; data uint8 [row tiles of 16, blocks of 128 k, bytes]:
+    each piece's group words, then its codes (tilec_mm_w4 in include/tilec_mm.h).
+    matrix_mul_w4 reads it in place."""
 
-    def __init__(self, shape, group_size, codes, scales, zeros):
-        self.shape, self.group_size = tuple(shape), group_size
-        self.codes, self.scales, self.zeros = codes, scales, zeros
+    def __init__(self, shape, group_size, scale_dtype, data):
+        self.shape, self.group_size, self.scale_dtype, self.data = tuple(shape), group_size, scale_dtype, data
 
     @property
     def device(self):
-        return self.codes.device
+        return self.data.device
 
     def to(self, device):
-        zeros = None if self.zeros is None else self.zeros.to(device)
-        return W4Weight(self.shape, self.group_size, self.codes.to(device), self.scales.to(device), zeros)
+        return W4Weight(self.shape, self.group_size, self.scale_dtype, self.data.to(device))
 
     def unpack(self):
         """The codes as uint8 [N, K], one per byte, in k order."""
         n, k = self.shape
-        w = self.codes.view(n, -1, 4, 4, 4)                        # block, t, j, byte of the word
+        codes = self.data[:, :, -1024:].reshape(*self.data.shape[:2], 16, 64)
+        w = codes.transpose(1, 2).reshape(-1, self.data.shape[1], 4, 4, 4)   # row, block, t, j, byte of the word
         nib = torch.stack((w & 15, w >> 4), -1).flatten(-2)        # nibbles 0..7 of the word
         nib = nib.view(*nib.shape[:-1], 2, 4).transpose(-1, -2)    # (i, parity): k = 2i + parity
-        return nib.flatten(-2).transpose(2, 3).reshape(n, -1)[:, :k]
+        return nib.flatten(-2).transpose(2, 3).reshape(-1, self.data.shape[1] * _BLOCK)[:n, :k]
+
+    def _words(self):
+        """The group words as int32 [N, groups, 1 or 2]."""
+        n, k = self.shape
+        tiles, blocks = self.data.shape[:2]
+        wide = 2 if self.scale_dtype == torch.float32 else 1
+        words = self.data[:, :, :-1024].contiguous().view(torch.int32).view(tiles, blocks, 16, -1, wide)
+        words = words.transpose(1, 2).reshape(tiles * 16, -1, wide)[:n, ::max(1, self.group_size // _BLOCK)]
+        return words[:, :-(-k // self.group_size)]
+
+    def scales(self):
+        """[N, ceil(K / group_size)], as given."""
+        words = self._words()
+        if self.scale_dtype == torch.float32:
+            return words[..., 1].contiguous().view(torch.float32)
+        return (words[..., 0] >> 16).to(torch.int16).view(self.scale_dtype)
+
+    def zeros(self):
+        """[N, ceil(K / group_size)] uint8."""
+        return (self._words()[..., 0] & 15).to(torch.uint8)
 
     def dequantize(self):
         """(code - zero) * scale as float32 [N, K]."""
-        n, k = self.shape
-        scales = self.scales.float().t().repeat_interleave(self.group_size, 1)[:, :k]
-        zeros = 8.0 if self.zeros is None else self.zeros.float().t().repeat_interleave(self.group_size, 1)[:, :k]
+        k = self.shape[1]
+        scales = self.scales().float().repeat_interleave(self.group_size, 1)[:, :k]
+        zeros = self.zeros().float().repeat_interleave(self.group_size, 1)[:, :k]
         return (self.unpack().float() - zeros) * scales
 
     def __repr__(self):
-        return (f"W4Weight(shape={self.shape}, group_size={self.group_size}, scales={self.scales.dtype}, "
-                f"zeros={self.zeros is not None}, device={self.device})")
+        return (f"W4Weight(shape={self.shape}, group_size={self.group_size}, scales={self.scale_dtype}, "
+                f"device={self.device})")
 
 
 def pack_w4(codes, scales, zeros=None, group_size=128):
@@ -215,20 +234,24 @@ def pack_w4(codes, scales, zeros=None, group_size=128):
         raise ValueError("pack_w4: codes, scales and zeros must be on one device")
     if n and (int(codes.max()) > 15 or (zeros is not None and int(zeros.max()) > 15)):
         raise ValueError("pack_w4: codes and zeros must be 0..15")
-    blocks = -(-k // _BLOCK)
-    if k % _BLOCK:
-        codes = torch.nn.functional.pad(codes, (0, blocks * _BLOCK - k))
-    c = codes.reshape(n, blocks, 4, 4, 4, 2)           # j, t, i, parity: k = 32j + 8t + 2i + parity
-    c = c.permute(0, 1, 3, 2, 5, 4).reshape(n, blocks, 4, 4, 4, 2)   # t, j, then nibbles 4 * parity + i
-    packed = (c[..., 0] | c[..., 1] << 4).reshape(n, blocks * 64)
-    rows = -(-blocks * _BLOCK // group_size)
-
-    def by_group(t):
-        out = torch.zeros(rows, n, dtype=t.dtype, device=t.device)
-        out[:groups] = t.t()
-        return out
-
-    return W4Weight((n, k), group_size, packed, by_group(scales), None if zeros is None else by_group(zeros))
+    blocks, tiles = -(-k // _BLOCK), -(-n // 16)
+    pad = torch.nn.functional.pad
+    codes = pad(codes, (0, blocks * _BLOCK - k, 0, tiles * 16 - n))
+    c = codes.reshape(-1, blocks, 4, 4, 4, 2)          # j, t, i, parity: k = 32j + 8t + 2i + parity
+    c = c.permute(0, 1, 3, 2, 5, 4).reshape(tiles, 16, blocks, 16, 4, 2)   # word, then nibbles 4 * parity + i
+    packed = (c[..., 0] | c[..., 1] << 4).reshape(tiles, 16, blocks, 64).transpose(1, 2).reshape(tiles, blocks, 1024)
+    wide = scales.dtype == torch.float32
+    bits = scales.contiguous()
+    bits = bits.view(torch.int32) if wide else bits.view(torch.int16).to(torch.int32) << 16
+    zero = torch.full_like(bits, 8) if zeros is None else zeros.to(torch.int32)
+    words = torch.stack((zero, bits), 2) if wide else (zero | bits)[:, :, None]
+    if group_size > _BLOCK:
+        words = words.repeat_interleave(group_size // _BLOCK, 1)[:, :blocks]
+    per_block = max(1, _BLOCK // group_size)
+    words = pad(words, (0, 0, 0, blocks * per_block - words.shape[1], 0, tiles * 16 - n))
+    words = words.reshape(tiles, 16, blocks, per_block * words.shape[2]).transpose(1, 2)
+    words = words.reshape(tiles, blocks, 16 * per_block * (2 if wide else 1)).contiguous().view(torch.uint8)
+    return W4Weight((n, k), group_size, scales.dtype, torch.cat((words, packed), 2))
 
 
 def quantize_w4(weight, group_size=128, symmetric=False):
@@ -268,8 +291,10 @@ def matrix_mul_w4(x, weight, bias=None, out=None):
     bfloat16 on the weight's device; bias None or [N] of x's dtype.  Returns (or writes into
     `out`, [..., N] with unit column stride) x's dtype.
 
-    Up to 32 rows of x (float32: 10), the decoding case, the codes are read once and enter
-    exactly: products are exact, sums fp32, one rounding at the end.  More rows: the weight is
+    Up to 32 rows of x (float32: 8), the decoding case, the codes are read once and enter
+    exactly: sums are fp32, with one rounding at the end.  Up to 8 of them go through
+    the integer tensor path, where x is held in steps of 2^-29 of the power of two at or below
+    the largest magnitude of its block of 128.  More rows: the weight is
     expanded into the workspace, rounded to x's dtype (float32: exact), at most 256 MiB (or
     256 rows of it) at a time, and multiplied on the tensor cores (float32: the 3xTF32 product
     of matrix_mul).  Not differentiable."""
@@ -282,9 +307,9 @@ def matrix_mul_w4(x, weight, bias=None, out=None):
     dt = _DTYPES.get(x.dtype)
     if dt is None:
         raise TypeError(f"matrix_mul_w4: x must be float32, float16 or bfloat16, got {x.dtype}")
-    codes, scales, zeros, dev = weight.codes, weight.scales, weight.zeros, x.device
-    if not (x.is_cuda and codes.device == dev):
-        raise ValueError(f"matrix_mul_w4: x and weight must be on one CUDA device (got {dev} and {codes.device}); "
+    dev = x.device
+    if not (x.is_cuda and weight.device == dev):
+        raise ValueError(f"matrix_mul_w4: x and weight must be on one CUDA device (got {dev} and {weight.device}); "
                          "tilec_b200 has no CPU path")
     if bias is not None and (bias.dtype != x.dtype or bias.dim() != 1 or bias.shape[0] != n or bias.device != dev):
         raise ValueError(f"matrix_mul_w4: bias must be a {x.dtype} [{n}] tensor on {dev}")
@@ -319,10 +344,11 @@ def matrix_mul_w4(x, weight, bias=None, out=None):
     try:
         stream = _stream(dev)
         px, po = xr.data_ptr(), out2.data_ptr()
-        nbytes = lib.tilec_mm_w4_workspace_bytes(px, dt, m, ldx, n, k, weight.group_size, po, ldo)
+        nbytes = lib.tilec_mm_w4_workspace_bytes(px, dt, m, ldx, _DTYPES[weight.scale_dtype], n, k,
+                                                 weight.group_size, po, ldo)
         ws = _workspace(nbytes, dev)
-        rc = lib.tilec_mm_w4(px, dt, m, ldx, codes.data_ptr(), scales.data_ptr(), _DTYPES[scales.dtype], _ptr(zeros),
-                             n, k, weight.group_size, _ptr(bias), po, ldo, _ptr(ws), nbytes, stream)
+        rc = lib.tilec_mm_w4(px, dt, m, ldx, weight.data.data_ptr(), _DTYPES[weight.scale_dtype], n, k,
+                             weight.group_size, _ptr(bias), po, ldo, _ptr(ws), nbytes, stream)
         _native.check(rc, "tilec_mm_w4")
         _check_device(stream)
     finally:
