@@ -138,11 +138,11 @@ int launch_f16(const Op16& A, const Op16& B, int64_t M, int64_t N, int64_t K, F1
 }
 
 // K slices of a product of few tiles: as many as fill the CTA pairs once, each at least
-// eight stages deep.
+// four stages (512) deep.
 int f16_slices(int64_t M, int64_t N, int64_t K, const LmInfo& lm, int* kb_per_slice) {
   const int64_t tiles = cdiv(M, 256) * cdiv(N, 256), nkb = cdiv(K, F16Cfg::BK);
   int64_t n = lm.f16_slots / tiles;
-  if (n > nkb / 8) n = nkb / 8;
+  if (n > nkb / 4) n = nkb / 4;
   if (n < 1) n = 1;
   const int64_t per = cdiv(nkb, n);
   *kb_per_slice = static_cast<int>(per);

@@ -4,8 +4,10 @@
 //
 // The schedule is that of tc2_tf32p.cuh (256 x 256 tiles, two TMEM accumulators, one relay
 // thread per stage in the peer CTA, bounded waits).  What differs:
-//   * a stage holds 64 of K (128 bytes a row, the 128-byte swizzle's width), four MMAs of
-//     K = 16 each;
+//   * a stage holds 128 of K as two halves of 64 (128 bytes a row, the 128-byte swizzle's
+//     width), eight MMAs of K = 16 each and one commit: at twice tf32's rate the issuing thread
+//     is what runs out of time first (see the MMA role); what lies past K is neither loaded
+//     nor multiplied;
 //   * an operand stored along M or N (MN-major) is staged as slabs of 64 columns x 64 of K,
 //     one TMA box {64, 64} each, 16-byte swizzle granules (for 16-bit types the tensor core
 //     reads the plain 128-byte swizzle in either order);
@@ -86,21 +88,20 @@ struct F16Args {
 
 struct F16Cfg {
   static constexpr int BN = 256;
-  static constexpr int BK = 64;
-  static constexpr int kStages = 5;
+  static constexpr int BK = 128;
+  static constexpr int kStages = 3;
   static constexpr int kBNHalf = BN / 2;
   static constexpr int kEpiWarps = 8;
   static constexpr int kThreads = 64 + 32 * kEpiWarps;
-  static constexpr int kABytes = 128 * BK * 2;
-  static constexpr int kBBytes = kBNHalf * BK * 2;
-  static constexpr int kStageBytes = kABytes + kBBytes;
-  static constexpr int kStorePitch = 36;
+  static constexpr int kHalfBytes = 128 * 64 * 2;       // 64 of K of either operand's 128 rows or columns
+  static constexpr int kStageBytes = 4 * kHalfBytes;     // A's two halves, then B's
+  static constexpr int kStorePitch = 32;
   static constexpr int kStoreFloatsPerWarp = 32 * kStorePitch;
   static constexpr int kStoreBytes = kEpiWarps * kStoreFloatsPerWarp * 4;
   static constexpr int kBarBytes = 512;
   static constexpr int kSmemBytes = kStages * kStageBytes + kStoreBytes + kBarBytes + 1024;
   static constexpr uint32_t kSbo = 1024u;          // 8 rows (K-major) or 8 of K (MN-major) x 128 bytes
-  static constexpr uint32_t kLbo = BK * 128u;      // MN-major: stride between 64-column slabs
+  static constexpr uint32_t kLbo = 64 * 128u;      // MN-major: stride between 64-column slabs
   static constexpr uint32_t kTmemCols = 2 * BN;
   static_assert(kSmemBytes <= 232448, "shared memory");
   static_assert((3 * kStages + 5) * 8 + 8 <= kBarBytes, "barrier area");
@@ -114,8 +115,9 @@ __device__ __forceinline__ uint32_t make_idesc_16(int m, int n, bool bf16, bool 
          ((uint32_t(n) >> 3) << 17) | ((uint32_t(m) >> 4) << 24);
 }
 
-// One warp's 32 rows x 32 columns of a tile, staged in shared memory (pitch 36 floats, one
-// row per lane's v[]), go out in 8-column pieces: four lanes cover a row's 64 (16-bit) or
+// One warp's 32 rows x 32 columns of a tile, staged in shared memory (one row per lane's v[],
+// its 16-byte pieces exchanged by the row's low bits, which keeps both passes free of bank
+// conflicts), go out in 8-column pieces: four lanes cover a row's 64 (16-bit) or
 // 128 (fp32) bytes.  `row_at(r)` maps staged row r to the row of `out`, or < 0 to skip it.
 template <int EPI, typename RowAt>
 __device__ __forceinline__ void f16_store_rows(const F16Args& p, const float* stage, RowAt row_at, int row0, int col0,
@@ -125,8 +127,9 @@ __device__ __forceinline__ void f16_store_rows(const F16Args& p, const float* st
     const int r = c >> 2, col = col0 + 8 * (c & 3);
     const int64_t orow = row_at(r);
     if (orow < 0 || col >= p.N) continue;
-    const float4 x0 = *reinterpret_cast<const float4*>(stage + r * F16Cfg::kStorePitch + 8 * (c & 3));
-    const float4 x1 = *reinterpret_cast<const float4*>(stage + r * F16Cfg::kStorePitch + 8 * (c & 3) + 4);
+    const float4* staged = reinterpret_cast<const float4*>(stage + r * F16Cfg::kStorePitch);
+    const float4 x0 = staged[(2 * (c & 3)) ^ (r & 7)];
+    const float4 x1 = staged[(2 * (c & 3) + 1) ^ (r & 7)];
     float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
     const int n = min(8, p.N - col);
     if constexpr (EPI == kEpiAcc || EPI == kEpiOut) {
@@ -180,7 +183,7 @@ __global__ void __launch_bounds__(F16Cfg::kThreads, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   auto a_tile = [&](int s) { return smem + s * Cfg::kStageBytes; };
-  auto b_tile = [&](int s) { return smem + s * Cfg::kStageBytes + Cfg::kABytes; };
+  auto b_tile = [&](int s) { return smem + s * Cfg::kStageBytes + 2 * Cfg::kHalfBytes; };
   float* store_area = reinterpret_cast<float*>(smem + STAGES * Cfg::kStageBytes);
   uint8_t* bar_area = smem + STAGES * Cfg::kStageBytes + Cfg::kStoreBytes;
   uint64_t* full = reinterpret_cast<uint64_t*>(bar_area);  // [STAGES] own TMA landed
@@ -273,19 +276,25 @@ __global__ void __launch_bounds__(F16Cfg::kThreads, 1)
           const int s = g % STAGES;
           const uint32_t ph = (g / STAGES) & 1;
           if (!mbar_wait_cluster(&empty[s], ph ^ 1, abort_flag)) { ok = false; break; }
-          mbar_arrive_expect_tx(&full[s], Cfg::kStageBytes);
           const int k0 = (ta.kb0 + kb) * BK;
-          if constexpr (A_MN) {
+          const int halves = K - k0 > 64 ? 2 : 1;
+          mbar_arrive_expect_tx(&full[s], halves * 2 * Cfg::kHalfBytes);
+          for (int h = 0; h < halves; ++h) {
+            uint8_t* a_dst = a_tile(s) + h * Cfg::kHalfBytes;
+            uint8_t* b_dst = b_tile(s) + h * Cfg::kHalfBytes;
+            const int k = k0 + 64 * h;
+            if constexpr (A_MN) {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) tma_load_2d(a_tile(s) + j * Cfg::kLbo, &tmA, &full[s], ta.m0 + 64 * j, k0);
-          } else {
-            tma_load_2d(a_tile(s), &tmA, &full[s], k0, ta.m0);
-          }
-          if constexpr (B_K) {
-            tma_load_2d(b_tile(s), &tmB, &full[s], k0, nb0);
-          } else {
+              for (int j = 0; j < 2; ++j) tma_load_2d(a_dst + j * Cfg::kLbo, &tmA, &full[s], ta.m0 + 64 * j, k);
+            } else {
+              tma_load_2d(a_dst, &tmA, &full[s], k, ta.m0);
+            }
+            if constexpr (B_K) {
+              tma_load_2d(b_dst, &tmB, &full[s], k, nb0);
+            } else {
 #pragma unroll
-            for (int j = 0; j < 2; ++j) tma_load_2d(b_tile(s) + j * Cfg::kLbo, &tmB, &full[s], nb0 + 64 * j, k0);
+              for (int j = 0; j < 2; ++j) tma_load_2d(b_dst + j * Cfg::kLbo, &tmB, &full[s], nb0 + 64 * j, k);
+            }
           }
           ++g;
         }
@@ -302,34 +311,50 @@ __global__ void __launch_bounds__(F16Cfg::kThreads, 1)
   } else if (warp == 1) {
     if (leader && lane == 0) {
       // ---------------------------------------------------------- MMA issuer (leader CTA)
+      // Sixteen-bit MMAs take half as long as tf32's, some 500 cycles per 64 of K, which this
+      // thread's own work per stage reached first: descriptors, addresses and phases are carried
+      // along instead of being built anew (4096 x 32768 x 4096: 0.905 -> 0.847 ms).
       const uint32_t idesc = make_idesc_16(256, BN, p.bf16 != 0, A_MN, !B_K);
-      auto desc = [&](uint32_t base, int kk, bool mn) {
-        return mn ? make_smem_desc(base + kk * 2048, Cfg::kLbo, Cfg::kSbo, kLayoutSw128)
-                  : make_smem_desc(base + kk * 32, 16, Cfg::kSbo, kLayoutSw128);
+      auto desc0 = [&](const void* tile, bool mn) {
+        return make_smem_desc(smem_u32(tile), mn ? Cfg::kLbo : 16, Cfg::kSbo, kLayoutSw128);
       };
-      int g = 0;
+      const uint64_t a_desc = desc0(a_tile(0), A_MN), b_desc = desc0(b_tile(0), !B_K);
+      constexpr uint64_t kAStep = (A_MN ? 2048 : 32) >> 4, kBStep = (B_K ? 32 : 2048) >> 4;  // K = 16
+      constexpr uint64_t kHalfStep = Cfg::kHalfBytes >> 4;
+      const uint32_t full_at = smem_u32(full), peer_at = smem_u32(peer_full), empty_at = smem_u32(empty);
+      uint32_t s = 0, ph = 0;
       bool ok = true;
       for (int i = 0; i < n_my && ok; ++i) {
         const int b = i & 1;
-        const uint32_t dcol = static_cast<uint32_t>(b * BN);
-        const int nkb = tile_at(i).nkb;
+        const uint32_t dcol = tmem + static_cast<uint32_t>(b * BN);
+        const TileAt ta = tile_at(i);
+        const int nkb = ta.nkb;
+        int left = K - ta.kb0 * BK;  // of K, from this stage on
         // Buffer b last held tile i - 2: both CTAs' epilogues must have drained it.
         if (i >= 2 && !mbar_wait_cluster(&acc_empty[b], ((i >> 1) - 1) & 1, abort_flag)) { ok = false; break; }
         tc_fence_after();
+        uint32_t accumulate = 0;
         for (int kb = 0; kb < nkb; ++kb) {
-          const int s = g % STAGES;
-          const uint32_t ph = (g / STAGES) & 1;
-          if (!mbar_wait(&full[s], ph, abort_flag) || !mbar_wait_cluster(&peer_full[s], ph, abort_flag)) {
+          if (!(mbar_try_wait_at(full_at + 8 * s, ph) || mbar_wait(&full[s], ph, abort_flag)) ||
+              !(mbar_try_wait_cluster_at(peer_at + 8 * s, ph) || mbar_wait_cluster(&peer_full[s], ph, abort_flag))) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t a0 = smem_u32(a_tile(s)), b0 = smem_u32(b_tile(s));
+          const uint64_t ad = a_desc + s * (Cfg::kStageBytes >> 4), bd = b_desc + s * (Cfg::kStageBytes >> 4);
 #pragma unroll
-          for (int kk = 0; kk < BK / 16; ++kk)
-            umma_bf16_pair(tmem + dcol, desc(a0, kk, A_MN), desc(b0, kk, !B_K), idesc, (kb == 0 && kk == 0) ? 0u : 1u);
-          umma_commit_pair_both(smem_u32(&empty[s]));
-          ++g;
+          for (int kk = 0; kk < BK / 16; ++kk) {
+            if (16 * kk >= left) break;
+            umma_bf16_pair(dcol, ad + (kk >> 2) * kHalfStep + (kk & 3) * kAStep,
+                           bd + (kk >> 2) * kHalfStep + (kk & 3) * kBStep, idesc, accumulate);
+            accumulate = 1;
+          }
+          left -= BK;
+          umma_commit_pair_both(empty_at + 8 * s);
+          if (++s == STAGES) {
+            s = 0;
+            ph ^= 1;
+          }
         }
         if (ok) umma_commit_pair_both(smem_u32(&acc_full[b]));
       }
@@ -425,9 +450,9 @@ __global__ void __launch_bounds__(F16Cfg::kThreads, 1)
             }
           }
 #pragma unroll
-          for (int j = 0; j < 32; j += 4)
-            *reinterpret_cast<float4*>(stage + lane * Cfg::kStorePitch + j) =
-                make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+          for (int j = 0; j < 8; ++j)
+            reinterpret_cast<float4*>(stage + lane * Cfg::kStorePitch)[j ^ (lane & 7)] =
+                make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
           __syncwarp();
           const int row0 = ta.m0 + 32 * q;
           auto row_at = [&](int rr) -> int64_t {
