@@ -97,30 +97,6 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
   return ok != 0;
 }
 
-// The same by shared-memory address, for loops that carry it along.
-__device__ __forceinline__ bool mbar_try_wait_at(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity), "r"(uint32_t(TILEC_WAIT_HINT_NS))
-      : "memory");
-  return ok != 0;
-}
-__device__ __forceinline__ bool mbar_try_wait_cluster_at(uint32_t bar, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}"
-      : "=r"(ok)
-      : "r"(bar), "r"(parity), "r"(uint32_t(TILEC_WAIT_HINT_NS))
-      : "memory");
-  return ok != 0;
-}
-
 // Bounded wait for the phase with the given parity.  `abort_flag` (shared) lets
 // one role that gave up release every other role quickly.  limit_ns == 0: the device's
 // limit (wait_limit()); the clock is read every 64 polls at the default limit and on

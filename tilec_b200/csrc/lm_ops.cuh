@@ -125,7 +125,7 @@ int launch_f16(const Op16& A, const Op16& B, int64_t M, int64_t N, int64_t K, F1
   p.N = static_cast<int>(N);
   p.K = static_cast<int>(K);
   p.n_tiles = static_cast<int>(cdiv(N, 256));
-  p.group_m = 8;
+  p.group_m = 16;
   if (p.slices <= 1) {
     p.slices = 1;
     p.kb_per_slice = static_cast<int>(cdiv(K, F16Cfg::BK));

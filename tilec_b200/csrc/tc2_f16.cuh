@@ -107,6 +107,54 @@ struct F16Cfg {
   static_assert((3 * kStages + 5) * 8 + 8 <= kBarBytes, "barrier area");
 };
 
+// Bounded waits with their clock-reading loop out of line.  This kernel's roles share an SM's
+// instruction caches, and the MMA thread cannot afford misses: with those loops inlined, builds
+// of one source ran 12 % apart by where their code happened to lie (4096 x 32768 x 4096: 0.77
+// to 0.88 ms, twice the instruction cache requests, tensor pipe 84 % busy against 67).  `hint`: how long a try may suspend the
+// thread; the waits for a whole tile sleep instead of polling.
+template <bool CLUSTER>
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity, uint32_t hint) {
+  uint32_t ok;
+  if constexpr (CLUSTER)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(hint)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity), "r"(hint)
+        : "memory");
+  return ok != 0;
+}
+__device__ __noinline__ bool mbar_poll(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint32_t hint) {
+  const unsigned long long t0 = global_ns(), limit = wait_limit();
+  for (;;) {
+    if (mbar_try<true>(bar, parity, hint)) return true;
+    if (*abort_flag) return false;
+    if (global_ns() - t0 > limit) {
+      *abort_flag = 1;
+      record_status(TILEC_DEV_TIMEOUT);
+      return false;
+    }
+  }
+}
+constexpr uint32_t kHintStage = 64, kHintTile = 1000;  // ns
+template <bool CLUSTER>
+__device__ __forceinline__ bool mbar_wait_far(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint32_t hint) {
+  // A short loop first: entering the call costs the MMA thread more than polling (0.79 -> 0.74 ms).
+#pragma unroll 1
+  for (int i = 0; i < 32; ++i)
+    if (mbar_try<CLUSTER>(bar, parity, kHintStage)) return true;
+  return mbar_poll(bar, parity, abort_flag, hint);
+}
+
 // Instruction descriptor for kind::f16 (format 0 = f16, 1 = bf16 for A and B alike), fp32
 // accumulate; the other bits as in make_idesc_bf16.
 __device__ __forceinline__ uint32_t make_idesc_16(int m, int n, bool bf16, bool a_mn, bool b_mn) {
@@ -275,7 +323,7 @@ __global__ void __launch_bounds__(F16Cfg::kThreads, 1)
         for (int kb = 0; kb < ta.nkb; ++kb) {
           const int s = g % STAGES;
           const uint32_t ph = (g / STAGES) & 1;
-          if (!mbar_wait_cluster(&empty[s], ph ^ 1, abort_flag)) { ok = false; break; }
+          if (!mbar_wait_far<true>(smem_u32(&empty[s]), ph ^ 1, abort_flag, kHintStage)) { ok = false; break; }
           const int k0 = (ta.kb0 + kb) * BK;
           const int halves = K - k0 > 64 ? 2 : 1;
           mbar_arrive_expect_tx(&full[s], halves * 2 * Cfg::kHalfBytes);
@@ -302,7 +350,7 @@ __global__ void __launch_bounds__(F16Cfg::kThreads, 1)
       if (ok) {
         // Tail: the leader's release of each of the last fills has arrived before the CTA exits.
         for (int f = g - STAGES < 0 ? 0 : g - STAGES; f < g; ++f)
-          if (!mbar_wait_cluster(&empty[f % STAGES], (f / STAGES) & 1, abort_flag)) { ok = false; break; }
+          if (!mbar_wait_far<true>(smem_u32(&empty[f % STAGES]), (f / STAGES) & 1, abort_flag, kHintStage)) { ok = false; break; }
       }
       if (!ok) {
         for (int f = g - STAGES < 0 ? 0 : g - STAGES; f < g; ++f) mbar_drain(&full[f % STAGES], (f / STAGES) & 1);
@@ -331,23 +379,31 @@ __global__ void __launch_bounds__(F16Cfg::kThreads, 1)
         const int nkb = ta.nkb;
         int left = K - ta.kb0 * BK;  // of K, from this stage on
         // Buffer b last held tile i - 2: both CTAs' epilogues must have drained it.
-        if (i >= 2 && !mbar_wait_cluster(&acc_empty[b], ((i >> 1) - 1) & 1, abort_flag)) { ok = false; break; }
+        if (i >= 2 && !mbar_wait_far<true>(smem_u32(&acc_empty[b]), ((i >> 1) - 1) & 1, abort_flag, kHintStage)) {
+          ok = false;
+          break;
+        }
         tc_fence_after();
         uint32_t accumulate = 0;
         for (int kb = 0; kb < nkb; ++kb) {
-          if (!(mbar_try_wait_at(full_at + 8 * s, ph) || mbar_wait(&full[s], ph, abort_flag)) ||
-              !(mbar_try_wait_cluster_at(peer_at + 8 * s, ph) || mbar_wait_cluster(&peer_full[s], ph, abort_flag))) {
+          if (!mbar_wait_far<false>(full_at + 8 * s, ph, abort_flag, kHintStage) ||
+              !mbar_wait_far<true>(peer_at + 8 * s, ph, abort_flag, kHintStage)) {
             ok = false;
             break;
           }
           tc_fence_after();
           const uint64_t ad = a_desc + s * (Cfg::kStageBytes >> 4), bd = b_desc + s * (Cfg::kStageBytes >> 4);
-#pragma unroll
-          for (int kk = 0; kk < BK / 16; ++kk) {
-            if (16 * kk >= left) break;
+          auto step = [&](int kk) {
             umma_bf16_pair(dcol, ad + (kk >> 2) * kHalfStep + (kk & 3) * kAStep,
                            bd + (kk >> 2) * kHalfStep + (kk & 3) * kBStep, idesc, accumulate);
             accumulate = 1;
+          };
+          if (left >= BK) {
+#pragma unroll
+            for (int kk = 0; kk < BK / 16; ++kk) step(kk);
+          } else {
+#pragma unroll 1
+            for (int kk = 0; 16 * kk < left; ++kk) step(kk);
           }
           left -= BK;
           umma_commit_pair_both(empty_at + 8 * s);
@@ -371,7 +427,7 @@ __global__ void __launch_bounds__(F16Cfg::kThreads, 1)
         const int nkb = tile_at(i).nkb;
         for (int kb = 0; kb < nkb; ++kb, ++g) {
           const int s = g % STAGES;
-          if (!mbar_wait(&full[s], (g / STAGES) & 1, abort_flag)) { ok = false; break; }
+          if (!mbar_wait_far<false>(smem_u32(&full[s]), (g / STAGES) & 1, abort_flag, kHintStage)) { ok = false; break; }
           mbar_arrive_remote_cta(pf + static_cast<uint32_t>(s * 8));
         }
       }
@@ -407,7 +463,9 @@ __global__ void __launch_bounds__(F16Cfg::kThreads, 1)
           }
         }
       }
-      if (!mbar_wait_cluster(&acc_full[b], (i >> 1) & 1, abort_flag)) break;
+      // One answer for the warp: what follows is warp-wide.
+      if (!__all_sync(0xffffffffu, mbar_wait_far<true>(smem_u32(&acc_full[b]), (i >> 1) & 1, abort_flag, kHintTile)))
+        break;
       tc_fence_after();
       if (i == n_my - 1) pdl_launch_dependents();
       float run_max = -INFINITY, run_sum = 0.f;
