@@ -287,7 +287,7 @@ TILEC_API int tilec_linear_ce_forward(const void* x, const void* w, const int64_
 
 /* Gradients of the above, from the same operands and the forward pass's stats:
  *   dlogit[t, v] = g[t] * (softmax[t, v] - [v == target[t]])
- *   dx = dlogit . w ([T, D], row-major, dense)    dw = dlogit^T . x ([V, D], row-major, dense)
+ *   dx = dlogit . w ([T, D])    dw = dlogit^T . x ([V, D])    row-major, dense, 16-byte aligned
  * grad: the loss's gradient, T floats (TILEC_REDUCE_NONE) or one float.  dx or dw may be
  * NULL.  dx and dw have the operands' dtype; sums are fp32, dlogit is rounded to the
  * operands' dtype for the products (fp32: not rounded).  Logits are computed again, a piece

@@ -135,6 +135,8 @@ def test_abi_refusals():
     assert back(256, 256, 256, 2, 4, 16, 8, 8, 8, -100, 2, None, 256, 256, 256, None, 0, None) == 1
     assert back(256, 256, 256, 2, 4, 16, 8, 8, 8, -100, 2, 256, None, 256, 256, None, 0, None) == 1
     assert back(256, 256, 256, 2, 4, 16, 8, 8, 8, -100, 2, 256, 256, None, None, None, 0, None) == 0
+    assert back(256, 256, 256, 2, 4, 16, 8, 8, 8, -100, 2, 256, 256, 264, 256, None, 0, None) == 1
+    assert back(256, 256, 256, 2, 4, 16, 8, 8, 8, -100, 2, 256, 256, 256, 264, None, 0, None) == 1
     assert lib.tilec_linear_ce_workspace_bytes(None, None, 3, 4, 16, 8, 8, 8, 2, 0) == 0
 
 

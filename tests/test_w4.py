@@ -255,6 +255,11 @@ def test_strides_out_and_shapes(m, dtype):
         else:
             assert torch.equal(view, base)
         assert (buf[:, :off] == 7).all() and (buf[:, off + 200:] == 7).all()
+    odd = ext.pack_w4(codes[:197], scales[:197], zeros[:197], 64).to("cuda")   # N no multiple of 8, the stride one
+    buf = torch.full((m, 256), 7.0, dtype=x.dtype, device="cuda")
+    ext.matrix_mul_w4(x, odd, bias[:197], out=buf[:, :197])
+    torch.testing.assert_close(buf[:, :197], base[:, :197], rtol=1e-5, atol=1e-4)
+    assert (buf[:, 197:] == 7).all()
     for bad in (base.float() if dtype != "f32" else base.half(), base[:, :-1], base.t().contiguous().t(), base.cpu()):
         with pytest.raises(ValueError, match="out must"):
             ext.matrix_mul_w4(x, w, bias, out=bad)

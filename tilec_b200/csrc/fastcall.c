@@ -9,6 +9,8 @@
  *   install(addr_mm_f32, addr_workspace_bytes) -> None
  *   mm(a, b, c, M, N, K, lda, ldb, ldc, variant, split_k, flags, ws, ws_bytes, stream) -> int
  *   ws_bytes(a, b, c, M, N, K, lda, ldb, ldc, variant, split_k, flags) -> int
+ *   install_w4(addr_mm_w4) -> None
+ *   w4(x, dtype, M, ldx, weight, scale_dtype, N, K, group, bias, out, ldo, ws, ws_bytes, stream) -> int
  *
  * Pointers (a, b, c, ws, stream) are Python ints (0 or None for NULL); the rest are ints.
  * Return values are the C ABI's status codes and byte counts, unchanged.
@@ -130,12 +132,65 @@ static PyObject* py_ws_bytes(PyObject* self, PyObject* const* args, Py_ssize_t n
   return PyLong_FromSize_t(n);
 }
 
+typedef int (*mm_w4_fn)(const void*, int32_t, int64_t, int64_t, const void*, int32_t, int64_t, int64_t, int64_t,
+                        const void*, void*, int64_t, void*, size_t, void*);
+static mm_w4_fn g_w4 = NULL;
+
+static PyObject* py_install_w4(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  void* a = NULL;
+  if (nargs != 1) {
+    PyErr_SetString(PyExc_TypeError, "install_w4(addr_mm_w4)");
+    return NULL;
+  }
+  if (as_ptr(args[0], &a)) return NULL;
+  if (a == NULL) {
+    PyErr_SetString(PyExc_ValueError, "install_w4: null function address");
+    return NULL;
+  }
+  g_w4 = (mm_w4_fn)a;
+  Py_RETURN_NONE;
+}
+
+static PyObject* py_w4(PyObject* self, PyObject* const* args, Py_ssize_t nargs) {
+  (void)self;
+  if (nargs != 15) {
+    PyErr_SetString(PyExc_TypeError, "w4() takes 15 arguments");
+    return NULL;
+  }
+  if (g_w4 == NULL) {
+    PyErr_SetString(PyExc_RuntimeError, "tilec fastcall: install_w4() was not called");
+    return NULL;
+  }
+  /* x, weight, bias, out, ws, stream; dtype, M, ldx, scale_dtype, N, K, group, ldo, ws_bytes */
+  static const int kPtr[6] = {0, 4, 9, 10, 12, 14}, kInt[9] = {1, 2, 3, 5, 6, 7, 8, 11, 13};
+  void* p[6];
+  int64_t v[9];
+  for (int i = 0; i < 6; ++i)
+    if (as_ptr(args[kPtr[i]], &p[i])) return NULL;
+  for (int i = 0; i < 9; ++i)
+    if (as_i64(args[kInt[i]], &v[i])) return NULL;
+  if (v[8] < 0) {
+    PyErr_SetString(PyExc_ValueError, "w4: negative workspace size");
+    return NULL;
+  }
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = g_w4(p[0], (int32_t)v[0], v[1], v[2], p[1], (int32_t)v[3], v[4], v[5], v[6], p[2], p[3], v[7], p[4],
+            (size_t)v[8], p[5]);
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(rc);
+}
+
 static PyMethodDef kMethods[] = {
     {"install", (PyCFunction)(void (*)(void))py_install, METH_FASTCALL, "install(addr_mm_f32, addr_workspace_bytes)"},
     {"mm", (PyCFunction)(void (*)(void))py_mm, METH_FASTCALL,
      "mm(a, b, c, M, N, K, lda, ldb, ldc, variant, split_k, flags, ws, ws_bytes, stream) -> status"},
     {"ws_bytes", (PyCFunction)(void (*)(void))py_ws_bytes, METH_FASTCALL,
      "ws_bytes(a, b, c, M, N, K, lda, ldb, ldc, variant, split_k, flags) -> bytes"},
+    {"install_w4", (PyCFunction)(void (*)(void))py_install_w4, METH_FASTCALL, "install_w4(addr_mm_w4)"},
+    {"w4", (PyCFunction)(void (*)(void))py_w4, METH_FASTCALL,
+     "w4(x, dtype, M, ldx, weight, scale_dtype, N, K, group, bias, out, ldo, ws, ws_bytes, stream) -> status"},
     {NULL, NULL, 0, NULL},
 };
 

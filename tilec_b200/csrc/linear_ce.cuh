@@ -126,9 +126,24 @@ __global__ void __launch_bounds__(256) pack16_kernel(const unsigned short* __res
           h = *reinterpret_cast<const uint4*>(s + c);
         } else {
           uint32_t w[4] = {0, 0, 0, 0};
+          if (c + 8 <= cols) {
+            // Aligned 4-byte words, shifted into place: each holds an element of the row, so
+            // none lies on another page.
+            const uintptr_t at = reinterpret_cast<uintptr_t>(s + c);
+            const uint32_t* v = reinterpret_cast<const uint32_t*>(at & ~uintptr_t(3));
+            const unsigned shift = (at & 2) * 8;
+            uint32_t lo = v[0];
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (c + j < cols) w[j >> 1] |= uint32_t(s[c + j]) << (16 * (j & 1));
+            for (int j = 0; j < 4; ++j) {
+              const uint32_t hi = j < 3 || shift ? v[j + 1] : 0u;
+              w[j] = __funnelshift_r(lo, hi, shift);
+              lo = hi;
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (c + j < cols) w[j >> 1] |= uint32_t(s[c + j]) << (16 * (j & 1));
+          }
           h = make_uint4(w[0], w[1], w[2], w[3]);
         }
       }
@@ -263,6 +278,49 @@ __global__ void __launch_bounds__(256) f16_join_slabs_kernel(const float* __rest
       for (int j = 0; j < 8; ++j)
         if (c + j < N) d[j] = static_cast<unsigned short>(w[j >> 1] >> (16 * (j & 1)));
     }
+  }
+}
+
+// Rows of `src` (row stride lds) to rows of `dst` that 16-byte stores cannot take, dst row
+// rows[r] (or r).  The product kernel stores whole 8-column pieces; storing odd rows from there
+// cost 155 us for the gradient of a 30011 x 777 weight, through this copy it is 70.  Dense rows
+// (rows == nullptr, ldd == cols) go out as one run, 16 bytes a thread; others by element.
+__global__ void __launch_bounds__(256) unpad16_kernel(const unsigned short* __restrict__ src, int64_t lds,
+                                                      unsigned short* __restrict__ dst, int64_t ldd, int64_t nrows,
+                                                      int cols, const int* __restrict__ count,
+                                                      const int* __restrict__ rows, int dense) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const int64_t n = count != nullptr ? *count : nrows;
+  const int64_t threads = int64_t(gridDim.x) * 256, self = int64_t(blockIdx.x) * 256 + threadIdx.x;
+  if (dense) {
+    const int64_t total = n * cols;
+    for (int64_t i = self * 8; i < total; i += threads * 8) {
+      int64_t r = i / cols;
+      int c = static_cast<int>(i - r * cols);
+      uint32_t w[4] = {0, 0, 0, 0};
+      const int m = total - i < 8 ? static_cast<int>(total - i) : 8;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (j < m) w[j >> 1] |= uint32_t(src[r * lds + c]) << (16 * (j & 1));
+        if (++c == cols) {
+          c = 0;
+          ++r;
+        }
+      }
+      if (m == 8) {
+        *reinterpret_cast<uint4*>(dst + i) = make_uint4(w[0], w[1], w[2], w[3]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (j < m) dst[i + j] = static_cast<unsigned short>(w[j >> 1] >> (16 * (j & 1)));
+      }
+    }
+    return;
+  }
+  for (int64_t i = self; i < n * cols; i += threads) {
+    const int64_t r = i / cols;
+    dst[(rows != nullptr ? int64_t(rows[r]) : r) * ldd + (i - r * cols)] = src[r * lds + (i - r * cols)];
   }
 }
 

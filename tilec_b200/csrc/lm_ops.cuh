@@ -157,12 +157,16 @@ int f16_slices(int64_t M, int64_t N, int64_t K, const LmInfo& lm, int* kb_per_sl
 
 // A 16-bit product with its sums in fp32: K slices go through slabs ([slices][M][lda] floats),
 // a sum over several products (dx over pieces of the vocabulary) through acc_in / acc_out
-// ([M][lda] floats).  out == nullptr: the sums stay in acc_out.
+// ([M][lda] floats).  out == nullptr: the sums stay in acc_out.  `odd`: room for M rows of lda
+// 16-bit values, where out's rows are not made of whole 16-byte pieces and slices == 1.
+inline bool odd_rows(const void* out, int64_t ldo, int64_t N) {
+  return !aligned16(out) || ldo % 8 != 0 || N % 8 != 0;
+}
+
 template <bool A_MN, bool B_K>
 int product16(const Op16& A, const Op16& B, int64_t M, int64_t N, int64_t K, F16Args a, int slices, int kb,
               int64_t lda, const float* acc_in, float* acc_out, void* out, int64_t ldo, float* slabs,
-              const LmInfo& lm, const DeviceInfo& d, cudaStream_t s) {
-  const int vec = aligned16(out) && ldo % 8 == 0;
+              void* odd, const LmInfo& lm, const DeviceInfo& d, cudaStream_t s) {
   a.slices = slices;
   a.kb_per_slice = kb;
   if (slices > 1) {
@@ -177,7 +181,7 @@ int product16(const Op16& A, const Op16& B, int64_t M, int64_t N, int64_t K, F16
     return launch_k(f16_join_slabs_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, 1,
                     static_cast<const float*>(slabs), slices, b.slab, lda, acc_in, acc_out,
                     static_cast<unsigned short*>(out), ldo, M, N, a.count_is_k ? nullptr : a.count, a.rows, a.scale,
-                    a.scale2, a.bias, a.bf16, vec);
+                    a.scale2, a.bias, a.bf16, odd_rows(out, ldo, N) ? 0 : 1);
   }
   a.acc = acc_in;
   a.ldacc = lda;
@@ -186,10 +190,23 @@ int product16(const Op16& A, const Op16& B, int64_t M, int64_t N, int64_t K, F16
     a.ldo = lda;
     return launch_f16<kEpiAcc, A_MN, B_K>(A, B, M, N, K, a, lm, s);
   }
-  a.out = out;
-  a.ldo = ldo;
-  a.vec_out = vec;
-  return launch_f16<kEpiOut, A_MN, B_K>(A, B, M, N, K, a, lm, s);
+  if (!odd_rows(out, ldo, N)) {
+    a.out = out;
+    a.ldo = ldo;
+    return launch_f16<kEpiOut, A_MN, B_K>(A, B, M, N, K, a, lm, s);
+  }
+  const int* rows = a.rows;
+  const int* count = a.count_is_k ? nullptr : a.count;
+  a.rows = nullptr;
+  a.out = odd;
+  a.ldo = lda;
+  TILEC_TRY((launch_f16<kEpiOut, A_MN, B_K>(A, B, M, N, K, a, lm, s)));
+  const int dense = rows == nullptr && ldo == N && aligned16(out);
+  int64_t blocks = cdiv(M * N, dense ? 2048 : 256);
+  if (blocks > int64_t(d.sms) * 16) blocks = int64_t(d.sms) * 16;
+  return launch_k(unpad16_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, 1,
+                  static_cast<const unsigned short*>(odd), lda, static_cast<unsigned short*>(out), ldo, M,
+                  static_cast<int>(N), count, rows, dense);
 }
 
 // ---------------------------------------------------------------- linear cross entropy
@@ -216,7 +233,7 @@ struct CePlan {
   int64_t ldacc = 0;             // row stride of fp32 sums of dx
   int dx_slices = 1, dx_kb = 0, dw_slices = 1, dw_kb = 0;
   size_t off_head = 0, off_rows = 0, off_x = 0, off_w = 0, off_part = 0, off_tlogit = 0, off_loss = 0, off_p = 0,
-         off_acc = 0, off_slabs = 0, off_mm = 0;
+         off_acc = 0, off_slabs = 0, off_odd = 0, off_mm = 0;
   size_t mm_bytes = 0, bytes = 0;
 };
 
@@ -303,6 +320,11 @@ void plan_ce(const CeCall& c, int grads, const LmInfo& lm, CePlan* p) {
       }
     }
     if (slabs) p->off_slabs = take(slabs);
+    // The gradients lie dense on 16-byte boundaries: whole pieces when D is a multiple of 8.
+    size_t odd = 0;
+    if ((grads & 1) && p->dx_slices == 1) odd = size_t(c.T) * p->ldacc * 2;
+    if ((grads & 2) && p->dw_slices == 1 && size_t(p->piece) * p->ldacc * 2 > odd) odd = size_t(p->piece) * p->ldacc * 2;
+    if (odd && c.D % 8 != 0) p->off_odd = take(odd);
   }
   if (p->f32) {
     const float* x = static_cast<const float*>(c.x);
@@ -516,14 +538,15 @@ int ce_backward(const CeCall& c, const float* stats_buf, const float* grad, void
       g.rows = rows;
       TILEC_TRY((product16<false, false>(Op16{prob, p.ldp, false}, Op16{wi, ldw, true}, c.T, c.D, n, g, p.dx_slices,
                                          p.dx_kb, p.ldacc, i > 0 ? acc : nullptr, acc, last ? dx : nullptr, c.D, slabs,
-                                         *lm, *d, s)));
+                                         ws + p.off_odd, *lm, *d, s)));
     }
     if (dw) {
       g.rows = nullptr;
       g.count_is_k = 1;
       TILEC_TRY((product16<true, false>(Op16{prob, p.ldp, true}, Op16{xc, p.dp, true}, n, c.D, c.T, g, p.dw_slices,
                                         p.dw_kb, p.ldacc, nullptr, nullptr,
-                                        static_cast<unsigned short*>(dw) + v0 * c.D, c.D, slabs, *lm, *d, s)));
+                                        static_cast<unsigned short*>(dw) + v0 * c.D, c.D, slabs, ws + p.off_odd, *lm,
+                                        *d, s)));
     }
   }
   return TILEC_OK;
@@ -572,7 +595,7 @@ struct W4Plan {
   int64_t blocks = 0, kp = 0, piece = 0;
   int slices = 1, kb = 0;
   int64_t ldslab = 0;
-  size_t off_x = 0, off_w = 0, off_slabs = 0, off_mm = 0, mm_bytes = 0, bytes = 0;
+  size_t off_x = 0, off_w = 0, off_slabs = 0, off_odd = 0, off_mm = 0, mm_bytes = 0, bytes = 0;
 };
 
 int check_w4(const W4Call& c) {
@@ -673,6 +696,7 @@ void plan_w4(const W4Call& c, const DeviceInfo& d, const LmInfo& lm, W4Plan* p) 
       p->slices = f16_slices(c.M, p->piece, c.K, lm, &p->kb);
       p->ldslab = round_up(p->piece, 8);
       if (p->slices > 1) p->off_slabs = take(size_t(p->slices) * c.M * p->ldslab * 4);
+      else if (odd_rows(c.out, c.ldo, c.N)) p->off_odd = take(size_t(c.M) * p->ldslab * 2);
     }
   }
   p->bytes = at;
@@ -820,7 +844,7 @@ int run_w4(const W4Call& c, void* workspace, size_t ws_bytes, cudaStream_t s) {
       f.bias = bias;
       TILEC_TRY((product16<false, true>(Op16{x, ldx, false}, Op16{wd, p.kp, false}, c.M, n, c.K, f, p.slices, p.kb,
                                         p.ldslab, nullptr, nullptr, out, c.ldo,
-                                        reinterpret_cast<float*>(ws + p.off_slabs), *lm, *d, s)));
+                                        reinterpret_cast<float*>(ws + p.off_slabs), ws + p.off_odd, *lm, *d, s)));
     }
   }
   return TILEC_OK;
@@ -863,6 +887,7 @@ int tilec_linear_ce_backward(const void* x, const void* w, const int64_t* target
   const int rc = check_ce(c);
   if (rc) return rc;
   if (!stats || (!grad && (T > 0 || reduction != kReduceNone))) return TILEC_ERR_BAD_ARG;
+  if (!aligned16(dx) || !aligned16(dw)) return TILEC_ERR_BAD_ARG;
   return ce_backward(c, stats, grad, dx, dw, workspace, ws_bytes, static_cast<cudaStream_t>(stream));
 }
 

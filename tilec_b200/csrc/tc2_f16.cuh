@@ -77,8 +77,7 @@ struct F16Args {
   int m_alloc;            // rows of `out`: rows past the last one are written as zeros up to here
   // outputs
   void* out;              // 16-bit (kEpiProb, kEpiOut) or fp32 (kEpiAcc)
-  int64_t ldo, slab;      // row stride and K-slice stride in elements
-  int vec_out;            // 16-byte stores allowed
+  int64_t ldo, slab;      // row stride (16-bit: a multiple of 8, of whole 8-column pieces) and K-slice stride
   const float* acc;       // earlier sums to add (kEpiAcc with slices == 1: may equal out), or nullptr
   int64_t ldacc;
   const float* scale;     // kEpiOut: *scale * scale2 multiplies the sums (nullptr: scale2 alone)
@@ -179,7 +178,6 @@ __device__ __forceinline__ void f16_store_rows(const F16Args& p, const float* st
     const float4 x0 = staged[(2 * (c & 3)) ^ (r & 7)];
     const float4 x1 = staged[(2 * (c & 3) + 1) ^ (r & 7)];
     float x[8] = {x0.x, x0.y, x0.z, x0.w, x1.x, x1.y, x1.z, x1.w};
-    const int n = min(8, p.N - col);
     if constexpr (EPI == kEpiAcc || EPI == kEpiOut) {
       if (p.acc != nullptr) {  // rows of `acc` are padded to whole pieces
         const float4* a = reinterpret_cast<const float4*>(p.acc + static_cast<int64_t>(row0 + r) * p.ldacc + col);
@@ -199,7 +197,7 @@ __device__ __forceinline__ void f16_store_rows(const F16Args& p, const float* st
         if (p.bias != nullptr) {
 #pragma unroll
           for (int j = 0; j < 8; ++j)
-            if (j < n) x[j] += load_16(p.bias, col + j, p.bf16);
+            if (col + j < p.N) x[j] += load_16(p.bias, col + j, p.bf16);
         }
       }
       uint4 h;
@@ -207,15 +205,8 @@ __device__ __forceinline__ void f16_store_rows(const F16Args& p, const float* st
       h.y = pack_16x2(x[2], x[3], p.bf16);
       h.z = pack_16x2(x[4], x[5], p.bf16);
       h.w = pack_16x2(x[6], x[7], p.bf16);
-      unsigned short* d = static_cast<unsigned short*>(p.out) + orow * p.ldo + col;
-      if (EPI == kEpiProb || (p.vec_out && n == 8)) {  // rows of the probabilities are padded too
-        *reinterpret_cast<uint4*>(d) = h;
-      } else {
-        const uint32_t w[4] = {h.x, h.y, h.z, h.w};
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (j < n) d[j] = static_cast<unsigned short>(w[j >> 1] >> (16 * (j & 1)));
-      }
+      // Whole pieces: rows of `out` start and go on in steps of 16 bytes.
+      *reinterpret_cast<uint4*>(static_cast<unsigned short*>(p.out) + orow * p.ldo + col) = h;
     }
   }
 }

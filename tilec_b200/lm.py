@@ -38,15 +38,20 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+_ext = None   # tilec_b200.ext, which imports this module
+
+
 def _stream(device):
-    from . import ext
-    return ext._current_stream(device.index)
+    global _ext
+    if _ext is None:
+        from . import ext
+        _ext = ext
+    return _ext._current_stream(device.index)
 
 
 def _check_device(stream):
-    from . import ext
-    if ext._check_enabled():
-        ext.check_device(stream)
+    if _ext._check_enabled():
+        _ext.check_device(stream)
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
@@ -315,43 +320,62 @@ def matrix_mul_w4(x, weight, bias=None, out=None):
         raise ValueError(f"matrix_mul_w4: bias must be a {x.dtype} [{n}] tensor on {dev}")
     if torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad)):
         raise ValueError("matrix_mul_w4: not differentiable; call it under torch.no_grad() or detach the inputs")
-    xr, ldx = _rows(x if x.dim() == 2 else x.reshape(-1, k))
-    m = xr.shape[0]
-    shape = x.shape[:-1] + (n,)
-    if out is None:
-        out = torch.empty(shape, dtype=x.dtype, device=dev)
-        out2, ldo = out, n
+    if x.is_contiguous():
+        xr, ldx, m = x, k, x.numel() // k
     else:
-        if out.dtype != x.dtype or out.shape != shape or out.device != dev:
-            raise ValueError(f"matrix_mul_w4: out must be a {x.dtype} {tuple(shape)} tensor on {dev}")
-        try:
-            out2 = out.view(m, n)
-        except RuntimeError:
-            raise ValueError("matrix_mul_w4: the rows of out must lie at one stride") from None
-        s0, s1 = out2.stride()
-        if not ((n <= 1 or s1 == 1) and (m <= 1 or s0 >= n)):
-            raise ValueError("matrix_mul_w4: out must have unit column stride and non-overlapping rows")
-        ldo = s0 if m > 1 else n
+        xr, ldx = _rows(x if x.dim() == 2 else x.reshape(-1, k))
+        m = xr.shape[0]
+    if out is None:
+        out = out2 = x.new_empty(x.shape[:-1] + (n,))
+        ldo = n
+    else:
+        out2, ldo = _w4_out(out, x, dev, m, n)
     if m == 0 or n == 0:
         return out
     if bias is not None:
         bias = bias.contiguous()
     lib = _native.load()
+    index = dev.index
     prev = torch.cuda.current_device()
-    switch = prev != dev.index
+    switch = prev != index
     if switch:
-        torch.cuda.set_device(dev.index)
+        torch.cuda.set_device(index)
     try:
         stream = _stream(dev)
-        px, po = xr.data_ptr(), out2.data_ptr()
-        nbytes = lib.tilec_mm_w4_workspace_bytes(px, dt, m, ldx, _DTYPES[weight.scale_dtype], n, k,
-                                                 weight.group_size, po, ldo)
+        px, po, sdt, group = xr.data_ptr(), out2.data_ptr(), _DTYPES[weight.scale_dtype], weight.group_size
+        # The size depends on the operands' alignment only as far as their low bits tell.
+        key = (dt, m, ldx, sdt, n, k, group, ldo, (px | po << 4) & 0xFF, index)
+        nbytes = _W4_BYTES.get(key)
+        if nbytes is None:
+            nbytes = lib.tilec_mm_w4_workspace_bytes(px, dt, m, ldx, sdt, n, k, group, po, ldo)
+            if len(_W4_BYTES) >= 4096:  # a process that sees many shapes: start over
+                _W4_BYTES.clear()
+            _W4_BYTES[key] = nbytes
         ws = _workspace(nbytes, dev)
-        rc = lib.tilec_mm_w4(px, dt, m, ldx, weight.data.data_ptr(), _DTYPES[weight.scale_dtype], n, k,
-                             weight.group_size, _ptr(bias), po, ldo, _ptr(ws), nbytes, stream)
+        fast = _native.fast()
+        rc = (fast.w4 if fast is not None else lib.tilec_mm_w4)(
+            px, dt, m, ldx, weight.data.data_ptr(), sdt, n, k, group, _ptr(bias), po, ldo, _ptr(ws), nbytes, stream)
         _native.check(rc, "tilec_mm_w4")
         _check_device(stream)
     finally:
         if switch:
             torch.cuda.set_device(prev)
     return out
+
+
+_W4_BYTES = {}   # arguments that decide it -> workspace bytes of tilec_mm_w4
+
+
+def _w4_out(out, x, dev, m, n):
+    """(the [m, n] view of a caller's out, its row stride)"""
+    shape = x.shape[:-1] + (n,)
+    if out.dtype != x.dtype or out.shape != shape or out.device != dev:
+        raise ValueError(f"matrix_mul_w4: out must be a {x.dtype} {tuple(shape)} tensor on {dev}")
+    try:
+        out2 = out.view(m, n)
+    except RuntimeError:
+        raise ValueError("matrix_mul_w4: the rows of out must lie at one stride") from None
+    s0, s1 = out2.stride()
+    if not ((n <= 1 or s1 == 1) and (m <= 1 or s0 >= n)):
+        raise ValueError("matrix_mul_w4: out must have unit column stride and non-overlapping rows")
+    return out2, (s0 if m > 1 else n)
