@@ -8,9 +8,10 @@ S = sum_k |x (code - zero) scale|:
   parts) and four digits' sums are added in fp32, (64 + 4) * 2^-24 S for the upper digit, which
   holds all but 2^-7 of S: below 2^-17.8 S at worst, and the roundings are independent: 2^-18 S
   is held to; then one rounding, u |y|.
-* up to 32 rows: products of codes and x are exact; a 128-k block adds 8 groups of 16 products
-  to an accumulator, each sum truncated at worst (16 * 2^-23 S), and the at most 64 blocks are
-  added in fp32 (64 * 2^-24 S), the scale's product rounds once: below 2^-18 S.
+  Three to eight rows of 16-bit x: products of codes and x are exact; a 128-k block adds 8
+  groups of 16 products to an accumulator, each sum truncated at worst (16 * 2^-23 S), and the
+  at most 64 blocks are added in fp32 (64 * 2^-24 S), the scale's product rounds once: below
+  2^-18 S.
 * more rows: the weight is rounded to the type, u S more (fp32: the 3xTF32 product,
   3 * 2^-20 S); sums over K <= 8192 in the tensor cores' fp32 stay below 2^-14 S (K / 16 sums,
   each truncated by 2^-23).
@@ -45,7 +46,7 @@ def _weight64(codes, scales, zeros, group):
 
 def _bound(x, w, y, dtype, rows):
     s = x.double().abs() @ w.abs().t()
-    few = rows <= (8 if dtype == "f32" else 32)
+    few = rows <= 8
     rel = 2.0 ** -18 if few else 2.0 ** -14 + (3 * 2.0 ** -20 if dtype == "f32" else U[dtype])
     return rel * s + 1.001 * U[dtype] * y.abs() + (2.0 ** -25 if dtype == "f16" else 0.0)
 
@@ -188,7 +189,7 @@ def test_one_token(n, k, group, dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
-@pytest.mark.parametrize("m", [2, 3, 8, 9, 10, 11, 16, 17, 32, 33, 65, 257])
+@pytest.mark.parametrize("m", [2, 3, 8, 9, 10, 11, 16, 17, 32, 33, 65, 127, 128, 129, 257])
 def test_rows(m, dtype):
     """Either side of each variant's row count, with bias, symmetric and with zero points."""
     for zeros, group, n, k in ((True, 32, 90, 640), (False, 128, 259, 1157)):
@@ -199,13 +200,14 @@ def test_rows(m, dtype):
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
 @pytest.mark.parametrize("sdtype", ["bf16", "f16", "f32"])
 def test_scale_types(sdtype, dtype):
-    for m in (1, 40):
+    for m in (1, 5, 40):
         _check(*_make(m, 70, 384, 64, dtype, sdtype=sdtype), 64, dtype)
 
 
 @gpu
 @pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
-@pytest.mark.parametrize("m,n,k", [(1, 16, 8192), (5, 4096, 512), (1, 300, 8190), (40, 520, 8192), (300, 700, 2048)])
+@pytest.mark.parametrize("m,n,k", [(1, 16, 8192), (5, 4096, 512), (1, 300, 8190), (40, 520, 8192), (20, 2500, 1000),
+                                   (128, 130, 4000), (300, 700, 2048)])
 def test_long_sums_and_many_tiles(m, n, k, dtype):
     _check(*_make(m, n, k, 128, dtype), 128, dtype)
 
@@ -375,9 +377,9 @@ def test_train_quantise_serve(dtype):
     w = q.dequantize().double()
     ref = x.double() @ w.t()
     bound = 2.0 ** -18 * (x.double().abs() @ w.abs().t()) + 1.001 * U[dtype] * ref.abs()
-    if dtype == "f32":   # 24 rows of fp32 go through the 3xTF32 product
-        bound = bound + (2.0 ** -14) * (x.double().abs() @ w.abs().t())
-    assert ((whole.double() - ref).abs() <= bound).all()
+    # 24 rows at once: the weight is rounded to bf16, or (fp32) goes through the 3xTF32 product
+    more = (2.0 ** -14 + (U[dtype] if dtype == "bf16" else 0)) * (x.double().abs() @ w.abs().t())
+    assert ((whole.double() - ref).abs() <= bound + more).all()
     assert ((torch.stack(per_token).double() - ref).abs() <= bound).all()
     if dtype == "f32":
         got = ext.linear_cross_entropy(x, q.dequantize(), y, reduction="none").double()

@@ -56,12 +56,11 @@ int lm_device(DeviceInfo** d, LmInfo** lm) {
       }
       w4_attr(w4_mma_kernel<true, 1, 1, G, W>);
       w4_attr(w4_mma_kernel<false, 1, 1, G, W>);
-      w4_attr(w4_mma_kernel<true, 2, 2, G, W>);
-      w4_attr(w4_mma_kernel<true, 4, 2, G, W>);
-      w4_attr(w4_mma_kernel<false, 2, 2, G, W>);
-      w4_attr(w4_mma_kernel<false, 4, 2, G, W>);
     };
     auto w4_all = [&](auto gpb) {
+      constexpr int G = decltype(gpb)::value;
+      w4_attr(w4_tc_kernel<true, G>);
+      w4_attr(w4_tc_kernel<false, G>);
       w4_attrs(gpb, std::true_type{});
       w4_attrs(gpb, std::false_type{});
     };
@@ -587,7 +586,8 @@ int64_t w4_stream_fixed(int nt, int gpb, bool wide) {
 
 struct W4Plan {
   bool stream = false;   // w4_stream_kernel
-  bool mma = false;      // w4_mma_kernel; otherwise expanded weights and a plain product
+  bool mma = false;      // w4_mma_kernel
+  bool tc = false;       // w4_tc_kernel; otherwise expanded weights and a plain product
   bool pack_x = false;   // x is copied to aligned rows first (expanded weights)
   int nt = 1, mt = 1, splits = 1, row_warps = 1, slab = 1, per_cta = 0, ctas = 0;
   bool cut_before = false;
@@ -620,8 +620,9 @@ int check_w4_pointers(const W4Call& c) {
 }
 
 // How many rows of x run where: one or two (a tile of 8 columns of digits; fp32: up to 8, four
-// tiles) on w4_stream_kernel, up to 32 rows of 16-bit x on w4_mma_kernel; above, W is expanded once into the workspace and
-// multiplied on the tcgen05 kernels (fp32: 3xTF32).
+// tiles) on w4_stream_kernel; three to 8 of 16-bit x on w4_mma_kernel; up to 128 of 16-bit x
+// whose type the scales share on w4_tc_kernel; for the rest W is expanded once into the
+// workspace and multiplied on the tcgen05 kernels (fp32: 3xTF32).
 constexpr int64_t kW4MaxCols = 32;
 
 void plan_w4(const W4Call& c, const DeviceInfo& d, const LmInfo& lm, W4Plan* p) {
@@ -664,10 +665,29 @@ void plan_w4(const W4Call& c, const DeviceInfo& d, const LmInfo& lm, W4Plan* p) 
       p->off_sums = take(size_t(p->blocks) * gpb * pad * 4);
       p->off_scale = take(size_t(p->blocks) * pad * 4);
     }
-  } else if (!f32 && c.M <= kW4MaxCols) {
+  } else if (!f32 && c.M > 8 && c.M <= W4TcCfg<1>::kMaxCols && c.sdt == c.dtype) {
+    p->tc = true;
+    p->pack_x = !rows_aligned16(c.x, c.ldx);
+    if (p->pack_x) p->off_x = take(size_t(c.M) * p->kp * 2);
+    // K splits: waves of one CTA per SM, each split's share of K, and about a microsecond's
+    // worth (4 blocks) of start-up per CTA and of slab traffic per split.
+    const int64_t tiles = cdiv(c.N, W4TcCfg<1>::kRows);
+    double best = 0;
+    for (int sp = 1; sp <= 8 && sp * 4 <= p->blocks + 3; ++sp) {
+      const double cost = double(cdiv(tiles * sp, d.sms)) * (double(cdiv(p->blocks, sp)) + 8.0) + 2.0 * (sp - 1);
+      if (sp == 1 || cost < best) {
+        best = cost;
+        p->splits = sp;
+      }
+    }
+    p->per_cta = static_cast<int>(round_up(cdiv(p->blocks, p->splits), 2));
+    p->splits = static_cast<int>(cdiv(p->blocks, p->per_cta));
+    p->ldslab = round_up(c.N, 8);
+    if (p->splits > 1) p->off_slabs = take(size_t(p->splits) * c.M * p->ldslab * 4);
+  } else if (!f32 && c.M <= 8) {
     p->mma = true;
-    p->nt = c.M <= 8 ? 1 : c.M <= 16 ? 2 : 4;
-    p->mt = c.M <= 8 ? 1 : 2;
+    p->nt = 1;
+    p->mt = 1;
     p->row_warps = 8;
     const int64_t tiles = cdiv(c.N, 16 * p->mt * p->row_warps), slots = int64_t(d.sms) * (p->mt == 1 ? 3 : 2);
     while (p->splits < 8 && tiles * p->splits * 2 <= slots && p->blocks >= 4 * p->splits) p->splits *= 2;
@@ -765,11 +785,7 @@ int launch_w4(const W4Args& a, const W4Plan& p, bool bf16, int sms, uint8_t* ws,
       return a.scale_bf16 ? by_columns(std::integral_constant<int, TILEC_DTYPE_BF16>{})
                           : by_columns(std::integral_constant<int, TILEC_DTYPE_F16>{});
   }
-  if (p.nt == 1)
-    return bf16 ? launch_w4_mma<true, 1, 1, GPB, WIDE>(a, sms, s) : launch_w4_mma<false, 1, 1, GPB, WIDE>(a, sms, s);
-  if (p.nt == 2)
-    return bf16 ? launch_w4_mma<true, 2, 2, GPB, WIDE>(a, sms, s) : launch_w4_mma<false, 2, 2, GPB, WIDE>(a, sms, s);
-  return bf16 ? launch_w4_mma<true, 4, 2, GPB, WIDE>(a, sms, s) : launch_w4_mma<false, 4, 2, GPB, WIDE>(a, sms, s);
+  return bf16 ? launch_w4_mma<true, 1, 1, GPB, WIDE>(a, sms, s) : launch_w4_mma<false, 1, 1, GPB, WIDE>(a, sms, s);
 }
 
 template <bool WIDE>
@@ -777,6 +793,49 @@ int launch_w4(const W4Args& a, const W4Plan& p, int gpb, bool bf16, int sms, uin
   return gpb == 4   ? launch_w4<4, WIDE>(a, p, bf16, sms, ws, s)
          : gpb == 2 ? launch_w4<2, WIDE>(a, p, bf16, sms, ws, s)
                     : launch_w4<1, WIDE>(a, p, bf16, sms, ws, s);
+}
+
+template <bool BF16, int GPB>
+int launch_w4_tc(const W4Args& w, const W4Plan& p, const CUtensorMap& tm, float* slabs, cudaStream_t s) {
+  W4TcArgs a;
+  a.w = w;
+  a.n_cols = static_cast<int>(round_up(w.M, 16));
+  a.per_cta = p.per_cta;
+  a.slabs = slabs;
+  a.lds = p.ldslab;
+  return launch_k(w4_tc_kernel<BF16, GPB>, dim3(static_cast<unsigned>(cdiv(w.N, W4TcCfg<GPB>::kRows) * w.splits)),
+                  dim3(W4TcCfg<GPB>::kThreads), W4TcCfg<GPB>::kSmemBytes, s, 1, tm, a);
+}
+
+int run_w4_tc(const W4Call& c, const W4Plan& p, W4Args a, int gpb, uint8_t* ws, const DeviceInfo& d, cudaStream_t s) {
+  const bool bf16 = c.dtype == TILEC_DTYPE_BF16;
+  const void* x = c.x;
+  int64_t ldx = c.ldx;
+  if (p.pack_x) {
+    TILEC_TRY(pack16(c.x, c.ldx, ws + p.off_x, p.kp, c.M, c.K, nullptr, nullptr, nullptr, 0, nullptr, d, s));
+    x = ws + p.off_x;
+    ldx = p.kp;
+  }
+  CUtensorMap tm;
+  TILEC_TRY(encode16(&tm, x, c.K, c.M, ldx, static_cast<int>(round_up(c.M, 16)), bf16));
+  float* slabs = reinterpret_cast<float*>(ws + p.off_slabs);
+  if (bf16)
+    TILEC_TRY((gpb == 4   ? launch_w4_tc<true, 4>(a, p, tm, slabs, s)
+               : gpb == 2 ? launch_w4_tc<true, 2>(a, p, tm, slabs, s)
+                          : launch_w4_tc<true, 1>(a, p, tm, slabs, s)));
+  else
+    TILEC_TRY((gpb == 4   ? launch_w4_tc<false, 4>(a, p, tm, slabs, s)
+               : gpb == 2 ? launch_w4_tc<false, 2>(a, p, tm, slabs, s)
+                          : launch_w4_tc<false, 1>(a, p, tm, slabs, s)));
+  if (p.splits == 1) return TILEC_OK;
+  int64_t blocks = cdiv(c.M * cdiv(c.N, 8), 256);
+  if (blocks > int64_t(d.sms) * 8) blocks = int64_t(d.sms) * 8;
+  return launch_k(f16_join_slabs_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, 1,
+                  static_cast<const float*>(slabs), p.splits, c.M * p.ldslab, p.ldslab,
+                  static_cast<const float*>(nullptr), static_cast<float*>(nullptr),
+                  static_cast<unsigned short*>(c.out), c.ldo, c.M, c.N, static_cast<const int*>(nullptr),
+                  static_cast<const int*>(nullptr), static_cast<const float*>(nullptr), 1.f, c.bias, bf16 ? 1 : 0,
+                  odd_rows(c.out, c.ldo, c.N) ? 0 : 1);
 }
 
 int run_w4(const W4Call& c, void* workspace, size_t ws_bytes, cudaStream_t s) {
@@ -797,7 +856,7 @@ int run_w4(const W4Call& c, void* workspace, size_t ws_bytes, cudaStream_t s) {
   a.K = static_cast<int>(c.K);
   a.blocks = static_cast<int>(p.blocks);
   const int gpb = c.group == 32 ? 4 : c.group == 64 ? 2 : 1;
-  if (p.stream || p.mma) {
+  if (p.stream || p.mma || p.tc) {
     a.x = c.x;
     a.ldx = c.ldx;
     a.dtype = c.dtype;
@@ -811,6 +870,7 @@ int run_w4(const W4Call& c, void* workspace, size_t ws_bytes, cudaStream_t s) {
     a.row_warps = p.row_warps;
     a.slab = p.slab;
     const bool bf16 = c.dtype == TILEC_DTYPE_BF16;
+    if (p.tc) return run_w4_tc(c, p, a, gpb, ws, *d, s);
     return a.wide ? launch_w4<true>(a, p, gpb, bf16, d->sms, ws, s) : launch_w4<false>(a, p, gpb, bf16, d->sms, ws, s);
   }
   const void* x = c.x;

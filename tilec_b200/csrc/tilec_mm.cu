@@ -31,6 +31,7 @@
 #include "linear_ce.cuh"
 #include "w4.cuh"
 #include "w4_stream.cuh"
+#include "w4_tc.cuh"
 
 static_assert(TILEC_DEV_STATUS_TIMEOUT == tilec::TILEC_DEV_TIMEOUT && TILEC_DEV_STATUS_TMEM == tilec::TILEC_DEV_TMEM &&
                   TILEC_DEV_STATUS_BAD_LAUNCH == tilec::TILEC_DEV_BAD_LAUNCH &&

@@ -1,0 +1,274 @@
+// w4_tc.cuh -- products of some tens of rows with 4-bit weights on the 5th-generation tensor
+// cores (tcgen05, fp32 accumulators in TMEM), the weight expanded on the way.
+//
+// From 9 rows of x on, mma.sync's share of the work grows with the rows while the weight still
+// has to be read once; expanding it in HBM first (w4_expand_kernel) costs five times its bytes.
+// Here a CTA takes 128 rows of W as the M side of the product and up to 128 rows of x as its N
+// side (swapped, so that the few rows of x pad to 16 and not to 128 or 256):
+//   * one thread fetches codes (bulk copies of two blocks per 16-row tile, a run of memory
+//     each) and x (TMA boxes of 64 k x rows, 128-byte swizzle) into rings;
+//   * 16 warps expand: 8 codes of a row become one 16-byte piece of the K-major operand tile,
+//     (code - zero) exactly, times the scale with one rounding to x's type, and go where the
+//     swizzle wants them.  Two groups of 8 warps take alternate blocks, a buffer each;
+//   * one thread issues the MMAs (M = 128, N = rows of x, K = 16);
+//   * the same 16 warps read the accumulator and store: lanes are rows of W, so a warp stores
+//     32 neighbouring outputs of one row of x.
+// K is split over CTAs that write fp32 slabs (f16_join_slabs_kernel adds them in order).
+#pragma once
+
+#include "w4_stream.cuh"
+
+namespace tilec {
+
+struct W4TcArgs {
+  W4Args w;
+  int n_cols;          // rows of x rounded up to 16
+  int per_cta;         // blocks of K a CTA takes (even)
+  float* slabs;        // splits > 1: [split][M][lds]
+  int64_t lds;
+};
+
+template <int GPB>
+struct W4TcCfg {
+  static constexpr int kExpandWarps = 16;
+  static constexpr int kThreads = 64 + 32 * kExpandWarps;
+  static constexpr int kRows = 128;
+  static constexpr int kMaxCols = 128;
+  static constexpr int kPiece = w4_piece_bytes(GPB, false);
+  static constexpr int kCodeTile = 2 * kPiece;                 // two blocks of one 16-row tile
+  static constexpr int kCodeStage = 8 * kCodeTile;
+  static constexpr int kCodeStages = 3;
+  static constexpr int kHalf = kRows * 128;                    // 64 of K, K-major
+  static constexpr int kABytes = 2 * kHalf;                    // a block
+  static constexpr int kBStages = 3;
+  static constexpr int kBBytes = 2 * kMaxCols * 128;
+  static constexpr int kOffB = 2 * kABytes, kOffCodes = kOffB + kBStages * kBBytes;
+  static constexpr int kOffBars = kOffCodes + kCodeStages * kCodeStage;
+  static constexpr int kBarBytes = 256;
+  static constexpr int kSmemBytes = kOffBars + kBarBytes + 1024;
+  static_assert(kSmemBytes <= 232448 && kOffBars % 16 == 0, "shared memory");
+};
+
+// D[tmem] (+)= A[smem desc] * B[smem desc], kind::f16, one CTA.
+__device__ __forceinline__ void umma_16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t mul_16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if constexpr (BF16)
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// Grid: x = 128-row tiles * splits.  The scales are of x's type (a product of two such numbers
+// rounds once).
+template <bool BF16, int GPB>
+__global__ void __launch_bounds__(W4TcCfg<GPB>::kThreads, 1)
+    w4_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ W4TcArgs a) {
+  using Cfg = W4TcCfg<GPB>;
+  constexpr int WB = w4_word_bytes(GPB, false), SC = Cfg::kCodeStages, SB = Cfg::kBStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* a_buf = smem;                        // [2][kABytes]
+  uint8_t* b_buf = smem + Cfg::kOffB;           // [SB][kBBytes]
+  uint8_t* codes = smem + Cfg::kOffCodes;       // [SC][16-row tile][kCodeTile]
+  uint64_t* c_full = reinterpret_cast<uint64_t*>(smem + Cfg::kOffBars);
+  uint64_t* c_empty = c_full + SC;
+  uint64_t* b_full = c_empty + SC;
+  uint64_t* b_empty = b_full + SB;
+  uint64_t* a_full = b_empty + SB;   // [2]
+  uint64_t* a_empty = a_full + 2;    // [2]
+  uint64_t* acc_full = a_empty + 2;
+  uint64_t* drain_bar = acc_full + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  const W4Args& p = a.w;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (blockDim.x != Cfg::kThreads) {
+    if (threadIdx.x == 0) record_status(TILEC_DEV_BAD_LAUNCH);
+    return;
+  }
+  const int tile = static_cast<int>(blockIdx.x) / p.splits, split = static_cast<int>(blockIdx.x) - tile * p.splits;
+  const int n0 = tile * Cfg::kRows;
+  const int b_begin = min(p.blocks, split * a.per_cta), b_end = min(p.blocks, b_begin + a.per_cta);
+  const int nblk = b_end - b_begin;
+  const uint32_t tmem_cols = a.n_cols <= 32 ? 32 : a.n_cols <= 64 ? 64 : 128;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < SC; ++s) {
+      mbar_init(&c_full[s], 1);
+      mbar_init(&c_empty[s], Cfg::kExpandWarps);
+    }
+    for (int s = 0; s < SB; ++s) {
+      mbar_init(&b_full[s], 1);
+      mbar_init(&b_empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&a_full[s], Cfg::kExpandWarps / 2);
+      mbar_init(&a_empty[s], 1);
+    }
+    mbar_init(acc_full, 1);
+    mbar_init(drain_bar, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&tm_x);
+  }
+  if (warp == 1) {
+    __syncwarp();
+    tmem_alloc(tmem_slot, tmem_cols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  pdl_launch_dependents();
+
+  bool ok = true;
+  if (warp == 0) {
+    // ------------------------------------------------------------ fetching thread
+    if (lane == 0) {
+      const int row_tiles = min(8, (p.N - n0 + 15) / 16);
+      const uint32_t half_bytes = static_cast<uint32_t>(a.n_cols) * 128;
+      int i = 0;
+      for (; i < nblk && ok; ++i) {
+        if ((i & 1) == 0) {  // codes of this block and the next
+          const int u = i >> 1, s = u % SC, run = min(2, nblk - i);
+          if (u >= SC && !mbar_wait(&c_empty[s], ((u / SC) - 1) & 1, abort_flag)) { ok = false; break; }
+          mbar_arrive_expect_tx(&c_full[s], static_cast<uint32_t>(row_tiles * run * Cfg::kPiece));
+          const uint8_t* src = p.data + (static_cast<int64_t>(tile) * 8 * p.blocks + b_begin + i) * Cfg::kPiece;
+          for (int r = 0; r < row_tiles; ++r)
+            bulk_load(codes + s * Cfg::kCodeStage + r * Cfg::kCodeTile,
+                      src + static_cast<int64_t>(r) * p.blocks * Cfg::kPiece, run * Cfg::kPiece, &c_full[s]);
+        }
+        const int s = i % SB;
+        if (i >= SB && !mbar_wait(&b_empty[s], ((i / SB) - 1) & 1, abort_flag)) { ok = false; break; }
+        mbar_arrive_expect_tx(&b_full[s], 2 * half_bytes);
+        for (int h = 0; h < 2; ++h)
+          tma_load_2d(b_buf + s * Cfg::kBBytes + h * half_bytes, &tm_x, &b_full[s], (b_begin + i) * kW4Block + 64 * h, 0);
+      }
+      // Every copy has landed before this CTA may end, on every path.
+      const int units = (i + 1) / 2;
+      for (int f = max(0, units - SC); f < units; ++f) mbar_drain(&c_full[f % SC], (f / SC) & 1);
+      for (int f = max(0, i - SB); f < i; ++f) mbar_drain(&b_full[f % SB], (f / SB) & 1);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      const uint32_t idesc = make_idesc_16(128, a.n_cols, BF16, false, false);
+      for (int i = 0; i < nblk; ++i) {
+        const int s = i % SB, buf = i & 1;
+        if (!mbar_wait(&b_full[s], (i / SB) & 1, abort_flag) || !mbar_wait(&a_full[buf], (i >> 1) & 1, abort_flag)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t at = smem_u32(a_buf + buf * Cfg::kABytes), bt = smem_u32(b_buf + s * Cfg::kBBytes);
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk)
+          umma_16(tmem,
+                  make_smem_desc(at + (kk >> 2) * Cfg::kHalf + (kk & 3) * 32, 16, 1024, kLayoutSw128),
+                  make_smem_desc(bt + (kk >> 2) * a.n_cols * 128 + (kk & 3) * 32, 16, 1024, kLayoutSw128), idesc,
+                  i > 0 || kk > 0);
+        umma_commit(&a_empty[buf]);
+        umma_commit(&b_empty[s]);
+      }
+      if (ok) umma_commit(acc_full);
+      umma_commit(drain_bar);  // every MMA issued here completes before this thread goes on
+      mbar_drain(drain_bar, 0);
+    }
+  } else {
+    // ------------------------------------------------------------ expanding, then storing warps
+    const int e = warp - 2, group = e >> 3;  // blocks group, group + 2, ...
+    const int g = lane >> 2, t = lane & 3;
+    // Rows of the 16-row tile: pairs of lane groups whose codes and operand pieces lie in
+    // different banks.
+    const int row = (g & 1) ? (g >> 1) ^ 5 : g >> 1;
+    const uint32_t rt = e & 7;
+    uint32_t magic;
+    asm volatile("mov.b32 %0, %1;" : "=r"(magic) : "n"(BF16 ? 0x43004300u : 0x64006400u));
+    for (int i = group; i < nblk; i += 2) {
+      const int u = i >> 1, s = u % SC;
+      ok = __all_sync(0xffffffffu, mbar_wait(&c_full[s], (u / SC) & 1, abort_flag) &&
+                                       (i < 2 || mbar_wait(&a_empty[group], ((i >> 1) - 1) & 1, abort_flag)));
+      if (!ok) break;
+      const uint32_t piece = smem_u32(codes) + s * Cfg::kCodeStage + rt * Cfg::kCodeTile + (i & 1) * Cfg::kPiece;
+      const uint32_t dst = smem_u32(a_buf) + group * Cfg::kABytes + (16 * rt + row) * 128;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {  // row, row + 8
+        const uint4 q = lds128(piece + 16 * WB + (row + 8 * h) * 64 + t * 16);
+        uint32_t words[WB / 4];
+        lds_words(words, piece + (row + 8 * h) * WB);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t word = words[j * GPB / 4];
+          const uint32_t zm = magic | __byte_perm(word, 0, 0x1010), sc = __byte_perm(word, 0, 0x3232);
+          const uint32_t w = j == 0 ? q.x : j == 1 ? q.y : j == 2 ? q.z : q.w;
+          uint32_t v[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) v[k] = mul_16x2<BF16>(w4_pair<BF16>(w, k, magic, zm), sc);
+          // Piece 4j + t of the row's 16: half j >> 1, exchanged by the row's low bits.
+          const uint32_t chunk = (4 * (j & 1) + t) ^ (row & 7);
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst + h * 1024 + (j >> 1) * Cfg::kHalf +
+                                                                         chunk * 16),
+                       "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3])
+                       : "memory");
+        }
+      }
+      fence_proxy_async_smem();  // the MMAs read what was just stored
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&a_full[group]);
+        mbar_arrive(&c_empty[s]);
+        // A last unit of one block is not touched by the other group.
+        if ((i & 1) == 0 && i + 1 == nblk) mbar_arrive(&c_empty[s]);
+      }
+    }
+    if (ok) ok = __all_sync(0xffffffffu, nblk == 0 || mbar_wait(acc_full, 0, abort_flag));
+    tc_fence_after();
+    const int q = warp & 3, col0 = (e >> 2) * 32;  // TMEM lanes 32q .., 32 columns
+    const int n = n0 + 32 * q + lane;
+    if (col0 < a.n_cols) {
+      uint32_t r[32];
+      if (nblk > 0 && ok) {
+        tmem_ld_32x32b_x32(tmem + (static_cast<uint32_t>(32 * q) << 16) + col0, r);
+        tmem_ld_wait();
+      } else {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) r[j] = ok ? 0u : 0x7fc00000u;  // gave up: NaN
+      }
+      if (n < p.N) {
+        const float bias = p.splits == 1 && p.bias != nullptr ? load_16(p.bias, n, BF16) : 0.f;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          const int m = col0 + j;
+          if (m >= p.M) break;
+          const float v = __uint_as_float(r[j]);
+          if (p.splits > 1)
+            a.slabs[(static_cast<int64_t>(split) * p.M + m) * a.lds + n] = v;
+          else
+            store_from_float(p.out, int64_t(m) * p.ldo + n, BF16 ? 2 : 1, v + bias);
+        }
+      }
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, tmem_cols);
+  }
+}
+
+}  // namespace tilec

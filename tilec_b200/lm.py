@@ -296,13 +296,13 @@ def matrix_mul_w4(x, weight, bias=None, out=None):
     bfloat16 on the weight's device; bias None or [N] of x's dtype.  Returns (or writes into
     `out`, [..., N] with unit column stride) x's dtype.
 
-    Up to 32 rows of x (float32: 8), the decoding case, the codes are read once and enter
-    exactly: sums are fp32, with one rounding at the end.  Up to 8 of them go through
-    the integer tensor path, where x is held in steps of 2^-29 of the power of two at or below
-    the largest magnitude of its block of 128.  More rows: the weight is
-    expanded into the workspace, rounded to x's dtype (float32: exact), at most 256 MiB (or
-    256 rows of it) at a time, and multiplied on the tensor cores (float32: the 3xTF32 product
-    of matrix_mul).  Not differentiable."""
+    Up to 8 rows of x, the decoding case, the codes are read once and enter exactly: sums are
+    fp32, with one rounding at the end.  One or two rows (float32: all 8) go through the integer
+    tensor path, where x is held in steps of 2^-29 of the power of two at or below the largest
+    magnitude of its block of 128.  With more rows the weight is rounded once to x's dtype and
+    multiplied on the tensor cores: up to 128 rows of 16-bit x (and scales of its dtype) it is
+    expanded on the way, otherwise into the workspace, at most 256 MiB (or 256 rows of it) at a
+    time (float32: exact, and the 3xTF32 product of matrix_mul).  Not differentiable."""
     if not isinstance(weight, W4Weight):
         raise TypeError(f"matrix_mul_w4: weight must be a W4Weight (pack_w4, quantize_w4), got {type(weight).__name__}")
     n, k = weight.shape
