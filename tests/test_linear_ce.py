@@ -430,3 +430,35 @@ def test_captured_training_step(dtype):
     for (_, _, out), ref in zip(graphs, want):
         for a, b in zip(out, ref):
             assert torch.equal(a, b)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_gave_up_is_nan_and_the_context_works(dtype):
+    """Every bounded wait cut to 1 ns: the loss and gradients that were not finished are NaN,
+    the status word says so, and the next call with the limit restored is right."""
+    from tilec_b200 import _native
+    x, w, y = _make(600, 2000, 1024, dtype, ignored=0.1)
+    x.requires_grad_(True), w.requires_grad_(True)
+
+    def step():
+        loss = ext.linear_cross_entropy(x, w, y)
+        return (loss.detach(), *torch.autograd.grad(loss, (x, w)))
+
+    good = step()
+    ext.check_device()
+    lib = _native.load()
+    _native.check(lib.tilec_mm_set_wait_limit(1, None), "set_wait_limit")
+    try:
+        bad = step()
+        torch.cuda.synchronize()
+        with pytest.raises(TilecError, match="TIMEOUT"):
+            ext.check_device()
+    finally:
+        _native.check(lib.tilec_mm_set_wait_limit(0, None), "set_wait_limit")
+    for b, g in zip(bad, good):
+        assert torch.isnan(b).any() or torch.equal(b, g)
+    assert any(torch.isnan(b).any() for b in bad)
+    for again, g in zip(step(), good):
+        assert torch.equal(again, g)
+    ext.check_device()

@@ -386,3 +386,38 @@ def test_train_quantise_serve(dtype):
         want = torch.logsumexp(ref, 1) - ref.gather(1, y[:, None])[:, 0]
         e = 1e-5 + 2e-6 * (x.double().norm(dim=1).max() * w.norm(dim=1).max()).item()
         assert ((got - want).abs() <= e + 1e-5 * want).all()
+
+
+@gpu
+@pytest.mark.parametrize("m,dtype", [(1, "bf16"), (5, "f32"), (4, "f16"), (64, "bf16"), (200, "f16"), (300, "bf16")])
+def test_gave_up_is_nan_or_right_and_the_context_works(m, dtype, monkeypatch):
+    """Every bounded wait cut to 1 ns: what a kernel did not finish is NaN (a few-row kernel may
+    compute such outputs one by one instead), the status word says so, and the next call with
+    the limit restored is right.  No fault, no endless wait."""
+    from tilec_b200 import TilecError, _native
+    x, codes, scales, zeros, _ = _make(m, 260, 2048, 64, dtype)
+    w = ext.pack_w4(codes, scales, zeros, 64).to("cuda")
+    x = x.cuda()
+    good = ext.matrix_mul_w4(x, w)
+    out = torch.full_like(good, 12345.0)
+    ext.check_device()
+    lib = _native.load()
+    _native.check(lib.tilec_mm_set_wait_limit(1, None), "set_wait_limit")
+    try:
+        ext.matrix_mul_w4(x, w, out=out)
+        torch.cuda.synchronize()
+        gave_up = False
+        try:
+            ext.check_device()
+        except TilecError as e:
+            assert "TIMEOUT" in str(e)
+            gave_up = True
+    finally:
+        _native.check(lib.tilec_mm_set_wait_limit(0, None), "set_wait_limit")
+    nan = torch.isnan(out)
+    assert gave_up or not nan.any()
+    w64 = _weight64(codes, scales, zeros, 64).cuda()
+    err = (out.double() - x.double() @ w64.t()).abs()
+    assert (err[~nan] <= _bound(x.cpu(), w64.cpu(), good.cpu().double(), dtype, m).cuda()[~nan] * 2).all()
+    assert torch.equal(ext.matrix_mul_w4(x, w), good)
+    ext.check_device()

@@ -620,8 +620,9 @@ int check_w4_pointers(const W4Call& c) {
 }
 
 // How many rows of x run where: one or two (a tile of 8 columns of digits; fp32: up to 8, four
-// tiles) on w4_stream_kernel; three to 8 of 16-bit x on w4_mma_kernel; up to 128 of 16-bit x
-// whose type the scales share on w4_tc_kernel; for the rest W is expanded once into the
+// tiles) on w4_stream_kernel; three to 8 of 16-bit x on w4_mma_kernel; up to 256 of 16-bit x
+// whose type the scales share on w4_tc_kernel, 128 at a time (8192 x 8192: 128 rows 35 us, twice
+// that for 256; expanded first, either takes 89); for the rest W is expanded once into the
 // workspace and multiplied on the tcgen05 kernels (fp32: 3xTF32).
 constexpr int64_t kW4MaxCols = 32;
 
@@ -665,7 +666,7 @@ void plan_w4(const W4Call& c, const DeviceInfo& d, const LmInfo& lm, W4Plan* p) 
       p->off_sums = take(size_t(p->blocks) * gpb * pad * 4);
       p->off_scale = take(size_t(p->blocks) * pad * 4);
     }
-  } else if (!f32 && c.M > 8 && c.M <= W4TcCfg<1>::kMaxCols && c.sdt == c.dtype) {
+  } else if (!f32 && c.M > 8 && c.M <= 2 * W4TcCfg<1>::kMaxCols && c.sdt == c.dtype) {
     p->tc = true;
     p->pack_x = !rows_aligned16(c.x, c.ldx);
     if (p->pack_x) p->off_x = take(size_t(c.M) * p->kp * 2);
@@ -683,7 +684,9 @@ void plan_w4(const W4Call& c, const DeviceInfo& d, const LmInfo& lm, W4Plan* p) 
     p->per_cta = static_cast<int>(round_up(cdiv(p->blocks, p->splits), 2));
     p->splits = static_cast<int>(cdiv(p->blocks, p->per_cta));
     p->ldslab = round_up(c.N, 8);
-    if (p->splits > 1) p->off_slabs = take(size_t(p->splits) * c.M * p->ldslab * 4);
+    if (p->splits > 1)
+      p->off_slabs =
+          take(size_t(p->splits) * (c.M < W4TcCfg<1>::kMaxCols ? c.M : W4TcCfg<1>::kMaxCols) * p->ldslab * 4);
   } else if (!f32 && c.M <= 8) {
     p->mma = true;
     p->nt = 1;
@@ -816,26 +819,35 @@ int run_w4_tc(const W4Call& c, const W4Plan& p, W4Args a, int gpb, uint8_t* ws, 
     x = ws + p.off_x;
     ldx = p.kp;
   }
-  CUtensorMap tm;
-  TILEC_TRY(encode16(&tm, x, c.K, c.M, ldx, static_cast<int>(round_up(c.M, 16)), bf16));
   float* slabs = reinterpret_cast<float*>(ws + p.off_slabs);
-  if (bf16)
-    TILEC_TRY((gpb == 4   ? launch_w4_tc<true, 4>(a, p, tm, slabs, s)
-               : gpb == 2 ? launch_w4_tc<true, 2>(a, p, tm, slabs, s)
-                          : launch_w4_tc<true, 1>(a, p, tm, slabs, s)));
-  else
-    TILEC_TRY((gpb == 4   ? launch_w4_tc<false, 4>(a, p, tm, slabs, s)
-               : gpb == 2 ? launch_w4_tc<false, 2>(a, p, tm, slabs, s)
-                          : launch_w4_tc<false, 1>(a, p, tm, slabs, s)));
-  if (p.splits == 1) return TILEC_OK;
-  int64_t blocks = cdiv(c.M * cdiv(c.N, 8), 256);
-  if (blocks > int64_t(d.sms) * 8) blocks = int64_t(d.sms) * 8;
-  return launch_k(f16_join_slabs_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, 1,
-                  static_cast<const float*>(slabs), p.splits, c.M * p.ldslab, p.ldslab,
-                  static_cast<const float*>(nullptr), static_cast<float*>(nullptr),
-                  static_cast<unsigned short*>(c.out), c.ldo, c.M, c.N, static_cast<const int*>(nullptr),
-                  static_cast<const int*>(nullptr), static_cast<const float*>(nullptr), 1.f, c.bias, bf16 ? 1 : 0,
-                  odd_rows(c.out, c.ldo, c.N) ? 0 : 1);
+  constexpr int64_t kStep = W4TcCfg<1>::kMaxCols;
+  for (int64_t m0 = 0; m0 < c.M; m0 += kStep) {
+    const int64_t m = c.M - m0 < kStep ? c.M - m0 : kStep;
+    CUtensorMap tm;
+    TILEC_TRY(encode16(&tm, static_cast<const unsigned short*>(x) + m0 * ldx, c.K, m, ldx,
+                       static_cast<int>(round_up(m, 16)), bf16));
+    unsigned short* out = static_cast<unsigned short*>(c.out) + m0 * c.ldo;
+    a.M = static_cast<int>(m);
+    a.out = out;
+    if (bf16)
+      TILEC_TRY((gpb == 4   ? launch_w4_tc<true, 4>(a, p, tm, slabs, s)
+                 : gpb == 2 ? launch_w4_tc<true, 2>(a, p, tm, slabs, s)
+                            : launch_w4_tc<true, 1>(a, p, tm, slabs, s)));
+    else
+      TILEC_TRY((gpb == 4   ? launch_w4_tc<false, 4>(a, p, tm, slabs, s)
+                 : gpb == 2 ? launch_w4_tc<false, 2>(a, p, tm, slabs, s)
+                            : launch_w4_tc<false, 1>(a, p, tm, slabs, s)));
+    if (p.splits == 1) continue;
+    int64_t blocks = cdiv(m * cdiv(c.N, 8), 256);
+    if (blocks > int64_t(d.sms) * 8) blocks = int64_t(d.sms) * 8;
+    TILEC_TRY(launch_k(f16_join_slabs_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, s, 1,
+                       static_cast<const float*>(slabs), p.splits, m * p.ldslab, p.ldslab,
+                       static_cast<const float*>(nullptr), static_cast<float*>(nullptr), out, c.ldo, m, c.N,
+                       static_cast<const int*>(nullptr), static_cast<const int*>(nullptr),
+                       static_cast<const float*>(nullptr), 1.f, c.bias, bf16 ? 1 : 0,
+                       odd_rows(out, c.ldo, c.N) ? 0 : 1));
+  }
+  return TILEC_OK;
 }
 
 int run_w4(const W4Call& c, void* workspace, size_t ws_bytes, cudaStream_t s) {

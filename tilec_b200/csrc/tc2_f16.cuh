@@ -145,11 +145,14 @@ __device__ __noinline__ bool mbar_poll(uint32_t bar, uint32_t parity, volatile i
   }
 }
 constexpr uint32_t kHintStage = 64, kHintTile = 1000;  // ns
+// A short loop first: entering the call costs the MMA thread more than polling (0.79 -> 0.74
+// ms).  `tries`: its length, 1 where the device's limit is shortened.
+__device__ __forceinline__ int wait_tries() { return wait_limit() < kWaitLimitNs ? 1 : 32; }
 template <bool CLUSTER>
-__device__ __forceinline__ bool mbar_wait_far(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint32_t hint) {
-  // A short loop first: entering the call costs the MMA thread more than polling (0.79 -> 0.74 ms).
+__device__ __forceinline__ bool mbar_wait_far(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint32_t hint,
+                                              int tries) {
 #pragma unroll 1
-  for (int i = 0; i < 32; ++i)
+  for (int i = 0; i < tries; ++i)
     if (mbar_try<CLUSTER>(bar, parity, kHintStage)) return true;
   return mbar_poll(bar, parity, abort_flag, hint);
 }
@@ -272,6 +275,7 @@ __global__ void __launch_bounds__(F16Cfg::kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   pdl_wait();
+  const int tries = wait_tries();
 
   const int counted = p.count != nullptr ? *p.count : 0;
   const int M = p.count != nullptr && !p.count_is_k ? counted : p.M;
@@ -314,7 +318,7 @@ __global__ void __launch_bounds__(F16Cfg::kThreads, 1)
         for (int kb = 0; kb < ta.nkb; ++kb) {
           const int s = g % STAGES;
           const uint32_t ph = (g / STAGES) & 1;
-          if (!mbar_wait_far<true>(smem_u32(&empty[s]), ph ^ 1, abort_flag, kHintStage)) { ok = false; break; }
+          if (!mbar_wait_far<true>(smem_u32(&empty[s]), ph ^ 1, abort_flag, kHintStage, tries)) { ok = false; break; }
           const int k0 = (ta.kb0 + kb) * BK;
           const int halves = K - k0 > 64 ? 2 : 1;
           mbar_arrive_expect_tx(&full[s], halves * 2 * Cfg::kHalfBytes);
@@ -341,7 +345,7 @@ __global__ void __launch_bounds__(F16Cfg::kThreads, 1)
       if (ok) {
         // Tail: the leader's release of each of the last fills has arrived before the CTA exits.
         for (int f = g - STAGES < 0 ? 0 : g - STAGES; f < g; ++f)
-          if (!mbar_wait_far<true>(smem_u32(&empty[f % STAGES]), (f / STAGES) & 1, abort_flag, kHintStage)) { ok = false; break; }
+          if (!mbar_wait_far<true>(smem_u32(&empty[f % STAGES]), (f / STAGES) & 1, abort_flag, kHintStage, tries)) { ok = false; break; }
       }
       if (!ok) {
         for (int f = g - STAGES < 0 ? 0 : g - STAGES; f < g; ++f) mbar_drain(&full[f % STAGES], (f / STAGES) & 1);
@@ -370,15 +374,15 @@ __global__ void __launch_bounds__(F16Cfg::kThreads, 1)
         const int nkb = ta.nkb;
         int left = K - ta.kb0 * BK;  // of K, from this stage on
         // Buffer b last held tile i - 2: both CTAs' epilogues must have drained it.
-        if (i >= 2 && !mbar_wait_far<true>(smem_u32(&acc_empty[b]), ((i >> 1) - 1) & 1, abort_flag, kHintStage)) {
+        if (i >= 2 && !mbar_wait_far<true>(smem_u32(&acc_empty[b]), ((i >> 1) - 1) & 1, abort_flag, kHintStage, tries)) {
           ok = false;
           break;
         }
         tc_fence_after();
         uint32_t accumulate = 0;
         for (int kb = 0; kb < nkb; ++kb) {
-          if (!mbar_wait_far<false>(full_at + 8 * s, ph, abort_flag, kHintStage) ||
-              !mbar_wait_far<true>(peer_at + 8 * s, ph, abort_flag, kHintStage)) {
+          if (!mbar_wait_far<false>(full_at + 8 * s, ph, abort_flag, kHintStage, tries) ||
+              !mbar_wait_far<true>(peer_at + 8 * s, ph, abort_flag, kHintStage, tries)) {
             ok = false;
             break;
           }
@@ -418,7 +422,7 @@ __global__ void __launch_bounds__(F16Cfg::kThreads, 1)
         const int nkb = tile_at(i).nkb;
         for (int kb = 0; kb < nkb; ++kb, ++g) {
           const int s = g % STAGES;
-          if (!mbar_wait_far<false>(smem_u32(&full[s]), (g / STAGES) & 1, abort_flag, kHintStage)) { ok = false; break; }
+          if (!mbar_wait_far<false>(smem_u32(&full[s]), (g / STAGES) & 1, abort_flag, kHintStage, tries)) { ok = false; break; }
           mbar_arrive_remote_cta(pf + static_cast<uint32_t>(s * 8));
         }
       }
@@ -455,7 +459,7 @@ __global__ void __launch_bounds__(F16Cfg::kThreads, 1)
         }
       }
       // One answer for the warp: what follows is warp-wide.
-      if (!__all_sync(0xffffffffu, mbar_wait_far<true>(smem_u32(&acc_full[b]), (i >> 1) & 1, abort_flag, kHintTile)))
+      if (!__all_sync(0xffffffffu, mbar_wait_far<true>(smem_u32(&acc_full[b]), (i >> 1) & 1, abort_flag, kHintTile, tries)))
         break;
       tc_fence_after();
       if (i == n_my - 1) pdl_launch_dependents();

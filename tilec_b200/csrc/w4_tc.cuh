@@ -5,15 +5,21 @@
 // has to be read once; expanding it in HBM first (w4_expand_kernel) costs five times its bytes.
 // Here a CTA takes 128 rows of W as the M side of the product and up to 128 rows of x as its N
 // side (swapped, so that the few rows of x pad to 16 and not to 128 or 256):
-//   * one thread fetches codes (bulk copies of two blocks per 16-row tile, a run of memory
-//     each) and x (TMA boxes of 64 k x rows, 128-byte swizzle) into rings;
+//   * one warp fetches codes (bulk copies of four blocks per 16-row tile, a run of memory each,
+//     a lane each: an SM starts one some 55 ns after another, so two blocks a copy were too
+//     few) and x (TMA boxes of 64 k x rows, 128-byte swizzle) into rings;
 //   * 16 warps expand: 8 codes of a row become one 16-byte piece of the K-major operand tile,
 //     (code - zero) exactly, times the scale with one rounding to x's type, and go where the
-//     swizzle wants them.  Two groups of 8 warps take alternate blocks, a buffer each;
+//     swizzle wants them.  Two groups of 8 warps take alternate blocks, into two buffers;
 //   * one thread issues the MMAs (M = 128, N = rows of x, K = 16);
 //   * the same 16 warps read the accumulator and store: lanes are rows of W, so a warp stores
 //     32 neighbouring outputs of one row of x.
 // K is split over CTAs that write fp32 slabs (f16_join_slabs_kernel adds them in order).
+//
+// Measured (graph replay): 4096 x 4096 10.7 us for 16 rows, 13.0 for 128; 8192 x 8192 25.2 and
+// 35 (the codes alone: 6 at HBM's rate); 28672 x 8192 82 and 112.  Without the expansion's
+// arithmetic it is no faster, without seven of eight MMAs a fifth: what bounds it is the
+// hand-over of a block between the roles (about half a microsecond).
 #pragma once
 
 #include "w4_stream.cuh"
@@ -35,14 +41,16 @@ struct W4TcCfg {
   static constexpr int kRows = 128;
   static constexpr int kMaxCols = 128;
   static constexpr int kPiece = w4_piece_bytes(GPB, false);
-  static constexpr int kCodeTile = 2 * kPiece;                 // two blocks of one 16-row tile
+  static constexpr int kRun = 4;                               // blocks a copy
+  static constexpr int kCodeTile = kRun * kPiece;              // of one 16-row tile
   static constexpr int kCodeStage = 8 * kCodeTile;
-  static constexpr int kCodeStages = 3;
+  static constexpr int kCodeStages = 2;
   static constexpr int kHalf = kRows * 128;                    // 64 of K, K-major
   static constexpr int kABytes = 2 * kHalf;                    // a block
-  static constexpr int kBStages = 3;
-  static constexpr int kBBytes = 2 * kMaxCols * 128;
-  static constexpr int kOffB = 2 * kABytes, kOffCodes = kOffB + kBStages * kBBytes;
+  static constexpr int kMaxBStages = 8;
+  static constexpr int kBBytes = 65536;                        // x: as many blocks as fit, up to 8
+  static constexpr int kABufs = 2;   // three, with copies of three blocks: as fast
+  static constexpr int kOffB = kABufs * kABytes, kOffCodes = kOffB + kBBytes;
   static constexpr int kOffBars = kOffCodes + kCodeStages * kCodeStage;
   static constexpr int kBarBytes = 256;
   static constexpr int kSmemBytes = kOffBars + kBarBytes + 1024;
@@ -76,19 +84,19 @@ template <bool BF16, int GPB>
 __global__ void __launch_bounds__(W4TcCfg<GPB>::kThreads, 1)
     w4_tc_kernel(const __grid_constant__ CUtensorMap tm_x, const __grid_constant__ W4TcArgs a) {
   using Cfg = W4TcCfg<GPB>;
-  constexpr int WB = w4_word_bytes(GPB, false), SC = Cfg::kCodeStages, SB = Cfg::kBStages;
+  constexpr int WB = w4_word_bytes(GPB, false), SC = Cfg::kCodeStages, RUN = Cfg::kRun, NA = Cfg::kABufs;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* a_buf = smem;                        // [2][kABytes]
-  uint8_t* b_buf = smem + Cfg::kOffB;           // [SB][kBBytes]
+  uint8_t* a_buf = smem;                        // [NA][kABytes]
+  uint8_t* b_buf = smem + Cfg::kOffB;           // [SB][half][n_cols][128]
   uint8_t* codes = smem + Cfg::kOffCodes;       // [SC][16-row tile][kCodeTile]
   uint64_t* c_full = reinterpret_cast<uint64_t*>(smem + Cfg::kOffBars);
   uint64_t* c_empty = c_full + SC;
   uint64_t* b_full = c_empty + SC;
-  uint64_t* b_empty = b_full + SB;
-  uint64_t* a_full = b_empty + SB;   // [2]
-  uint64_t* a_empty = a_full + 2;    // [2]
-  uint64_t* acc_full = a_empty + 2;
+  uint64_t* b_empty = b_full + Cfg::kMaxBStages;
+  uint64_t* a_full = b_empty + Cfg::kMaxBStages;   // [NA]
+  uint64_t* a_empty = a_full + NA;   // [NA]
+  uint64_t* acc_full = a_empty + NA;
   uint64_t* drain_bar = acc_full + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -102,18 +110,20 @@ __global__ void __launch_bounds__(W4TcCfg<GPB>::kThreads, 1)
   const int n0 = tile * Cfg::kRows;
   const int b_begin = min(p.blocks, split * a.per_cta), b_end = min(p.blocks, b_begin + a.per_cta);
   const int nblk = b_end - b_begin;
+  const uint32_t b_half = static_cast<uint32_t>(a.n_cols) * 128;  // bytes of x per 64 k
+  const int SB = min(Cfg::kMaxBStages, static_cast<int>(Cfg::kBBytes / (2 * b_half)));
   const uint32_t tmem_cols = a.n_cols <= 32 ? 32 : a.n_cols <= 64 ? 64 : 128;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < SC; ++s) {
       mbar_init(&c_full[s], 1);
-      mbar_init(&c_empty[s], Cfg::kExpandWarps);
+      mbar_init(&c_empty[s], Cfg::kExpandWarps / 2 * RUN);
     }
-    for (int s = 0; s < SB; ++s) {
+    for (int s = 0; s < Cfg::kMaxBStages; ++s) {
       mbar_init(&b_full[s], 1);
       mbar_init(&b_empty[s], 1);
     }
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < NA; ++s) {
       mbar_init(&a_full[s], Cfg::kExpandWarps / 2);
       mbar_init(&a_empty[s], 1);
     }
@@ -134,55 +144,79 @@ __global__ void __launch_bounds__(W4TcCfg<GPB>::kThreads, 1)
   const uint32_t tmem = *tmem_slot;
   pdl_wait();
   pdl_launch_dependents();
+  const int tries = wait_tries();
 
   bool ok = true;
   if (warp == 0) {
-    // ------------------------------------------------------------ fetching thread
-    if (lane == 0) {
-      const int row_tiles = min(8, (p.N - n0 + 15) / 16);
-      const uint32_t half_bytes = static_cast<uint32_t>(a.n_cols) * 128;
-      int i = 0;
-      for (; i < nblk && ok; ++i) {
-        if ((i & 1) == 0) {  // codes of this block and the next
-          const int u = i >> 1, s = u % SC, run = min(2, nblk - i);
-          if (u >= SC && !mbar_wait(&c_empty[s], ((u / SC) - 1) & 1, abort_flag)) { ok = false; break; }
-          mbar_arrive_expect_tx(&c_full[s], static_cast<uint32_t>(row_tiles * run * Cfg::kPiece));
-          const uint8_t* src = p.data + (static_cast<int64_t>(tile) * 8 * p.blocks + b_begin + i) * Cfg::kPiece;
-          for (int r = 0; r < row_tiles; ++r)
-            bulk_load(codes + s * Cfg::kCodeStage + r * Cfg::kCodeTile,
-                      src + static_cast<int64_t>(r) * p.blocks * Cfg::kPiece, run * Cfg::kPiece, &c_full[s]);
-        }
-        const int s = i % SB;
-        if (i >= SB && !mbar_wait(&b_empty[s], ((i / SB) - 1) & 1, abort_flag)) { ok = false; break; }
-        mbar_arrive_expect_tx(&b_full[s], 2 * half_bytes);
-        for (int h = 0; h < 2; ++h)
-          tma_load_2d(b_buf + s * Cfg::kBBytes + h * half_bytes, &tm_x, &b_full[s], (b_begin + i) * kW4Block + 64 * h, 0);
+    // ------------------------------------------------------------ fetching warp
+    const int row_tiles = min(8, (p.N - n0 + 15) / 16);
+    const uint8_t* src =
+        p.data + ((static_cast<int64_t>(tile) * 8 + min(lane, row_tiles - 1)) * p.blocks + b_begin) * Cfg::kPiece;
+    int i = 0, bs = 0;
+    uint32_t b_phase = 1;
+    for (; i < nblk && ok; ++i) {
+      if (i % RUN == 0) {  // codes of this block and the next ones
+        const int u = i / RUN, s = u % SC, run = min(RUN, nblk - i);
+        ok = __all_sync(0xffffffffu, u < SC || mbar_wait(&c_empty[s], ((u / SC) - 1) & 1, abort_flag));
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_expect_tx(&c_full[s], static_cast<uint32_t>(row_tiles * run * Cfg::kPiece));
+        __syncwarp();
+        if (lane < row_tiles)
+          bulk_load(codes + s * Cfg::kCodeStage + lane * Cfg::kCodeTile, src + static_cast<int64_t>(i) * Cfg::kPiece,
+                    run * Cfg::kPiece, &c_full[s]);
       }
-      // Every copy has landed before this CTA may end, on every path.
-      const int units = (i + 1) / 2;
+      ok = __all_sync(0xffffffffu, i < SB || mbar_wait(&b_empty[bs], b_phase, abort_flag));
+      if (!ok) break;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&b_full[bs], 2 * b_half);
+        for (int h = 0; h < 2; ++h)
+          tma_load_2d(b_buf + (2 * bs + h) * b_half, &tm_x, &b_full[bs], (b_begin + i) * kW4Block + 64 * h, 0);
+      }
+      if (++bs == SB) {
+        bs = 0;
+        b_phase ^= 1;
+      }
+    }
+    // Every copy has landed before this CTA may end, on every path.
+    if (lane == 0) {
+      const int units = (i + RUN - 1) / RUN;
       for (int f = max(0, units - SC); f < units; ++f) mbar_drain(&c_full[f % SC], (f / SC) & 1);
       for (int f = max(0, i - SB); f < i; ++f) mbar_drain(&b_full[f % SB], (f / SB) & 1);
     }
+    __syncwarp();
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
     if (lane == 0) {
       const uint32_t idesc = make_idesc_16(128, a.n_cols, BF16, false, false);
+      // Descriptors and addresses are carried along: this thread's own work per block counts.
+      const uint64_t a_desc = make_smem_desc(smem_u32(a_buf), 16, 1024, kLayoutSw128);
+      const uint64_t b_desc = make_smem_desc(smem_u32(b_buf), 16, 1024, kLayoutSw128);
+      const uint32_t af = smem_u32(a_full), bf = smem_u32(b_full);
+      uint32_t s = 0, b_phase = 0, buf = 0, a_phase = 0, accumulate = 0;
       for (int i = 0; i < nblk; ++i) {
-        const int s = i % SB, buf = i & 1;
-        if (!mbar_wait(&b_full[s], (i / SB) & 1, abort_flag) || !mbar_wait(&a_full[buf], (i >> 1) & 1, abort_flag)) {
+        if (!mbar_wait_far<false>(bf + 8 * s, b_phase, abort_flag, kHintStage, tries) ||
+            !mbar_wait_far<false>(af + 8 * buf, a_phase, abort_flag, kHintStage, tries)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const uint32_t at = smem_u32(a_buf + buf * Cfg::kABytes), bt = smem_u32(b_buf + s * Cfg::kBBytes);
+        const uint64_t ad = a_desc + buf * (Cfg::kABytes >> 4), bd = b_desc + s * (b_half >> 3);
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk)
-          umma_16(tmem,
-                  make_smem_desc(at + (kk >> 2) * Cfg::kHalf + (kk & 3) * 32, 16, 1024, kLayoutSw128),
-                  make_smem_desc(bt + (kk >> 2) * a.n_cols * 128 + (kk & 3) * 32, 16, 1024, kLayoutSw128), idesc,
-                  i > 0 || kk > 0);
+        for (int kk = 0; kk < 8; ++kk) {
+          umma_16(tmem, ad + (kk >> 2) * (Cfg::kHalf >> 4) + (kk & 3) * 2, bd + (kk >> 2) * (b_half >> 4) + (kk & 3) * 2, idesc,
+                  accumulate);
+          accumulate = 1;
+        }
         umma_commit(&a_empty[buf]);
         umma_commit(&b_empty[s]);
+        if (++buf == NA) {
+          buf = 0;
+          a_phase ^= 1;
+        }
+        if (++s == static_cast<uint32_t>(SB)) {
+          s = 0;
+          b_phase ^= 1;
+        }
       }
       if (ok) umma_commit(acc_full);
       umma_commit(drain_bar);  // every MMA issued here completes before this thread goes on
@@ -199,12 +233,12 @@ __global__ void __launch_bounds__(W4TcCfg<GPB>::kThreads, 1)
     uint32_t magic;
     asm volatile("mov.b32 %0, %1;" : "=r"(magic) : "n"(BF16 ? 0x43004300u : 0x64006400u));
     for (int i = group; i < nblk; i += 2) {
-      const int u = i >> 1, s = u % SC;
+      const int u = i / RUN, s = u % SC, buf = i % NA;
       ok = __all_sync(0xffffffffu, mbar_wait(&c_full[s], (u / SC) & 1, abort_flag) &&
-                                       (i < 2 || mbar_wait(&a_empty[group], ((i >> 1) - 1) & 1, abort_flag)));
+                                       (i < NA || mbar_wait(&a_empty[buf], ((i / NA) - 1) & 1, abort_flag)));
       if (!ok) break;
-      const uint32_t piece = smem_u32(codes) + s * Cfg::kCodeStage + rt * Cfg::kCodeTile + (i & 1) * Cfg::kPiece;
-      const uint32_t dst = smem_u32(a_buf) + group * Cfg::kABytes + (16 * rt + row) * 128;
+      const uint32_t piece = smem_u32(codes) + s * Cfg::kCodeStage + rt * Cfg::kCodeTile + (i % RUN) * Cfg::kPiece;
+      const uint32_t dst = smem_u32(a_buf) + buf * Cfg::kABytes + (16 * rt + row) * 128;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {  // row, row + 8
         const uint4 q = lds128(piece + 16 * WB + (row + 8 * h) * 64 + t * 16);
@@ -229,10 +263,8 @@ __global__ void __launch_bounds__(W4TcCfg<GPB>::kThreads, 1)
       fence_proxy_async_smem();  // the MMAs read what was just stored
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(&a_full[group]);
+        mbar_arrive(&a_full[buf]);
         mbar_arrive(&c_empty[s]);
-        // A last unit of one block is not touched by the other group.
-        if ((i & 1) == 0 && i + 1 == nblk) mbar_arrive(&c_empty[s]);
       }
     }
     if (ok) ok = __all_sync(0xffffffffu, nblk == 0 || mbar_wait(acc_full, 0, abort_flag));

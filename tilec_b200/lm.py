@@ -300,7 +300,7 @@ def matrix_mul_w4(x, weight, bias=None, out=None):
     fp32, with one rounding at the end.  One or two rows (float32: all 8) go through the integer
     tensor path, where x is held in steps of 2^-29 of the power of two at or below the largest
     magnitude of its block of 128.  With more rows the weight is rounded once to x's dtype and
-    multiplied on the tensor cores: up to 128 rows of 16-bit x (and scales of its dtype) it is
+    multiplied on the tensor cores: up to 256 rows of 16-bit x (and scales of its dtype) it is
     expanded on the way, otherwise into the workspace, at most 256 MiB (or 256 rows of it) at a
     time (float32: exact, and the 3xTF32 product of matrix_mul).  Not differentiable."""
     if not isinstance(weight, W4Weight):
