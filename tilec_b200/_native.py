@@ -158,7 +158,8 @@ def _load_fast(lib):
         spec.loader.exec_module(mod)
         mod.install(ctypes.cast(lib.tilec_mm_f32, ctypes.c_void_p).value,
                     ctypes.cast(lib.tilec_mm_workspace_bytes, ctypes.c_void_p).value)
-        mod.install_w4(ctypes.cast(lib.tilec_mm_w4, ctypes.c_void_p).value)
+        mod.install_lm(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
+            lib.tilec_mm_w4, lib.tilec_linear_ce_forward, lib.tilec_linear_ce_backward)))
         _fast = mod
     except Exception as e:  # noqa: BLE001
         _fast, _fast_error = None, f"{type(e).__name__}: {e}"

@@ -54,25 +54,65 @@ def _check_device(stream):
         _ext.check_device(stream)
 
 
+class _OnDevice:
+    """torch.cuda.device without its cost where the device is already the current one."""
+
+    __slots__ = ("index", "prev")
+
+    def __init__(self, index):
+        self.index = index
+
+    def __enter__(self):
+        self.prev = torch.cuda.current_device()
+        if self.prev != self.index:
+            torch.cuda.set_device(self.index)
+
+    def __exit__(self, *exc):
+        if self.prev != self.index:
+            torch.cuda.set_device(self.prev)
+
+
+_CE_BYTES = {}   # arguments that decide it -> workspace bytes of tilec_linear_ce_*
+
+
+def _ce_workspace(lib, px, pw, dt, t, v, d, ldx, ldw, red, grads, device):
+    """(workspace, bytes); operands count as far as their alignment goes."""
+    key = (dt, t, v, d, ldx, ldw, red, grads, (px or 0) & 15, pw & 15, device.index)
+    nbytes = _CE_BYTES.get(key)
+    if nbytes is None:
+        nbytes = lib.tilec_linear_ce_workspace_bytes(px, pw, dt, t, v, d, ldx, ldw, red, grads)
+        if len(_CE_BYTES) >= 4096:   # a process that sees many shapes: start over
+            _CE_BYTES.clear()
+        _CE_BYTES[key] = nbytes
+    return _workspace(nbytes, device), nbytes
+
+
+def _ce_forward(x, weight, target, ignore_index, reduction):
+    """(loss, statistics for the backward pass)"""
+    lib, fast, dev = _native.load(), _native.fast(), x.device
+    xr, ldx = _rows(x)
+    wr, ldw = _rows(weight)
+    t, d = x.shape
+    v = weight.shape[0]
+    dt, red = _DTYPES[x.dtype], _REDUCTIONS[reduction]
+    with _OnDevice(dev.index):
+        stats = torch.empty(2 * t + 1, dtype=torch.float32, device=dev)
+        loss = stats.new_empty(t if reduction == "none" else ())
+        px, pw = xr.data_ptr(), wr.data_ptr()
+        ws, nbytes = _ce_workspace(lib, px, pw, dt, t, v, d, ldx, ldw, red, 0, dev)
+        stream = _stream(dev)
+        rc = (fast.ce_forward if fast is not None else lib.tilec_linear_ce_forward)(
+            px, pw, target.data_ptr(), dt, t, v, d, ldx, ldw, ignore_index, red, loss.data_ptr(), stats.data_ptr(),
+            _ptr(ws), nbytes, stream)
+        _native.check(rc, "tilec_linear_ce_forward")
+        _check_device(stream)
+    return loss, stats
+
+
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, target, ignore_index, reduction):
-        lib = _native.load()
-        xr, ldx = _rows(x)
-        wr, ldw = _rows(weight)
-        t, d = x.shape
-        v = weight.shape[0]
-        dt, red = _DTYPES[x.dtype], _REDUCTIONS[reduction]
-        with torch.cuda.device(x.device):
-            loss = torch.empty(t if reduction == "none" else (), dtype=torch.float32, device=x.device)
-            stats = torch.empty(2 * t + 1, dtype=torch.float32, device=x.device)
-            nbytes = lib.tilec_linear_ce_workspace_bytes(_ptr(xr), _ptr(wr), dt, t, v, d, ldx, ldw, red, 0)
-            ws = _workspace(nbytes, x.device)
-            stream = _stream(x.device)
-            rc = lib.tilec_linear_ce_forward(_ptr(xr), _ptr(wr), _ptr(target), dt, t, v, d, ldx, ldw, ignore_index,
-                                             red, _ptr(loss), _ptr(stats), _ptr(ws), nbytes, stream)
-            _native.check(rc, "tilec_linear_ce_forward")
-            _check_device(stream)
+        loss, stats = _ce_forward(x, weight, target, ignore_index, reduction)
         ctx.save_for_backward(x, weight, target, stats)
         ctx.ignore_index, ctx.reduction = ignore_index, reduction
         return loss
@@ -81,23 +121,23 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad):
         x, weight, target, stats = ctx.saved_tensors
-        lib = _native.load()
+        lib, fast, dev = _native.load(), _native.fast(), x.device
         xr, ldx = _rows(x)
         wr, ldw = _rows(weight)
         t, d = x.shape
         v = weight.shape[0]
         dt, red = _DTYPES[x.dtype], _REDUCTIONS[ctx.reduction]
-        with torch.cuda.device(x.device):
+        with _OnDevice(dev.index):
             grad = grad.to(torch.float32).contiguous()
-            dx = torch.empty(t, d, dtype=x.dtype, device=x.device) if ctx.needs_input_grad[0] else None
-            dw = torch.empty(v, d, dtype=x.dtype, device=x.device) if ctx.needs_input_grad[1] else None
+            dx = x.new_empty(t, d) if ctx.needs_input_grad[0] else None
+            dw = weight.new_empty(v, d) if ctx.needs_input_grad[1] else None
             grads = (1 if dx is not None else 0) | (2 if dw is not None else 0)
-            nbytes = lib.tilec_linear_ce_workspace_bytes(_ptr(xr), _ptr(wr), dt, t, v, d, ldx, ldw, red, grads)
-            ws = _workspace(nbytes, x.device)
-            stream = _stream(x.device)
-            rc = lib.tilec_linear_ce_backward(_ptr(xr), _ptr(wr), _ptr(target), dt, t, v, d, ldx, ldw,
-                                              ctx.ignore_index, red, _ptr(stats), _ptr(grad), _ptr(dx), _ptr(dw),
-                                              _ptr(ws), nbytes, stream)
+            px, pw = xr.data_ptr(), wr.data_ptr()
+            ws, nbytes = _ce_workspace(lib, px, pw, dt, t, v, d, ldx, ldw, red, grads, dev)
+            stream = _stream(dev)
+            rc = (fast.ce_backward if fast is not None else lib.tilec_linear_ce_backward)(
+                px, pw, target.data_ptr(), dt, t, v, d, ldx, ldw, ctx.ignore_index, red, stats.data_ptr(),
+                grad.data_ptr(), _ptr(dx), _ptr(dw), _ptr(ws), nbytes, stream)
             _native.check(rc, "tilec_linear_ce_backward")
             _check_device(stream)
         return dx, dw, None, None, None
@@ -140,9 +180,15 @@ def linear_cross_entropy(x, weight, target, ignore_index=-100, reduction="mean")
     if not (x.is_cuda and weight.device == x.device and target.device == x.device):
         raise ValueError(f"linear_cross_entropy: inputs must be CUDA tensors on one device (got {x.device}, "
                          f"{weight.device} and {target.device}); tilec_b200 has no CPU path")
-    loss = _LinearCrossEntropy.apply(x.reshape(-1, x.shape[-1]), weight, target.reshape(-1).contiguous(),
-                                     int(ignore_index), reduction)
-    return loss.view(target.shape) if reduction == "none" else loss
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    y = target if target.dim() == 1 else target.reshape(-1)
+    if not y.is_contiguous():
+        y = y.contiguous()
+    if torch.is_grad_enabled() and (x2.requires_grad or weight.requires_grad):
+        loss = _LinearCrossEntropy.apply(x2, weight, y, int(ignore_index), reduction)
+    else:
+        loss = _ce_forward(x2, weight, y, int(ignore_index), reduction)[0]
+    return loss.view(target.shape) if reduction == "none" and target.dim() != 1 else loss
 
 
 # ---------------------------------------------------------------- 4-bit weights
