@@ -175,6 +175,38 @@ def test_abi_refusals():
     assert lib.tilec_mm_w4_workspace_bytes(None, 9, 2, 64, 2, 8, 64, 32, None, 8) == 0
 
 
+def test_weight_fields_are_checked_and_read_only():
+    """The kernels read data in place by shape, group_size and scale_dtype."""
+    w = ext.pack_w4(torch.zeros(20, 300, dtype=torch.uint8), torch.ones(20, 5, dtype=torch.bfloat16), group_size=64)
+    again = ext.W4Weight(w.shape, w.group_size, w.scale_dtype, w.data)
+    assert torch.equal(again.unpack(), w.unpack()) and again.shape == (20, 300)
+    for bad in (dict(shape=(33, 300)), dict(shape=(20, 400)), dict(shape=(-1, 300)), dict(shape=(20, 0)),
+                dict(group_size=32), dict(group_size=48), dict(scale_dtype=torch.float32), dict(data=w.data[:1]),
+                dict(data=w.data.transpose(0, 1).contiguous().transpose(0, 1)),
+                dict(data=torch.zeros(w.data.numel() + 1, dtype=torch.uint8)[1:].view(w.data.shape))):
+        with pytest.raises(ValueError, match="W4Weight"):
+            ext.W4Weight(**{**dict(shape=w.shape, group_size=64, scale_dtype=w.scale_dtype, data=w.data), **bad})
+    for bad in (dict(scale_dtype=torch.float64), dict(data=w.data.view(torch.int8))):
+        with pytest.raises(TypeError, match="W4Weight"):
+            ext.W4Weight(**{**dict(shape=w.shape, group_size=64, scale_dtype=w.scale_dtype, data=w.data), **bad})
+    for name in ("shape", "group_size", "scale_dtype", "data"):
+        with pytest.raises(AttributeError):
+            setattr(w, name, getattr(w, name))
+    assert ext.pack_w4(torch.zeros(0, 5, dtype=torch.uint8), torch.ones(0, 1)).shape == (0, 5)
+
+
+def test_quantize_extremes():
+    top = 0.9 * torch.finfo(torch.float32).max   # high - low is past the type's range, 8 steps are not
+    w = torch.tensor([[top, -top, 0.0, top / 2], [0.0, 0.0, 0.0, 0.0], [1e-45, 0.0, 0.0, 0.0]])
+    q = ext.quantize_w4(w, 32)
+    step = top / 7.5
+    assert torch.isfinite(q.scales()).all() and ((q.dequantize()[0].double() - w[0].double()).abs() <= step * 1.001).all()
+    assert (q.dequantize()[1] == 0).all() and (q.dequantize()[2] <= 1e-44).all()
+    for bad in (float("inf"), float("-inf"), float("nan")):
+        with pytest.raises(ValueError, match="infinities"):
+            ext.quantize_w4(torch.tensor([[1.0, bad]]))
+
+
 # ---------------------------------------------------------------- GPU
 gpu = pytest.mark.gpu
 
@@ -421,3 +453,19 @@ def test_gave_up_is_nan_or_right_and_the_context_works(m, dtype, monkeypatch):
     assert (err[~nan] <= _bound(x.cpu(), w64.cpu(), good.cpu().double(), dtype, m).cuda()[~nan] * 2).all()
     assert torch.equal(ext.matrix_mul_w4(x, w), good)
     ext.check_device()
+
+
+@gpu
+def test_workspace_follows_each_operand_alignment():
+    """x 240 bytes into its storage, out on a 16-byte boundary or off it: each call's workspace
+    is sized for its own operands."""
+    x, codes, scales, zeros, _ = _make(300, 64, 256, 128, "bf16")
+    weight = ext.pack_w4(codes, scales, zeros).to("cuda")
+    xs = torch.zeros(300 * 256 + 120, dtype=torch.bfloat16, device="cuda")[120:].view(300, 256).copy_(x)
+    room = torch.empty(300 * 64 + 8, dtype=torch.bfloat16, device="cuda")
+    ref = ext.matrix_mul_w4(xs, weight)
+    for at in (0, 1, 3, 8):
+        out = room[at:at + 300 * 64].view(300, 64)
+        assert torch.equal(ext.matrix_mul_w4(xs, weight, out=out), ref)
+    with pytest.raises(ValueError, match="requires a gradient"):
+        ext.matrix_mul_w4(xs, weight, out=room[:300 * 64].view(300, 64).requires_grad_())

@@ -5,8 +5,7 @@
 namespace tilec {
 namespace {
 
-constexpr int64_t kW4MmaSlabBytes = 32768; // w4_mma_kernel: x in shared memory at a time
-constexpr int64_t kW4MaxSmem = 232448;    // shared memory a CTA may have, and an SM's for all of them
+constexpr int64_t kW4MaxSmem = 232448;    // shared memory a CTA may have
 
 // ---------------------------------------------------------------- 16-bit products
 struct LmInfo {
@@ -44,9 +43,9 @@ int lm_device(DeviceInfo** d, LmInfo** lm) {
       constexpr bool W = decltype(wide)::value;
       auto stream = [&](auto sc) {
         constexpr int C = decltype(sc)::value;
-        w4_attr(w4_stream_kernel<1, G, C>);
-        w4_attr(w4_stream_kernel<2, G, C>);
-        w4_attr(w4_stream_kernel<4, G, C>);
+        w4_attr(w4_stream_kernel<1, G, C, 0>);
+        w4_attr(w4_stream_kernel<2, G, C, 0>);
+        w4_attr(w4_stream_kernel<4, G, C, 0>);
       };
       if constexpr (W) {
         stream(std::integral_constant<int, TILEC_DTYPE_F32>{});
@@ -54,8 +53,10 @@ int lm_device(DeviceInfo** d, LmInfo** lm) {
         stream(std::integral_constant<int, TILEC_DTYPE_F16>{});
         stream(std::integral_constant<int, TILEC_DTYPE_BF16>{});
       }
-      w4_attr(w4_mma_kernel<true, 1, 1, G, W>);
-      w4_attr(w4_mma_kernel<false, 1, 1, G, W>);
+      w4_attr(w4_stream_kernel<1, G, W ? 0 : 1, TILEC_DTYPE_F16>);
+      w4_attr(w4_stream_kernel<1, G, W ? 0 : 1, TILEC_DTYPE_BF16>);
+      w4_attr(w4_stream_kernel<2, G, W ? 0 : 1, TILEC_DTYPE_F16>);
+      w4_attr(w4_stream_kernel<2, G, W ? 0 : 1, TILEC_DTYPE_BF16>);
     };
     auto w4_all = [&](auto gpb) {
       constexpr int G = decltype(gpb)::value;
@@ -572,24 +573,25 @@ struct W4Call {
   int64_t ldo;
 };
 
-template <int NT>
+template <int NT, int XT>
 int64_t w4_stream_fixed_nt(int gpb, bool wide) {
-  return gpb == 4   ? (wide ? W4StreamCfg<NT, 4, true>::kFixed : W4StreamCfg<NT, 4, false>::kFixed)
-         : gpb == 2 ? (wide ? W4StreamCfg<NT, 2, true>::kFixed : W4StreamCfg<NT, 2, false>::kFixed)
-                    : (wide ? W4StreamCfg<NT, 1, true>::kFixed : W4StreamCfg<NT, 1, false>::kFixed);
+  return gpb == 4   ? (wide ? W4StreamCfg<NT, 4, true, XT>::kFixed : W4StreamCfg<NT, 4, false, XT>::kFixed)
+         : gpb == 2 ? (wide ? W4StreamCfg<NT, 2, true, XT>::kFixed : W4StreamCfg<NT, 2, false, XT>::kFixed)
+                    : (wide ? W4StreamCfg<NT, 1, true, XT>::kFixed : W4StreamCfg<NT, 1, false, XT>::kFixed);
 }
-int64_t w4_stream_fixed(int nt, int gpb, bool wide) {
-  return nt == 1   ? w4_stream_fixed_nt<1>(gpb, wide)
-         : nt == 2 ? w4_stream_fixed_nt<2>(gpb, wide)
-                   : w4_stream_fixed_nt<4>(gpb, wide);
+int64_t w4_stream_fixed(int nt, int gpb, bool wide, bool x16) {
+  if (x16) return nt == 1 ? w4_stream_fixed_nt<1, 1>(gpb, wide) : w4_stream_fixed_nt<2, 1>(gpb, wide);
+  return nt == 1   ? w4_stream_fixed_nt<1, 0>(gpb, wide)
+         : nt == 2 ? w4_stream_fixed_nt<2, 0>(gpb, wide)
+                   : w4_stream_fixed_nt<4, 0>(gpb, wide);
 }
 
 struct W4Plan {
   bool stream = false;   // w4_stream_kernel
-  bool mma = false;      // w4_mma_kernel
+  bool x16 = false;      // ... with x in 16-bit values, not digits
   bool tc = false;       // w4_tc_kernel; otherwise expanded weights and a plain product
   bool pack_x = false;   // x is copied to aligned rows first (expanded weights)
-  int nt = 1, mt = 1, splits = 1, row_warps = 1, slab = 1, per_cta = 0, ctas = 0;
+  int nt = 1, splits = 1, slab = 1, per_cta = 0, ctas = 0;
   bool cut_before = false;
   size_t off_digits = 0, off_sums = 0, off_scale = 0;
   int64_t blocks = 0, kp = 0, piece = 0;
@@ -624,22 +626,23 @@ int check_w4_pointers(const W4Call& c) {
 // whose type the scales share on w4_tc_kernel, 128 at a time (8192 x 8192: 128 rows 35 us, twice
 // that for 256; expanded first, either takes 89); for the rest W is expanded once into the
 // workspace and multiplied on the tcgen05 kernels (fp32: 3xTF32).
-constexpr int64_t kW4MaxCols = 32;
+constexpr int64_t kW4MaxCols = 32;  // of digits
+constexpr int64_t kW4Max16 = 16;    // rows of 16-bit x
 
 void plan_w4(const W4Call& c, const DeviceInfo& d, const LmInfo& lm, W4Plan* p) {
   const bool f32 = c.dtype == TILEC_DTYPE_F32;
   p->blocks = cdiv(c.K, kW4Block);
   p->kp = p->blocks * kW4Block;
-  const int digits = kW4Digits;
   size_t at = 0;
   auto take = [&](size_t bytes) {
     const size_t o = at;
     at = align256(at + bytes);
     return o;
   };
-  if (c.M * digits <= (f32 ? kW4MaxCols : 8)) {
+  if (c.M * kW4Digits <= (f32 ? kW4MaxCols : 8) || (!f32 && c.M <= kW4Max16)) {
     p->stream = true;
-    const int cols = static_cast<int>(c.M * digits);
+    p->x16 = c.M * kW4Digits > (f32 ? kW4MaxCols : 8);
+    const int cols = static_cast<int>(p->x16 ? c.M : c.M * kW4Digits);
     p->nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
     const int gpb = c.group == 32 ? 4 : c.group == 64 ? 2 : 1;
     const int pad = 8 * p->nt;
@@ -655,18 +658,19 @@ void plan_w4(const W4Call& c, const DeviceInfo& d, const LmInfo& lm, W4Plan* p) 
     p->ctas = static_cast<int>((tiles < clusters ? tiles : clusters) * p->splits);
     // Two rows are cut in every CTA (a round of some 150 instructions per row and 48 blocks),
     // more once for all.
-    p->cut_before = c.M > 2;
+    p->cut_before = !p->x16 && c.M > 2;
     const bool wide = c.sdt == TILEC_DTYPE_F32;
-    const int64_t room = kW4MaxSmem - w4_stream_fixed(p->nt, gpb, wide);
+    const int64_t room = kW4MaxSmem - w4_stream_fixed(p->nt, gpb, wide, p->x16);
+    auto slab_bytes = [&](int64_t n) { return p->x16 ? w4_slab16_bytes(n, c.M) : w4_slab_bytes(n, cols, pad, gpb); };
     int64_t slab = p->per_cta;
-    while (slab > 1 && w4_slab_bytes(slab, cols, pad, gpb) > room) --slab;
-    p->slab = static_cast<int>(slab);
+    while (slab > 1 && slab_bytes(slab) > room) --slab;
+    p->slab = static_cast<int>(cdiv(p->per_cta, cdiv(p->per_cta, slab)));  // slabs of one size
     if (p->cut_before) {
       p->off_digits = take(size_t(cols) * p->blocks * kW4Block);
       p->off_sums = take(size_t(p->blocks) * gpb * pad * 4);
       p->off_scale = take(size_t(p->blocks) * pad * 4);
     }
-  } else if (!f32 && c.M > 8 && c.M <= 2 * W4TcCfg<1>::kMaxCols && c.sdt == c.dtype) {
+  } else if (!f32 && c.M <= 2 * W4TcCfg<1>::kMaxCols && c.sdt == c.dtype) {
     p->tc = true;
     p->pack_x = !rows_aligned16(c.x, c.ldx);
     if (p->pack_x) p->off_x = take(size_t(c.M) * p->kp * 2);
@@ -687,18 +691,6 @@ void plan_w4(const W4Call& c, const DeviceInfo& d, const LmInfo& lm, W4Plan* p) 
     if (p->splits > 1)
       p->off_slabs =
           take(size_t(p->splits) * (c.M < W4TcCfg<1>::kMaxCols ? c.M : W4TcCfg<1>::kMaxCols) * p->ldslab * 4);
-  } else if (!f32 && c.M <= 8) {
-    p->mma = true;
-    p->nt = 1;
-    p->mt = 1;
-    p->row_warps = 8;
-    const int64_t tiles = cdiv(c.N, 16 * p->mt * p->row_warps), slots = int64_t(d.sms) * (p->mt == 1 ? 3 : 2);
-    while (p->splits < 8 && tiles * p->splits * 2 <= slots && p->blocks >= 4 * p->splits) p->splits *= 2;
-    const int64_t per_cta = cdiv(p->blocks, p->splits);
-    int64_t slab = kW4MmaSlabBytes / (c.M * kW4Block * 2);
-    if (slab < 1) slab = 1;
-    if (slab > per_cta) slab = per_cta;
-    p->slab = static_cast<int>(slab);
   } else {
     int64_t piece = kW4ExpandBytes / (p->kp * (f32 ? 4 : 2)) / 256 * 256;
     if (piece < 256) piece = 256;
@@ -725,21 +717,7 @@ void plan_w4(const W4Call& c, const DeviceInfo& d, const LmInfo& lm, W4Plan* p) 
   p->bytes = at;
 }
 
-int w4_per_sm(size_t smem, int most) {
-  const int64_t n = kW4MaxSmem / (int64_t(smem) + 1024);  // 1 KB of each CTA's goes to the system
-  return static_cast<int>(n < 1 ? 1 : n > most ? most : n);
-}
-
-template <typename Kernel>
-int launch_w4_grid(Kernel kern, W4Args a, int rows, size_t smem, int most, int sms, cudaStream_t s) {
-  if (int64_t(smem) > kW4MaxSmem) return TILEC_ERR_UNSUPPORTED;
-  a.tiles = static_cast<int>(cdiv(a.N, rows));
-  int64_t clusters = int64_t(sms) * w4_per_sm(smem, most) / a.splits;
-  if (clusters > a.tiles) clusters = a.tiles;
-  return launch_k(kern, dim3(static_cast<unsigned>(clusters * a.splits)), dim3(32 * kW4Warps), smem, s, a.splits, a);
-}
-
-template <int NT, int GPB, int SC>
+template <int NT, int GPB, int SC, int XT>
 int launch_w4_stream(const W4Args& w, const W4Plan& p, uint8_t* ws, cudaStream_t s) {
   W4StreamArgs a;
   a.w = w;
@@ -752,50 +730,45 @@ int launch_w4_stream(const W4Args& w, const W4Plan& p, uint8_t* ws, cudaStream_t
   a.row_tiles = static_cast<int>(cdiv(w.N, 16));
   a.per_cta = p.per_cta;
   a.slab = p.slab;
-  using Cfg = W4StreamCfg<NT, GPB, SC == 0>;
-  const size_t smem = size_t(Cfg::kFixed + w4_slab_bytes(p.slab, w.cols, 8 * NT, GPB));
+  using Cfg = W4StreamCfg<NT, GPB, SC == 0, XT>;
+  const size_t smem = size_t(Cfg::kFixed + (XT != 0 ? w4_slab16_bytes(p.slab, w.M) : w4_slab_bytes(p.slab, w.cols, 8 * NT, GPB)));
   if (int64_t(smem) > kW4MaxSmem) return TILEC_ERR_UNSUPPORTED;
   if (p.cut_before)
     TILEC_TRY(launch_k(w4_digits_kernel, dim3(static_cast<unsigned>(cdiv(int64_t(w.M) * p.blocks, 8))), dim3(128), 0, s,
                        1, w, a.d, static_cast<int>(p.blocks)));
-  return launch_k(w4_stream_kernel<NT, GPB, SC>, dim3(static_cast<unsigned>(p.ctas)), dim3(Cfg::kThreads), smem, s,
+  return launch_k(w4_stream_kernel<NT, GPB, SC, XT>, dim3(static_cast<unsigned>(p.ctas)), dim3(Cfg::kThreads), smem, s,
                   w.splits, a);
 }
 
-template <bool BF16, int NT, int MT, int GPB, bool WIDE>
-int launch_w4_mma(const W4Args& a, int sms, cudaStream_t s) {
-  using Cfg = W4Cfg<MT, GPB, WIDE>;
-  const size_t smem = size_t(Cfg::kRingBytes) + size_t(kW4Warps) * 16 * MT * 8 * NT * 4 +
-                      size_t(a.cols) * (a.slab * kW4Block + 32) * 2;
-  static_assert(Cfg::kRingBytes + kW4Warps * 16 * MT * 8 * NT * 4 + kW4MmaSlabBytes + 8 * NT * 64 <= kW4MaxSmem,
-                "shared memory");
-  return launch_w4_grid(w4_mma_kernel<BF16, NT, MT, GPB, WIDE>, a, 16 * MT * a.row_warps, smem, Cfg::kPerSm, sms, s);
-}
-
-// The kernels' variants: by columns, groups per block, type of x and scales.
+// The kernel's variants: by columns, groups per block, type of x and scales.
 template <int GPB, bool WIDE>
-int launch_w4(const W4Args& a, const W4Plan& p, bool bf16, int sms, uint8_t* ws, cudaStream_t s) {
-  if (p.stream) {
-    auto by_columns = [&](auto sc) {
-      constexpr int SC = decltype(sc)::value;
-      return p.nt == 1   ? launch_w4_stream<1, GPB, SC>(a, p, ws, s)
-             : p.nt == 2 ? launch_w4_stream<2, GPB, SC>(a, p, ws, s)
-                         : launch_w4_stream<4, GPB, SC>(a, p, ws, s);
+int launch_w4(const W4Args& a, const W4Plan& p, uint8_t* ws, cudaStream_t s) {
+  if (p.x16) {
+    auto by_type = [&](auto nt) {
+      constexpr int NT = decltype(nt)::value;
+      return a.dtype == TILEC_DTYPE_BF16 ? launch_w4_stream<NT, GPB, WIDE ? 0 : 1, TILEC_DTYPE_BF16>(a, p, ws, s)
+                                         : launch_w4_stream<NT, GPB, WIDE ? 0 : 1, TILEC_DTYPE_F16>(a, p, ws, s);
     };
-    if constexpr (WIDE)
-      return by_columns(std::integral_constant<int, TILEC_DTYPE_F32>{});
-    else
-      return a.scale_bf16 ? by_columns(std::integral_constant<int, TILEC_DTYPE_BF16>{})
-                          : by_columns(std::integral_constant<int, TILEC_DTYPE_F16>{});
+    return p.nt == 1 ? by_type(std::integral_constant<int, 1>{}) : by_type(std::integral_constant<int, 2>{});
   }
-  return bf16 ? launch_w4_mma<true, 1, 1, GPB, WIDE>(a, sms, s) : launch_w4_mma<false, 1, 1, GPB, WIDE>(a, sms, s);
+  auto by_columns = [&](auto sc) {
+    constexpr int SC = decltype(sc)::value;
+    return p.nt == 1   ? launch_w4_stream<1, GPB, SC, 0>(a, p, ws, s)
+           : p.nt == 2 ? launch_w4_stream<2, GPB, SC, 0>(a, p, ws, s)
+                       : launch_w4_stream<4, GPB, SC, 0>(a, p, ws, s);
+  };
+  if constexpr (WIDE)
+    return by_columns(std::integral_constant<int, TILEC_DTYPE_F32>{});
+  else
+    return a.scale_bf16 ? by_columns(std::integral_constant<int, TILEC_DTYPE_BF16>{})
+                        : by_columns(std::integral_constant<int, TILEC_DTYPE_F16>{});
 }
 
 template <bool WIDE>
-int launch_w4(const W4Args& a, const W4Plan& p, int gpb, bool bf16, int sms, uint8_t* ws, cudaStream_t s) {
-  return gpb == 4   ? launch_w4<4, WIDE>(a, p, bf16, sms, ws, s)
-         : gpb == 2 ? launch_w4<2, WIDE>(a, p, bf16, sms, ws, s)
-                    : launch_w4<1, WIDE>(a, p, bf16, sms, ws, s);
+int launch_w4(const W4Args& a, const W4Plan& p, int gpb, uint8_t* ws, cudaStream_t s) {
+  return gpb == 4   ? launch_w4<4, WIDE>(a, p, ws, s)
+         : gpb == 2 ? launch_w4<2, WIDE>(a, p, ws, s)
+                    : launch_w4<1, WIDE>(a, p, ws, s);
 }
 
 template <bool BF16, int GPB>
@@ -868,22 +841,19 @@ int run_w4(const W4Call& c, void* workspace, size_t ws_bytes, cudaStream_t s) {
   a.K = static_cast<int>(c.K);
   a.blocks = static_cast<int>(p.blocks);
   const int gpb = c.group == 32 ? 4 : c.group == 64 ? 2 : 1;
-  if (p.stream || p.mma || p.tc) {
+  if (p.stream || p.tc) {
     a.x = c.x;
     a.ldx = c.ldx;
     a.dtype = c.dtype;
     a.M = static_cast<int>(c.M);
-    a.cols = static_cast<int>(c.M * (p.stream ? kW4Digits : 1));
+    a.cols = static_cast<int>(c.M * (p.stream && !p.x16 ? kW4Digits : 1));
     a.vec_x = !f32 && rows_aligned16(c.x, c.ldx);
     a.out = c.out;
     a.ldo = c.ldo;
     a.bias = c.bias;
     a.splits = p.splits;
-    a.row_warps = p.row_warps;
-    a.slab = p.slab;
-    const bool bf16 = c.dtype == TILEC_DTYPE_BF16;
     if (p.tc) return run_w4_tc(c, p, a, gpb, ws, *d, s);
-    return a.wide ? launch_w4<true>(a, p, gpb, bf16, d->sms, ws, s) : launch_w4<false>(a, p, gpb, bf16, d->sms, ws, s);
+    return a.wide ? launch_w4<true>(a, p, gpb, ws, s) : launch_w4<false>(a, p, gpb, ws, s);
   }
   const void* x = c.x;
   int64_t ldx = c.ldx;

@@ -60,17 +60,18 @@ struct W4StreamArgs {
   int slab;          // blocks of x in shared memory at a time
 };
 
-template <int NT, int GPB, bool WIDE>
+// XT: how x enters: 0 in digits, else as 16-bit values of that TILEC_DTYPE_*.
+template <int NT, int GPB, bool WIDE, int XT>
 struct W4StreamCfg {
   static constexpr int kThreads = 32 * kW4StreamWarps;
   static constexpr int kPiece = w4_piece_bytes(GPB, WIDE);
   // Pieces a copy.  An SM's bulk copies start some 60 ns apart, so few large ones keep up with
   // HBM; with more columns x needs the room.
-  static constexpr int kRun = NT == 1 && kPiece <= 1152 ? 4 : 2;
+  static constexpr int kRun = XT == 0 && NT == 1 && kPiece <= 1152 ? 4 : 2;
   static constexpr int kStage = kRun * kPiece;
   static constexpr int kStages = 2;
   static constexpr int kRingBytes = kW4StreamWarps * kStages * kStage;
-  static constexpr int kPart = 2 * NT * 16;  // floats: the sums of a row tile, [row of x][16]
+  static constexpr int kPart = (XT == 0 ? 2 : 8) * NT * 16;  // floats: the sums of a row tile, [row of x][16]
   static constexpr int kSumBytes = kW4GroupTiles * kPart * 4;
   static constexpr int kPartBytes = 2 * kW4StreamWarps * kPart * 4;
   static constexpr int kBarBytes = 1024;     // a barrier per warp and stage, the abort flag
@@ -80,6 +81,10 @@ struct W4StreamCfg {
 // Bytes of `slab` blocks of x: digits (16 bytes more a column: conflict-free reads), sums, scales.
 __host__ __device__ inline int64_t w4_slab_bytes(int64_t slab, int cols, int cols_pad, int gpb) {
   return cols * (slab * kW4Block + 16) + slab * cols_pad * 4 * (gpb + 1);
+}
+// The same in 16-bit values (64 bytes more a row: conflict-free reads).
+__host__ __device__ inline int64_t w4_slab16_bytes(int64_t slab, int64_t rows) {
+  return rows * (slab * (2 * kW4Block) + 64);
 }
 
 // Sixteen lanes (l = 0 .. 15) cut one 128-k block of one row of x; all lanes of a warp call.
@@ -220,12 +225,33 @@ __device__ __forceinline__ void lds_words(uint32_t (&w)[WORDS], uint32_t a) {
   }
 }
 
-// SC: type of the scales (TILEC_DTYPE_*).
+// 16-bit rows of x, blocks s0 .. s0 + n, to shared memory: [row][pitch], zeros past K.
+__device__ __forceinline__ void w4_stage16(const W4Args& p, uint8_t* xs, int pitch, int s0, int n) {
+  const int per_row = n * (kW4Block / 8);
+  for (int i = threadIdx.x; i < p.M * per_row; i += 32 * kW4StreamWarps) {
+    const int m = i / per_row, c = i - m * per_row, k = s0 * kW4Block + 8 * c;
+    const unsigned short* s = static_cast<const unsigned short*>(p.x) + m * p.ldx + k;
+    uint8_t* dst = xs + m * pitch + 16 * c;
+    if (p.vec_x && k + 8 <= p.K) {
+      cp_async_16(dst, s, 16);
+    } else {
+      uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (k + j < p.K) w[j >> 1] |= uint32_t(s[j]) << (16 * (j & 1));
+      *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+  cp_async_commit();
+  cp_async_wait<0>();
+}
+
+// SC: type of the scales (TILEC_DTYPE_*); with 16-bit x (XT != 0) 0, or 1 for either 16-bit type.
 // Grid: x = CTAs (clusters of `splits`, whose CTAs share their row tiles and split K).
-template <int NT, int GPB, int SC>
+template <int NT, int GPB, int SC, int XT>
 __global__ void __launch_bounds__(32 * kW4StreamWarps, 1) w4_stream_kernel(const __grid_constant__ W4StreamArgs a) {
   constexpr bool WIDE = SC == 0;
-  using Cfg = W4StreamCfg<NT, GPB, WIDE>;
+  using Cfg = W4StreamCfg<NT, GPB, WIDE, XT>;
   constexpr int COLS = 8 * NT, WB = w4_word_bytes(GPB, WIDE), T = Cfg::kThreads, S = Cfg::kStages, W = kW4StreamWarps;
   extern __shared__ __align__(128) uint8_t w4_smem[];
   const W4Args& p = a.w;
@@ -235,7 +261,7 @@ __global__ void __launch_bounds__(32 * kW4StreamWarps, 1) w4_stream_kernel(const
   float* parts = reinterpret_cast<float*>(w4_smem + Cfg::kRingBytes + Cfg::kSumBytes);     // [warp][first, last][kPart]
   uint64_t* bars = reinterpret_cast<uint64_t*>(w4_smem + Cfg::kFixed - Cfg::kBarBytes) + warp * S;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(w4_smem + Cfg::kFixed - 8);
-  const int pitch = a.slab * kW4Block + 16;
+  const int pitch = XT == 0 ? a.slab * kW4Block + 16 : a.slab * (2 * kW4Block) + 64;
   W4Digits d = a.d;                                // the slab in shared memory
   d.digits = w4_smem + Cfg::kFixed;
   d.pitch = pitch;
@@ -261,10 +287,64 @@ __global__ void __launch_bounds__(32 * kW4StreamWarps, 1) w4_stream_kernel(const
   const uint32_t ring_at = smem_u32(ring), lane_codes = 16 * WB + lane * 16, lane_words = g * WB;
   uint32_t x_col[NT];
 #pragma unroll
-  for (int i = 0; i < NT; ++i) x_col[i] = smem_u32(d.digits) + min(8 * i + g, p.cols - 1) * pitch + 32 * t;
+  for (int i = 0; i < NT; ++i)
+    x_col[i] = smem_u32(d.digits) + min(8 * i + g, p.cols - 1) * pitch + (XT == 0 ? 32 : 16) * t;
+  uint32_t magic = 0;  // in a register: the logic instruction takes one immediate
+  if constexpr (XT != 0) asm volatile("mov.b32 %0, %1;" : "=r"(magic) : "n"(XT == 2 ? 0x43004300u : 0x64006400u));
   const uint32_t sums_at = smem_u32(d.sums) + 8 * t, scale_at = smem_u32(d.scale) + 8 * t;
 
-  auto multiply = [&](uint32_t piece, int blk) {  // `blk`: the piece's block within the slab
+  auto multiply16 = [&](uint32_t piece, int blk) {
+    const uint4 qa = lds128(piece + lane_codes), qb = lds128(piece + lane_codes + 512);
+    uint32_t wa[WB / 4], wb[WB / 4];
+    lds_words(wa, piece + lane_words);
+    lds_words(wb, piece + lane_words + 8 * WB);
+    float acc[NT][4], sa = 0.f, sb = 0.f;
+    uint32_t za = 0, zb = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      constexpr int kSteps = 4 / GPB;  // words of codes per group
+      if (j % kSteps == 0) {
+        const int k = j / kSteps;
+        const uint32_t ga = wa[WIDE ? 2 * k : k], gb = wb[WIDE ? 2 * k : k];
+        if constexpr (WIDE) {
+          sa = __uint_as_float(wa[2 * k + 1]);
+          sb = __uint_as_float(wb[2 * k + 1]);
+        } else {
+          sa = w4_scale16(ga, p.scale_bf16);
+          sb = w4_scale16(gb, p.scale_bf16);
+        }
+        za = magic | __byte_perm(ga, 0, 0x1010);
+        zb = magic | __byte_perm(gb, 0, 0x1010);
+      }
+      const uint32_t ca = j == 0 ? qa.x : j == 1 ? qa.y : j == 2 ? qa.z : qa.w;
+      const uint32_t cb = j == 0 ? qb.x : j == 1 ? qb.y : j == 2 ? qb.z : qb.w;
+      uint32_t u[4], v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        u[i] = w4_pair<XT == 2>(ca, i, magic, za);
+        v[i] = w4_pair<XT == 2>(cb, i, magic, zb);
+      }
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        const uint4 xv = lds128(x_col[i] + blk * (2 * kW4Block) + 64 * j);
+        if (j % kSteps == 0)
+          mma_16816_zero<XT == 2>(acc[i], u[0], v[0], u[1], v[1], xv.x, xv.y);
+        else
+          mma_16816<XT == 2>(acc[i], u[0], v[0], u[1], v[1], xv.x, xv.y);
+        mma_16816<XT == 2>(acc[i], u[2], v[2], u[3], v[3], xv.z, xv.w);
+      }
+      if ((j + 1) % kSteps == 0) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          total[i][0] = fmaf(acc[i][0], sa, total[i][0]);
+          total[i][1] = fmaf(acc[i][1], sa, total[i][1]);
+          total[i][2] = fmaf(acc[i][2], sb, total[i][2]);
+          total[i][3] = fmaf(acc[i][3], sb, total[i][3]);
+        }
+      }
+    }
+  };
+  auto multiply8 = [&](uint32_t piece, int blk) {
     const uint4 qa = lds128(piece + lane_codes), qb = lds128(piece + lane_codes + 512);
     uint32_t wa[WB / 4], wb[WB / 4];
     lds_words(wa, piece + lane_words);
@@ -328,6 +408,11 @@ __global__ void __launch_bounds__(32 * kW4StreamWarps, 1) w4_stream_kernel(const
     }
   };
 
+  auto multiply = [&](uint32_t piece, int blk) {  // `blk`: the piece's block within the slab
+    if constexpr (XT == 0) multiply8(piece, blk);
+    else multiply16(piece, blk);
+  };
+
   int stage = 0;
   uint32_t phase = 0;
   bool ok = true, waited = false;
@@ -369,7 +454,9 @@ __global__ void __launch_bounds__(32 * kW4StreamWarps, 1) w4_stream_kernel(const
         waited = true;
       }
       if (!whole_x || (group == tile_begin && s0 == b_begin)) {
-        if (cut_here) {
+        if constexpr (XT != 0) {
+          w4_stage16(p, d.digits, pitch, s0, n);
+        } else if (cut_here) {
           for (int base = 0; base < p.M * n; base += T / 16) {
             const int task = base + (threadIdx.x >> 4);
             const bool live = task < p.M * n;
@@ -398,6 +485,16 @@ __global__ void __launch_bounds__(32 * kW4StreamWarps, 1) w4_stream_kernel(const
         float* dst = whole ? tile_sums + tile * Cfg::kPart : parts + (2 * warp + which) * Cfg::kPart;
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
+          if constexpr (XT != 0) {
+            float* r = dst + (8 * i + 2 * t) * 16 + g;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              float* at = r + (j & 1) * 16 + (j >> 1) * 8;
+              *at = whole ? *at + total[i][j] : total[i][j];
+              total[i][j] = 0.f;
+            }
+            continue;
+          }
           // Digits of one row of x: two columns here, two in the neighbouring lane.
           float v0 = total[i][0] + total[i][1], v1 = total[i][2] + total[i][3];
           v0 += __shfl_xor_sync(0xffffffffu, v0, 1);
@@ -482,7 +579,9 @@ __global__ void __launch_bounds__(32 * kW4StreamWarps, 1) w4_stream_kernel(const
           v += u;
         }
       }
-      if (v != v) v = w4_output(p, GPB, row, m);
+      if constexpr (XT == 0) {
+        if (v != v) v = w4_output(p, GPB, row, m);
+      }
       if (p.bias != nullptr) v += load_as_float(p.bias, row, p.dtype);
       store_from_float(p.out, int64_t(m) * p.ldo + row, p.dtype, v);
     }

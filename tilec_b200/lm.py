@@ -161,6 +161,11 @@ def linear_cross_entropy(x, weight, target, ignore_index=-100, reduction="mean")
     A token whose target is ignore_index has loss 0 and gradient 0 whatever its row holds; a
     16-bit call does no products for it.  Any other target outside [0, V) makes the token's
     loss and the gradients NaN and sets a device status bit (ext.check_device raises it).
+
+    Forward and backward can be captured into a CUDA graph.  As with any torch operator, drop
+    the losses of eager calls on the same leaves before capturing a backward() (or capture
+    torch.autograd.grad): torch adds to a leaf's .grad on the stream of the oldest live graph
+    that uses it, which is not the captured one.
     """
     if reduction not in _REDUCTIONS:
         raise ValueError(f"linear_cross_entropy: unknown reduction {reduction!r}; expected 'mean', 'sum' or 'none'")
@@ -205,14 +210,30 @@ class W4Weight:
 
     shape (N, K); group_size; scale_dtype; data uint8 [row tiles of 16, blocks of 128 k, bytes]:
     each piece's group words, then its codes (tilec_mm_w4 in include/tilec_mm.h).
-    matrix_mul_w4 reads it in place."""
+    matrix_mul_w4 reads it in place, so the four are checked against each other here and are
+    read-only."""
 
     def __init__(self, shape, group_size, scale_dtype, data):
-        self.shape, self.group_size, self.scale_dtype, self.data = tuple(shape), group_size, scale_dtype, data
+        n, k = (int(i) for i in shape)
+        _check_group(group_size, "W4Weight")
+        if n < 0 or k < 1:
+            raise ValueError(f"W4Weight: shape must be (N, K) with K >= 1, got {(n, k)}")
+        if scale_dtype not in _DTYPES:
+            raise TypeError(f"W4Weight: scales must be float32, float16 or bfloat16, got {scale_dtype}")
+        if data.dtype != torch.uint8:
+            raise TypeError(f"W4Weight: data must be uint8, got {data.dtype}")
+        words = 16 * max(1, _BLOCK // group_size) * (8 if scale_dtype == torch.float32 else 4)
+        want = (-(-n // 16), -(-k // _BLOCK), words + 1024)
+        if tuple(data.shape) != want or not data.is_contiguous() or data.data_ptr() % 16:
+            raise ValueError(f"W4Weight: data must be contiguous, 16-byte aligned and of shape {want}, "
+                             f"got shape {tuple(data.shape)}")
+        self._shape, self._group_size, self._scale_dtype, self._data = (n, k), group_size, scale_dtype, data
 
-    @property
-    def device(self):
-        return self.data.device
+    shape = property(lambda self: self._shape)
+    group_size = property(lambda self: self._group_size)
+    scale_dtype = property(lambda self: self._scale_dtype)
+    data = property(lambda self: self._data)
+    device = property(lambda self: self._data.device)
 
     def to(self, device):
         return W4Weight(self.shape, self.group_size, self.scale_dtype, self.data.to(device))
@@ -311,13 +332,17 @@ def quantize_w4(weight, group_size=128, symmetric=False):
     symmetric: steps of max|w| / 7 around zero (zero point 8).  Otherwise 15 steps over the
     group's range, widened to hold zero, which stays exact.  Scales have weight's dtype
     (float32, float16 or bfloat16); codes are chosen for the rounded scale, so an error is at
-    most half a step plus what the scale's rounding cuts off the ends of the range."""
+    most half a step, plus what the scale's rounding cuts off the ends of the range and, where
+    zero lies between two steps of it, up to half a step more at one end (so a magnitude above 15/16
+    of the type's largest may become infinite).  A weight with infinities or NaN is refused."""
     _check_group(group_size, "quantize_w4")
     if weight.dim() != 2 or weight.shape[1] == 0:
         raise ValueError(f"quantize_w4: weight must be [N, K] with K >= 1, got shape {tuple(weight.shape)}")
     if weight.dtype not in _DTYPES:
         raise TypeError(f"quantize_w4: weight must be float32, float16 or bfloat16, got {weight.dtype}")
     weight = weight.detach()
+    if not bool(torch.isfinite(weight).all()):
+        raise ValueError("quantize_w4: weight holds infinities or NaN")
     n, k = weight.shape
     groups = -(-k // group_size)
     w = torch.nn.functional.pad(weight.float(), (0, groups * group_size - k)).view(n, groups, group_size)
@@ -325,7 +350,7 @@ def quantize_w4(weight, group_size=128, symmetric=False):
         scales = w.abs().amax(2) / 7
     else:
         low, high = w.amin(2).clamp(max=0), w.amax(2).clamp(min=0)
-        scales = (high - low) / 15
+        scales = (high / 2 - low / 2) / 7.5   # high - low itself can overflow
     scales = scales.to(weight.dtype)
     step = torch.where(scales > 0, scales.float(), 1.0)
     if symmetric:
@@ -340,7 +365,7 @@ def quantize_w4(weight, group_size=128, symmetric=False):
 def matrix_mul_w4(x, weight, bias=None, out=None):
     """x @ W.T (+ bias) with W a W4Weight of shape (N, K); x [..., K] float32, float16 or
     bfloat16 on the weight's device; bias None or [N] of x's dtype.  Returns (or writes into
-    `out`, [..., N] with unit column stride) x's dtype.
+    `out`, [..., N] with unit column stride, sharing no memory with x or bias) x's dtype.
 
     Up to 8 rows of x, the decoding case, the codes are read once and enter exactly: sums are
     fp32, with one rounding at the end.  One or two rows (float32: all 8) go through the integer
@@ -390,7 +415,7 @@ def matrix_mul_w4(x, weight, bias=None, out=None):
         stream = _stream(dev)
         px, po, sdt, group = xr.data_ptr(), out2.data_ptr(), _DTYPES[weight.scale_dtype], weight.group_size
         # The size depends on the operands' alignment only as far as their low bits tell.
-        key = (dt, m, ldx, sdt, n, k, group, ldo, (px | po << 4) & 0xFF, index)
+        key = (dt, m, ldx, sdt, n, k, group, ldo, px & 15, po & 15, index)
         nbytes = _W4_BYTES.get(key)
         if nbytes is None:
             nbytes = lib.tilec_mm_w4_workspace_bytes(px, dt, m, ldx, sdt, n, k, group, po, ldo)
@@ -415,6 +440,8 @@ _W4_BYTES = {}   # arguments that decide it -> workspace bytes of tilec_mm_w4
 def _w4_out(out, x, dev, m, n):
     """(the [m, n] view of a caller's out, its row stride)"""
     shape = x.shape[:-1] + (n,)
+    if out.requires_grad and torch.is_grad_enabled():
+        raise ValueError("matrix_mul_w4: not differentiable, but out requires a gradient")
     if out.dtype != x.dtype or out.shape != shape or out.device != dev:
         raise ValueError(f"matrix_mul_w4: out must be a {x.dtype} {tuple(shape)} tensor on {dev}")
     try:
