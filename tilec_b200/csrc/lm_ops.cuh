@@ -573,6 +573,7 @@ struct W4Call {
   int64_t ldo;
 };
 
+// Shared memory of w4_stream_kernel without x.
 template <int NT, int XT>
 int64_t w4_stream_fixed_nt(int gpb, bool wide) {
   return gpb == 4   ? (wide ? W4StreamCfg<NT, 4, true, XT>::kFixed : W4StreamCfg<NT, 4, false, XT>::kFixed)
@@ -621,11 +622,11 @@ int check_w4_pointers(const W4Call& c) {
   return TILEC_OK;
 }
 
-// How many rows of x run where: one or two (a tile of 8 columns of digits; fp32: up to 8, four
-// tiles) on w4_stream_kernel; three to 8 of 16-bit x on w4_mma_kernel; up to 256 of 16-bit x
-// whose type the scales share on w4_tc_kernel, 128 at a time (8192 x 8192: 128 rows 35 us, twice
-// that for 256; expanded first, either takes 89); for the rest W is expanded once into the
-// workspace and multiplied on the tcgen05 kernels (fp32: 3xTF32).
+// How many rows of x run where: one (fp32: up to 8) in digits on w4_stream_kernel; up to 16 of
+// 16-bit x there too, as they are, but for two against a large weight (4096 x 4096: 7.4 us, in
+// digits 9.5; 8192 x 8192: 15.6 and 19.4; 28672 x 8192: 36.7 and 33.0); up to 256 of 16-bit x whose type the scales share on w4_tc_kernel, 128 at a time (8192 x 8192: 128 rows
+// 35 us, twice that for 256; expanded first, either takes 89); for the rest W is expanded once
+// into the workspace and multiplied on the tcgen05 kernels (fp32: 3xTF32).
 constexpr int64_t kW4MaxCols = 32;  // of digits
 constexpr int64_t kW4Max16 = 16;    // rows of 16-bit x
 
@@ -639,12 +640,24 @@ void plan_w4(const W4Call& c, const DeviceInfo& d, const LmInfo& lm, W4Plan* p) 
     at = align256(at + bytes);
     return o;
   };
-  if (c.M * kW4Digits <= (f32 ? kW4MaxCols : 8) || (!f32 && c.M <= kW4Max16)) {
+  const int gpb = c.group == 32 ? 4 : c.group == 64 ? 2 : 1;
+  const bool wide = c.sdt == TILEC_DTYPE_F32, two = c.M == 2 && c.N * p->kp >= int64_t(1) << 27;
+  const bool digits = f32 ? c.M * kW4Digits <= kW4MaxCols : c.M == 1 || two;
+  // Nine to 16 rows: each further slab of x costs w4_stream_kernel some 6 us, w4_tc_kernel is the
+  // slower the larger the weight (4096 x 4096, 16 rows in two slabs: 18.0 against 11.3 us;
+  // 8192 x 8192, 13 in two: 22.8 against 25.6, 16 in three: 28.0 against 25.6; 28672 x 8192, 16
+  // in three: 52 against 82).
+  bool in16 = !f32 && c.M <= kW4Max16;
+  if (in16 && c.M > 8 && c.sdt == c.dtype) {
+    const int64_t slabs =
+        cdiv(w4_slab16_bytes(p->blocks, c.M), kW4MaxSmem - w4_stream_fixed(2, gpb, wide, true));
+    in16 = c.N * p->kp >= (slabs - 1) << 26;
+  }
+  if (digits || in16) {
     p->stream = true;
-    p->x16 = c.M * kW4Digits > (f32 ? kW4MaxCols : 8);
+    p->x16 = !digits;
     const int cols = static_cast<int>(p->x16 ? c.M : c.M * kW4Digits);
     p->nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
-    const int gpb = c.group == 32 ? 4 : c.group == 64 ? 2 : 1;
     const int pad = 8 * p->nt;
     // One CTA per SM.  With fewer 16-row tiles than SMs, a cluster of CTAs shares each tile's K.
     const int64_t tiles = cdiv(c.N, 16);
@@ -659,7 +672,6 @@ void plan_w4(const W4Call& c, const DeviceInfo& d, const LmInfo& lm, W4Plan* p) 
     // Two rows are cut in every CTA (a round of some 150 instructions per row and 48 blocks),
     // more once for all.
     p->cut_before = !p->x16 && c.M > 2;
-    const bool wide = c.sdt == TILEC_DTYPE_F32;
     const int64_t room = kW4MaxSmem - w4_stream_fixed(p->nt, gpb, wide, p->x16);
     auto slab_bytes = [&](int64_t n) { return p->x16 ? w4_slab16_bytes(n, c.M) : w4_slab_bytes(n, cols, pad, gpb); };
     int64_t slab = p->per_cta;

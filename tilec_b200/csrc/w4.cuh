@@ -15,15 +15,11 @@
 //   scale << 16 (16-bit scales), or two, zero and the fp32 scale.  Groups longer than 128 have
 //   theirs in every block.
 //
-// Up to some tens of rows of x the product streams the codes once (K/2 bytes a row of W).
-// At full bandwidth an SM has under three lane-instructions per weight, too few to convert
-// and multiply each weight on the FMA pipe, so the sums run on mma.sync: 16 rows of W against
-// 8 columns at a time.  (tcgen05 would need the converted weights to pass through shared
-// memory first; with so few columns its rate is not what bounds this.)  The fewest rows take
-// the integer form (w4_stream.cuh); here, for 11 to 32 rows of 16-bit x, a code becomes a
-// 16-bit float exactly: 0x4300 | code is 128 + code in bf16 (0x6400 | code is 1024 + code in
-// fp16), minus (128 + zero).  Products are exact, sums fp32; the scale multiplies a group's
-// fp32 sum.
+// Up to 256 rows of x the product streams the codes once (K/2 bytes a row of W).  At full
+// bandwidth an SM has under three lane-instructions per weight, too few to convert and multiply
+// each weight on the FMA pipe, so the sums run on tensor cores: mma.sync, 16 rows of W against 8
+// columns at a time, for up to 16 rows of x (w4_stream.cuh), tcgen05 with the weight expanded in
+// shared memory for more (w4_tc.cuh).
 #pragma once
 
 #include <cuda_bf16.h>

@@ -1,10 +1,13 @@
-// w4_stream.cuh -- the few-rows product with 4-bit weights on the integer tensor path.
+// w4_stream.cuh -- the few-rows product with 4-bit weights on mma.sync: one row of x (fp32:
+// up to 8; two of a large weight) on the integer path, up to 16 rows of 16-bit x on the 16-bit one.
 //
 // One token's product reads N * K / 2 bytes of codes and is bound by memory, if only the
 // arithmetic keeps up: at 6.5 TB/s a quarter SM has about 180 cycles per 1 KB of codes (16
-// rows x 128 k).  On the 16-bit path (w4_mma_kernel) a code costs 1.4 instructions to become
-// a 16-bit float, most of them on the half-rate integer pipe: 28672 x 8192 took 40 us.  An
-// 8-bit operand needs 3 for 8 codes, and m16n8k32 takes twice the k at the same rate:
+// rows x 128 k).  As 16-bit floats (multiply16: 0x4300 | code is 128 + code in bf16, 0x6400 |
+// code is 1024 + code in fp16, minus 128 + zero; products are exact, sums fp32, the scale
+// multiplies a group's sum) a code costs 1.4 instructions, most of them on the half-rate integer
+// pipe.  An 8-bit operand (multiply8) needs 3 for 8 codes, and m16n8k32 takes twice the k at the
+// same rate, for four columns per row of x:
 //
 //   * per 128-k block and row, x becomes whole numbers X = round(x * 2^(29 - e)), 2^e <= the
 //     block's largest magnitude < 2^(e + 1), in four signed 8-bit digits: x is off by at most
@@ -17,10 +20,11 @@
 // The sums start at 0x4B400000 - zero * sum X: read as a float that is 1.5 * 2^23 + the sum
 // (|sum| < 2^22), which saves the conversions.
 //
-// One CTA per SM, persistent, with 24 warps that share one copy of x.  A CTA takes an equal
+// One CTA per SM, persistent, with 16 warps that share one copy of x.  A CTA takes an equal
 // run of 16-row tiles, and its warps equal runs of their pieces (16 rows x 128 k): a warp's
 // run is one run of memory too, streamed through a ring of its own in shared memory by bulk
-// copies of two pieces each, so that 150 KB are on their way to an SM at any time.  Where a
+// copies of four pieces each (two where x needs the room), so that 140 (70) KB are on their way
+// to an SM at any time.  Where a
 // tile is shared by several warps their sums meet in shared memory, in the order of K.
 //
 // x is cut by the CTAs themselves where that is little work (one or two rows), otherwise once,
@@ -31,7 +35,8 @@
 // Measured, 28672 x 8192, one token (125 MB): 27.8 us, 4.5 TB/s; loads alone take 25 in the
 // best of the forms tried.  On the way: rows of codes with the group words apart 35 to 40 us
 // (the words alone cost 6); 24 warps with copies of two pieces 30.5; 12 warps 30.3; CTAs of
-// 128 rows, two waves of them for want of one slot, 40.
+// 128 rows, two waves of them for want of one slot, 40.  8 rows: 34.8 us (a grid of small CTAs
+// with cp.async rings 48), 16 rows, x in three slabs: 52.
 #pragma once
 
 #include "w4.cuh"
@@ -66,7 +71,7 @@ struct W4StreamCfg {
   static constexpr int kThreads = 32 * kW4StreamWarps;
   static constexpr int kPiece = w4_piece_bytes(GPB, WIDE);
   // Pieces a copy.  An SM's bulk copies start some 60 ns apart, so few large ones keep up with
-  // HBM; with more columns x needs the room.
+  // HBM; with more columns, or 16-bit x, x needs the room (16-bit x, 3 rows: no faster with four).
   static constexpr int kRun = XT == 0 && NT == 1 && kPiece <= 1152 ? 4 : 2;
   static constexpr int kStage = kRun * kPiece;
   static constexpr int kStages = 2;
@@ -298,7 +303,9 @@ __global__ void __launch_bounds__(32 * kW4StreamWarps, 1) w4_stream_kernel(const
     uint32_t wa[WB / 4], wb[WB / 4];
     lds_words(wa, piece + lane_words);
     lds_words(wb, piece + lane_words + 8 * WB);
-    float acc[NT][4], sa = 0.f, sb = 0.f;
+    // A group's sum in two parts: one chain of eight dependent MMAs is what a warp would wait for
+    // (28672 x 8192, 8 rows: 38.9 us, in two parts 34.8, in four 37.7).
+    float acc[NT][2][4], sa = 0.f, sb = 0.f;
     uint32_t za = 0, zb = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -327,19 +334,20 @@ __global__ void __launch_bounds__(32 * kW4StreamWarps, 1) w4_stream_kernel(const
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
         const uint4 xv = lds128(x_col[i] + blk * (2 * kW4Block) + 64 * j);
-        if (j % kSteps == 0)
-          mma_16816_zero<XT == 2>(acc[i], u[0], v[0], u[1], v[1], xv.x, xv.y);
-        else
-          mma_16816<XT == 2>(acc[i], u[0], v[0], u[1], v[1], xv.x, xv.y);
-        mma_16816<XT == 2>(acc[i], u[2], v[2], u[3], v[3], xv.z, xv.w);
+        if (j % kSteps == 0) {
+          mma_16816_zero<XT == 2>(acc[i][0], u[0], v[0], u[1], v[1], xv.x, xv.y);
+          mma_16816_zero<XT == 2>(acc[i][1], u[2], v[2], u[3], v[3], xv.z, xv.w);
+        } else {
+          mma_16816<XT == 2>(acc[i][0], u[0], v[0], u[1], v[1], xv.x, xv.y);
+          mma_16816<XT == 2>(acc[i][1], u[2], v[2], u[3], v[3], xv.z, xv.w);
+        }
       }
       if ((j + 1) % kSteps == 0) {
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-          total[i][0] = fmaf(acc[i][0], sa, total[i][0]);
-          total[i][1] = fmaf(acc[i][1], sa, total[i][1]);
-          total[i][2] = fmaf(acc[i][2], sb, total[i][2]);
-          total[i][3] = fmaf(acc[i][3], sb, total[i][3]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            total[i][c] = fmaf(acc[i][0][c] + acc[i][1][c], c < 2 ? sa : sb, total[i][c]);
         }
       }
     }

@@ -367,13 +367,14 @@ def matrix_mul_w4(x, weight, bias=None, out=None):
     bfloat16 on the weight's device; bias None or [N] of x's dtype.  Returns (or writes into
     `out`, [..., N] with unit column stride, sharing no memory with x or bias) x's dtype.
 
-    Up to 8 rows of x, the decoding case, the codes are read once and enter exactly: sums are
-    fp32, with one rounding at the end.  One or two rows (float32: all 8) go through the integer
-    tensor path, where x is held in steps of 2^-29 of the power of two at or below the largest
-    magnitude of its block of 128.  With more rows the weight is rounded once to x's dtype and
-    multiplied on the tensor cores: up to 256 rows of 16-bit x (and scales of its dtype) it is
-    expanded on the way, otherwise into the workspace, at most 256 MiB (or 256 rows of it) at a
-    time (float32: exact, and the 3xTF32 product of matrix_mul).  Not differentiable."""
+    Up to 8 rows of x, the decoding case (many 16-bit calls of up to 16), the codes are read once
+    and enter exactly: sums are fp32, with one rounding at the end.  One row (float32: up to
+    8; two of a large weight) goes through the integer tensor path, where x is held in steps of 2^-29 of the power of two
+    at or below the largest magnitude of its block of 128.  With more rows the weight is rounded
+    once to x's dtype and multiplied on the tensor cores: up to 256 rows of 16-bit x (and scales
+    of its dtype) it is expanded on the way, otherwise into the workspace, at most 256 MiB (or
+    256 rows of it) at a time (float32: exact, and the 3xTF32 product of matrix_mul).  Not
+    differentiable."""
     if not isinstance(weight, W4Weight):
         raise TypeError(f"matrix_mul_w4: weight must be a W4Weight (pack_w4, quantize_w4), got {type(weight).__name__}")
     n, k = weight.shape
