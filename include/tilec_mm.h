@@ -316,10 +316,11 @@ TILEC_API size_t tilec_linear_ce_workspace_bytes(const void* x, const void* w, i
  *   Codes of a row as 32-bit little-endian words: word 4t + j (t, j = 0..3) holds k = 32j + 8t +
  *   0..7 of the block, k = 2i in bits 4i..4i+3 and k = 2i + 1 in bits 4i+16..4i+19 (i = 0..3).
  *   Rows past N and k past K: any codes, finite scales.
- * Up to 8 rows, codes, zero points and scales enter exactly and sums are fp32; one or two rows
- * (fp32: all 8) of x enter as whole multiples of 2^-29 of the power of two at or below the
- * largest magnitude of their block of 128 k.  With more rows the weight (code - zero) * scale
- * is rounded once to dtype and multiplied on the tensor cores (fp32: the 3xTF32 product).
+ * Up to 8 rows (many 16-bit calls of up to 16), codes, zero points and scales enter exactly and
+ * sums are fp32; one row (fp32: up to 8; two of a large weight) of x enters as whole multiples of
+ * 2^-29 of the power of two at or below the largest magnitude of its block of 128 k.  With more
+ * rows the weight (code - zero) * scale is rounded once to dtype and multiplied on the tensor
+ * cores (fp32: the 3xTF32 product).  out shares no memory with x or bias.
  * Workspace: tilec_mm_w4_workspace_bytes (at most 256 MiB of expanded weights or 256 rows). */
 TILEC_API int tilec_mm_w4(const void* x, int32_t dtype, int64_t M, int64_t ldx, const void* weight,
                           int32_t scale_dtype, int64_t N, int64_t K, int64_t group, const void* bias, void* out,

@@ -140,6 +140,23 @@ def test_abi_refusals():
     assert lib.tilec_linear_ce_workspace_bytes(None, None, 3, 4, 16, 8, 8, 8, 2, 0) == 0
 
 
+def test_abi_refuses_pointers_off_their_elements():
+    from tilec_b200 import _native
+    lib = _native.load()
+
+    def forward(y=256, loss=256, stats=256):
+        return lib.tilec_linear_ce_forward(256, 256, y, 2, 4, 16, 8, 8, 8, -100, 2, loss, stats, None, 0, None)
+
+    def backward(y=256, stats=256, grad=256):
+        return lib.tilec_linear_ce_backward(256, 256, y, 2, 4, 16, 8, 8, 8, -100, 2, stats, grad, 256, 256, None, 0,
+                                            None)
+
+    for bad in (dict(y=260), dict(loss=258), dict(stats=260)):
+        assert forward(**bad) == 1, bad
+    for bad in (dict(y=260), dict(stats=260), dict(grad=258)):
+        assert backward(**bad) == 1, bad
+
+
 # ---------------------------------------------------------------- numerics
 gpu = pytest.mark.gpu
 

@@ -7,7 +7,8 @@
 
 Layout: ``ext`` (the drop-in op, tilec/ext.py), ``language`` (host helpers), ``select``
 (per-shape kernel selection, the B200 counterpart of tilec/tune.py), ``dist`` (row-
-sharded multi-GPU matrix_mul over NCCL), ``_native`` (ctypes binding of the C ABI in
+sharded multi-GPU matrix_mul over NCCL), ``lm`` (linear_cross_entropy and matrix_mul_w4,
+products of a language model, exported by ``ext``), ``_native`` (ctypes binding of the C ABI in
 include/tilec_mm.h), ``build`` (nvcc build of the in-tree kernel library).
 Importing the package needs no GPU and no compiler; the kernel library is loaded on
 first use.

@@ -250,13 +250,15 @@ size_t mm_bytes(const Problem& q, int flags) {
   return workspace_for(q, &cfg);
 }
 
+inline bool misaligned(const void* p, unsigned bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) != 0; }
+
 int check_ce(const CeCall& c) {
   if (c.dtype < TILEC_DTYPE_F32 || c.dtype > TILEC_DTYPE_BF16) return TILEC_ERR_BAD_ARG;
   if (c.reduction < kReduceNone || c.reduction > kReduceMean) return TILEC_ERR_BAD_ARG;
   if (c.T < 0 || c.V < 1 || c.D < 1 || c.ldx < c.D || c.ldw < c.D) return TILEC_ERR_BAD_ARG;
   if (!c.w || (c.T > 0 && (!c.x || !c.target))) return TILEC_ERR_BAD_ARG;
-  const uintptr_t elem = c.dtype == TILEC_DTYPE_F32 ? 3 : 1;
-  if ((reinterpret_cast<uintptr_t>(c.x) & elem) || (reinterpret_cast<uintptr_t>(c.w) & elem)) return TILEC_ERR_BAD_ARG;
+  const unsigned elem = c.dtype == TILEC_DTYPE_F32 ? 4 : 2;
+  if (misaligned(c.x, elem) || misaligned(c.w, elem) || misaligned(c.target, 8)) return TILEC_ERR_BAD_ARG;
   if (c.T >= (int64_t(1) << 30) || c.V >= (int64_t(1) << 30) || c.D >= (int64_t(1) << 30)) return TILEC_ERR_UNSUPPORTED;
   return TILEC_OK;
 }
@@ -615,9 +617,8 @@ int check_w4(const W4Call& c) {
 int check_w4_pointers(const W4Call& c) {
   if (c.M == 0 || c.N == 0) return TILEC_OK;
   if (!c.x || !c.weight || !c.out || c.ldo < c.N) return TILEC_ERR_BAD_ARG;
-  const uintptr_t elem = c.dtype == TILEC_DTYPE_F32 ? 3 : 1;
-  auto off = [](const void* p, uintptr_t mask) { return (reinterpret_cast<uintptr_t>(p) & mask) != 0; };
-  if (off(c.weight, 15) || off(c.x, elem) || off(c.out, elem) || off(c.bias, elem))
+  const unsigned elem = c.dtype == TILEC_DTYPE_F32 ? 4 : 2;
+  if (misaligned(c.weight, 16) || misaligned(c.x, elem) || misaligned(c.out, elem) || misaligned(c.bias, elem))
     return TILEC_ERR_BAD_ARG;
   return TILEC_OK;
 }
@@ -930,6 +931,7 @@ int tilec_linear_ce_forward(const void* x, const void* w, const int64_t* target,
   const int rc = check_ce(c);
   if (rc) return rc;
   if (!stats || (!loss && (T > 0 || reduction != kReduceNone))) return TILEC_ERR_BAD_ARG;
+  if (misaligned(stats, 8) || misaligned(loss, 4)) return TILEC_ERR_BAD_ARG;
   return ce_forward(c, loss, stats, workspace, ws_bytes, static_cast<cudaStream_t>(stream));
 }
 
@@ -941,7 +943,7 @@ int tilec_linear_ce_backward(const void* x, const void* w, const int64_t* target
   const int rc = check_ce(c);
   if (rc) return rc;
   if (!stats || (!grad && (T > 0 || reduction != kReduceNone))) return TILEC_ERR_BAD_ARG;
-  if (!aligned16(dx) || !aligned16(dw)) return TILEC_ERR_BAD_ARG;
+  if (!aligned16(dx) || !aligned16(dw) || misaligned(stats, 8) || misaligned(grad, 4)) return TILEC_ERR_BAD_ARG;
   return ce_backward(c, stats, grad, dx, dw, workspace, ws_bytes, static_cast<cudaStream_t>(stream));
 }
 
