@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(256) f16_join_slabs_kernel(const float* __rest
 
 // Rows of `src` (row stride lds) to rows of `dst` that 16-byte stores cannot take, dst row
 // rows[r] (or r).  The product kernel stores whole 8-column pieces; storing odd rows from there
-// cost 155 us for the gradient of a 30011 x 777 weight, through this copy it is 70.  Dense rows
+// cost 155 us for the gradient of a 30011 x 777 weight, through this copy it is 76 (50 + 26).  Dense rows
 // (rows == nullptr, ldd == cols) go out as one run, 16 bytes a thread; others by element.
 __global__ void __launch_bounds__(256) unpad16_kernel(const unsigned short* __restrict__ src, int64_t lds,
                                                       unsigned short* __restrict__ dst, int64_t ldd, int64_t nrows,

@@ -16,7 +16,9 @@
 //     know how many there are.  Tiles past the last row are never started;
 //   * K can be cut into slices whose fp32 sums go to slabs (few tiles, long K).
 //
-// Where time goes (B200): see launch_f16 in lm_ops.cuh.
+// Where time goes (B200): 4096 x 32768 x 2048 keeps the tensor pipe 79 % (statistics) to 93 %
+// busy; a tile's epilogue reads tensor memory for 1.6 us, which the next tile's MMAs cover but
+// for the last tile.  Large products run into the power limit.
 #pragma once
 
 #include <cuda_bf16.h>
