@@ -625,9 +625,10 @@ int check_w4_pointers(const W4Call& c) {
 
 // How many rows of x run where: one (fp32: up to 8) in digits on w4_stream_kernel; up to 16 of
 // 16-bit x there too, as they are, but for two against a large weight (4096 x 4096: 7.4 us, in
-// digits 9.5; 8192 x 8192: 15.6 and 19.4; 28672 x 8192: 36.7 and 33.0); up to 256 of 16-bit x whose type the scales share on w4_tc_kernel, 128 at a time (8192 x 8192: 128 rows
-// 35 us, twice that for 256; expanded first, either takes 89); for the rest W is expanded once
-// into the workspace and multiplied on the tcgen05 kernels (fp32: 3xTF32).
+// digits 9.5; 8192 x 8192: 15.6 and 19.4; 28672 x 8192: 36.7 and 33.0); up to 256 of 16-bit x
+// whose type the scales share on w4_tc_kernel, 128 at a time (8192 x 8192: 128 rows 35 to 39 us,
+// twice that for 256; expanded first, either takes 89); for the rest W is expanded once into the
+// workspace and multiplied on the tcgen05 kernels (fp32: 3xTF32).
 constexpr int64_t kW4MaxCols = 32;  // of digits
 constexpr int64_t kW4Max16 = 16;    // rows of 16-bit x
 

@@ -1,7 +1,7 @@
 // w4_tc.cuh -- products of some tens of rows with 4-bit weights on the 5th-generation tensor
 // cores (tcgen05, fp32 accumulators in TMEM), the weight expanded on the way.
 //
-// From 9 rows of x on, mma.sync's share of the work grows with the rows while the weight still
+// From some 9 to 17 rows of x on (see plan_w4), mma.sync's share of the work grows with the rows while the weight still
 // has to be read once; expanding it in HBM first (w4_expand_kernel) costs five times its bytes.
 // Here a CTA takes 128 rows of W as the M side of the product and up to 128 rows of x as its N
 // side (swapped, so that the few rows of x pad to 16 and not to 128 or 256):
@@ -16,10 +16,10 @@
 //     32 neighbouring outputs of one row of x.
 // K is split over CTAs that write fp32 slabs (f16_join_slabs_kernel adds them in order).
 //
-// Measured (graph replay): 4096 x 4096 10.7 us for 16 rows, 13.0 for 128; 8192 x 8192 25.2 and
-// 35 (the codes alone: 6 at HBM's rate); 28672 x 8192 82 and 112.  Without the expansion's
-// arithmetic it is no faster, without seven of eight MMAs a fifth: what bounds it is the
-// hand-over of a block between the roles (about half a microsecond).
+// Measured (graph replay): 4096 x 4096 12 us for 32 rows, 15 for 128; 8192 x 8192 26.5 and 39
+// (the codes alone: 6 at HBM's rate); 28672 x 8192 84 and 128.  A CTA takes some 0.65 us per
+// block: the busier SMs issue 54 % of the time, three or four operand buffers and three code
+// stages are no faster, and a last wave of tiles that fills half the SMs is the rest.
 #pragma once
 
 #include "w4_stream.cuh"
@@ -49,7 +49,7 @@ struct W4TcCfg {
   static constexpr int kABytes = 2 * kHalf;                    // a block
   static constexpr int kMaxBStages = 8;
   static constexpr int kBBytes = 65536;                        // x: as many blocks as fit, up to 8
-  static constexpr int kABufs = 2;   // three, with copies of three blocks: as fast
+  static constexpr int kABufs = 2;   // three or four: no faster (28672 x 8192, 32 rows: 84, 86, 88 us)
   static constexpr int kOffB = kABufs * kABytes, kOffCodes = kOffB + kBBytes;
   static constexpr int kOffBars = kOffCodes + kCodeStages * kCodeStage;
   static constexpr int kBarBytes = 256;
