@@ -469,3 +469,35 @@ def test_workspace_follows_each_operand_alignment():
         assert torch.equal(ext.matrix_mul_w4(xs, weight, out=out), ref)
     with pytest.raises(ValueError, match="requires a gradient"):
         ext.matrix_mul_w4(xs, weight, out=room[:300 * 64].view(300, 64).requires_grad_())
+
+
+@gpu
+@pytest.mark.parametrize("m,k,dtype", [(128, 8192, "bf16"), (20, 14336, "f16"), (250, 4096, "bf16")])
+def test_gave_up_between_codes_and_x(m, k, dtype):
+    """The expanding kernel with every wait cut to 1 ns, over and over: it may give up between a
+    unit's codes and the blocks of x that go with them.  The calls in between, at the full limit
+    on the same SMs, give the same bits each time."""
+    from tilec_b200 import TilecError, _native
+    x, codes, scales, zeros, _ = _make(m, 260, k, 64, dtype)
+    w = ext.pack_w4(codes, scales, zeros, 64).to("cuda")
+    x = x.cuda()
+    good = ext.matrix_mul_w4(x, w)
+    ext.check_device()
+    lib = _native.load()
+    given_up = 0
+    for _ in range(20):
+        _native.check(lib.tilec_mm_set_wait_limit(1, None), "set_wait_limit")
+        try:
+            got = ext.matrix_mul_w4(x, w)
+        finally:
+            _native.check(lib.tilec_mm_set_wait_limit(0, None), "set_wait_limit")
+        assert torch.equal(ext.matrix_mul_w4(x, w), good)
+        nan = torch.isnan(got)
+        assert torch.equal(got[~nan], good[~nan])
+        try:
+            ext.check_device()
+            assert not nan.any()
+        except TilecError as e:
+            assert "TIMEOUT" in str(e)
+            given_up += 1
+    assert given_up

@@ -152,7 +152,7 @@ __global__ void __launch_bounds__(W4TcCfg<GPB>::kThreads, 1)
     const int row_tiles = min(8, (p.N - n0 + 15) / 16);
     const uint8_t* src =
         p.data + ((static_cast<int64_t>(tile) * 8 + min(lane, row_tiles - 1)) * p.blocks + b_begin) * Cfg::kPiece;
-    int i = 0, bs = 0;
+    int i = 0, units = 0, bs = 0;  // blocks of x and units of codes that were sent for
     uint32_t b_phase = 1;
     for (; i < nblk && ok; ++i) {
       if (i % RUN == 0) {  // codes of this block and the next ones
@@ -164,6 +164,7 @@ __global__ void __launch_bounds__(W4TcCfg<GPB>::kThreads, 1)
         if (lane < row_tiles)
           bulk_load(codes + s * Cfg::kCodeStage + lane * Cfg::kCodeTile, src + static_cast<int64_t>(i) * Cfg::kPiece,
                     run * Cfg::kPiece, &c_full[s]);
+        units = u + 1;
       }
       ok = __all_sync(0xffffffffu, i < SB || mbar_wait(&b_empty[bs], b_phase, abort_flag));
       if (!ok) break;
@@ -177,9 +178,9 @@ __global__ void __launch_bounds__(W4TcCfg<GPB>::kThreads, 1)
         b_phase ^= 1;
       }
     }
-    // Every copy has landed before this CTA may end, on every path.
+    // Every copy has landed before this CTA may end, on every path (a unit's codes go out before
+    // the wait for its first block's room in the ring of x, which may be given up).
     if (lane == 0) {
-      const int units = (i + RUN - 1) / RUN;
       for (int f = max(0, units - SC); f < units; ++f) mbar_drain(&c_full[f % SC], (f / SC) & 1);
       for (int f = max(0, i - SB); f < i; ++f) mbar_drain(&b_full[f % SB], (f / SB) & 1);
     }
