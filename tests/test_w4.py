@@ -501,3 +501,62 @@ def test_gave_up_between_codes_and_x(m, k, dtype):
             assert "TIMEOUT" in str(e)
             given_up += 1
     assert given_up
+
+
+@gpu
+@pytest.mark.parametrize("m,n,k,group,dtype,sdtype",
+                         [(16, 40005, 2700, 32, "bf16", "f32"),    # two slabs of x, two groups of row tiles a CTA
+                          (4, 40005, 1000, 64, "f16", "f16"),      # two groups
+                          (6, 40005, 5400, 128, "f32", "f32"),     # both, x cut beforehand
+                          (16, 260, 28672, 32, "f16", "f32")])     # slabs, K shared by a cluster
+def test_gave_up_before_the_last_slab_or_group(m, n, k, group, dtype, sdtype):
+    """A streaming warp that gave up goes on through the slabs of x and groups of row tiles that are
+    left: its outputs are NaN (digits: right), the others right, and correct calls in between on the
+    same SMs give the same bits each time."""
+    from tilec_b200 import TilecError, _native
+    x, codes, scales, zeros, _ = _make(m, n, k, group, dtype, sdtype=sdtype)
+    w = ext.pack_w4(codes.cuda(), scales.cuda(), zeros.cuda(), group)
+    x = x.cuda()
+    good = ext.matrix_mul_w4(x, w)
+    ext.check_device()
+    w64 = _weight64(codes.cuda(), scales.cuda(), zeros.cuda(), group)
+    y = x.double() @ w64.t()
+    # twice the bound of few rows: groups' sums and parts added in fp32 in any order (see _long_bound)
+    tol = 2 * _long_bound(x, w64, y, dtype, k, group)
+    assert ((good.double() - y).abs() <= tol).all()
+    lib = _native.load()
+    given_up = 0
+    flush = torch.empty(1 << 28, dtype=torch.uint8, device="cuda")
+    for _ in range(8):
+        flush.zero_()   # the weight comes from memory: waits last longer than a step of the clock
+        _native.check(lib.tilec_mm_set_wait_limit(1, None), "set_wait_limit")
+        try:
+            got = ext.matrix_mul_w4(x, w)
+        finally:
+            _native.check(lib.tilec_mm_set_wait_limit(0, None), "set_wait_limit")
+        assert torch.equal(ext.matrix_mul_w4(x, w), good)
+        nan = torch.isnan(got)
+        assert ((got.double() - y).abs() <= tol)[~nan].all()
+        try:
+            ext.check_device()
+            assert not nan.any()
+        except TilecError as e:
+            assert "TIMEOUT" in str(e)
+            given_up += 1
+    assert given_up or n < 1000    # few pieces a warp: they may all have landed before the first wait
+
+
+def _long_bound(x, w64, y, dtype, k, group):
+    """Up to 16 rows on the streaming kernel, any K, S = sum_k |x w|: one fp32 addition per group
+    (of at most 128 k), per warp (16), CTA of a cluster (8) and slab of x (8), each off by 2^-24 S at
+    worst, 8 more for the scale's product and the digits' sums; a group's 16-bit sums on the tensor
+    cores as in the header (16 * 2^-23 S).  Digits hold x to 2^-30 of the power of two at or below
+    the largest magnitude of its block of 128 k (fp32 x; a 16-bit row alone too)."""
+    adds = -(-k // min(group, 128)) + 40
+    s = x.double().abs() @ w64.abs().t()
+    blocks = torch.nn.functional.pad(x.double().abs(), (0, -k % 128)).view(len(x), -1, 128)
+    step = torch.exp2(torch.floor(torch.log2(blocks.amax(2).clamp(min=2.0 ** -90))) - 30)
+    wb = torch.nn.functional.pad(w64.abs(), (0, -k % 128)).view(len(w64), -1, 128).sum(2)
+    held = step @ wb.t()
+    return (adds * 2.0 ** -24 + 2.0 ** -19) * s + held + 1.001 * U[dtype] * y.abs() + (
+        2.0 ** -25 if dtype == "f16" else 0.0)

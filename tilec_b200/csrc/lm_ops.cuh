@@ -596,6 +596,7 @@ struct W4Plan {
   bool pack_x = false;   // x is copied to aligned rows first (expanded weights)
   int nt = 1, splits = 1, slab = 1, per_cta = 0, ctas = 0;
   bool cut_before = false;
+  bool polling = false;  // w4_stream_kernel's waits, see W4StreamArgs
   size_t off_digits = 0, off_sums = 0, off_scale = 0;
   int64_t blocks = 0, kp = 0, piece = 0;
   int slices = 1, kb = 0;
@@ -657,6 +658,7 @@ void plan_w4(const W4Call& c, const DeviceInfo& d, const LmInfo& lm, W4Plan* p) 
   }
   if (digits || in16) {
     p->stream = true;
+    p->polling = d.short_waits;
     p->x16 = !digits;
     const int cols = static_cast<int>(p->x16 ? c.M : c.M * kW4Digits);
     p->nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
@@ -744,6 +746,7 @@ int launch_w4_stream(const W4Args& w, const W4Plan& p, uint8_t* ws, cudaStream_t
   a.row_tiles = static_cast<int>(cdiv(w.N, 16));
   a.per_cta = p.per_cta;
   a.slab = p.slab;
+  a.polling = p.polling;
   using Cfg = W4StreamCfg<NT, GPB, SC == 0, XT>;
   const size_t smem = size_t(Cfg::kFixed + (XT != 0 ? w4_slab16_bytes(p.slab, w.M) : w4_slab_bytes(p.slab, w.cols, 8 * NT, GPB)));
   if (int64_t(smem) > kW4MaxSmem) return TILEC_ERR_UNSUPPORTED;

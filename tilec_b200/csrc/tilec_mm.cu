@@ -54,6 +54,7 @@ struct DeviceInfo {
   int max_smem_optin = 0;
   int pair_slots = 0;  // CTA pairs of the stream-K pair kernel resident at once (0: stream-K off)
   int tf32p_slots = 0; // CTA pairs of the persistent TF32 pair kernel resident at once (0: not used)
+  std::atomic<bool> short_waits{false};  // tilec_mm_set_wait_limit shortened the device's limit
   cudaError_t init_err = cudaSuccess;
 };
 
@@ -1378,6 +1379,7 @@ int tilec_mm_set_wait_limit(int64_t limit_ns, void* stream) {
     cudaGetLastError();
     return TILEC_ERR_DEVICE;
   }
+  d->short_waits = v != 0 && v < kWaitLimitNs;
   return TILEC_OK;
 }
 

@@ -39,6 +39,7 @@
 // with cp.async rings 48), 16 rows, x in three slabs: 52.
 #pragma once
 
+#include "tc2_f16.cuh"
 #include "w4.cuh"
 
 namespace tilec {
@@ -63,6 +64,7 @@ struct W4StreamArgs {
   int row_tiles;
   int per_cta;       // blocks of K a CTA takes; a cluster's CTAs follow one another along K
   int slab;          // blocks of x in shared memory at a time
+  int polling;       // the device's wait limit is shortened (w4_wait_on)
 };
 
 // XT: how x enters: 0 in digits, else as 16-bit values of that TILEC_DTYPE_*.
@@ -251,6 +253,34 @@ __device__ __forceinline__ void w4_stage16(const W4Args& p, uint8_t* xs, int pit
   cp_async_wait<0>();
 }
 
+// What a warp does when a copy has not landed after one try (mbar_wait's loop, out of line).
+// `polling`: the device's limit is shortened (failure tests).  The suspending form of the test
+// sleeps for longer than a copy takes, so with it no limit below that would ever run out.
+__device__ __noinline__ bool w4_wait_on(uint32_t bar, uint32_t parity, volatile int* abort_flag, bool polling) {
+  const unsigned long long t0 = global_ns(), limit = wait_limit();
+  for (;;) {
+    if (polling) {
+      uint32_t done;
+      asm volatile(
+          "{\n\t.reg .pred p;\n\t"
+          "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+          "selp.u32 %0, 1, 0, p;\n\t}"
+          : "=r"(done)
+          : "r"(bar), "r"(parity)
+          : "memory");
+      if (done) return true;
+    } else if (mbar_try<false>(bar, parity, kHintStage)) {
+      return true;
+    }
+    if (*abort_flag) return false;
+    if (global_ns() - t0 > limit) {
+      *abort_flag = 1;
+      record_status(TILEC_DEV_TIMEOUT);
+      return false;
+    }
+  }
+}
+
 // SC: type of the scales (TILEC_DTYPE_*); with 16-bit x (XT != 0) 0, or 1 for either 16-bit type.
 // Grid: x = CTAs (clusters of `splits`, whose CTAs share their row tiles and split K).
 template <int NT, int GPB, int SC, int XT>
@@ -434,7 +464,9 @@ __global__ void __launch_bounds__(32 * kW4StreamWarps, 1) w4_stream_kernel(const
       const int first = min(pieces, warp * share), last = min(pieces, first + share);
       const int first_tile = n > 0 ? first / n : 0, first_blk = first - first_tile * n;
       // Up to kRun pieces of one tile follow one another in memory and go out in one copy.
-      int f_left = last - first, f_blk = first_blk, fill = stage;
+      // Once this warp gave up it sends for nothing more: its barriers are no longer kept up.
+      const bool in_step = ok;
+      int f_left = ok ? last - first : 0, f_blk = first_blk, fill = stage;
       const uint8_t* f_src =
           p.data + (static_cast<int64_t>(group + first_tile) * p.blocks + s0 + f_blk) * Cfg::kPiece;
       const int64_t skip = static_cast<int64_t>(p.blocks - n) * Cfg::kPiece;  // from a tile's slab to the next one's
@@ -520,7 +552,9 @@ __global__ void __launch_bounds__(32 * kW4StreamWarps, 1) w4_stream_kernel(const
       int tile = first_tile, blk = first_blk;
       bool from_start = blk == 0;   // this warp has the tile's first block
       for (int at = first; at < last && ok;) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&bars[stage], phase, abort_flag));
+        const uint32_t bar = smem_u32(&bars[stage]);
+        ok = __all_sync(0xffffffffu, (!a.polling && mbar_try<false>(bar, phase, kHintStage)) ||
+                                         w4_wait_on(bar, phase, abort_flag, a.polling));
         if (!ok) break;
         const uint32_t piece = ring_at + stage * Cfg::kStage;
         const int run = min(Cfg::kRun, min(last - at, n - blk));
@@ -543,8 +577,14 @@ __global__ void __launch_bounds__(32 * kW4StreamWarps, 1) w4_stream_kernel(const
         }
       }
       if (ok && first < last && blk > 0) leave(tile, false, tile == first_tile ? 0 : 1);
-      if (!ok) {  // gave up: let what is on its way land, and leave NaN
-        for (int i = 0; i < S; ++i) mbar_drain(&bars[i], i >= stage ? phase : phase ^ 1);
+      if (!ok) {  // gave up, here or earlier: let what is on its way land, and leave NaN
+        if (in_step) {
+          const int on_way = fill == stage ? S : (fill - stage + S) % S;  // one at least: the one waited for
+          for (int i = 0; i < on_way; ++i) {
+            const int at = (stage + i) % S;
+            mbar_drain(&bars[at], at >= stage ? phase : phase ^ 1);
+          }
+        }
         for (int i = lane; i < 2 * Cfg::kPart; i += 32) parts[2 * warp * Cfg::kPart + i] = __int_as_float(0x7fc00000);
         for (int k = first; k < last; k = (k / n + 1) * n)
           for (int i = lane; i < Cfg::kPart; i += 32) tile_sums[k / n * Cfg::kPart + i] = __int_as_float(0x7fc00000);
