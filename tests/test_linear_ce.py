@@ -479,3 +479,23 @@ def test_gave_up_is_nan_and_the_context_works(dtype):
     for again, g in zip(step(), good):
         assert torch.equal(again, g)
     ext.check_device()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("reduction", ["sum", "mean"])
+@pytest.mark.parametrize("shape", [(1100, 130, 520), (2048, 1000, 1024), (5000, 300, 77)])
+def test_no_target_where_the_sums_over_tokens_are_cut(shape, reduction, dtype):
+    """No token has a target and dW's sum over tokens is cut into slices: its slices are empty and
+    its factor, 1 / 0 for the mean, is not a number to multiply them by.  Gradients are zeros."""
+    x, w, y = _make(*shape, dtype)
+    y.fill_(IGNORE)
+    x.requires_grad_(True), w.requires_grad_(True)
+    loss = ext.linear_cross_entropy(x, w, y, reduction=reduction)
+    assert torch.isnan(loss) if reduction == "mean" else loss == 0
+    for go in (1.0, float("inf")):
+        dx, dw = torch.autograd.grad(loss, (x, w), torch.full_like(loss, go), retain_graph=True)
+        assert (dx == 0).all() and (dw == 0).all()
+    # the same sizes with one token left
+    y[len(y) // 2] = 3
+    _check(x, w, y, dtype, reduction)

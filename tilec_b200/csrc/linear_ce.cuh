@@ -62,7 +62,9 @@ __global__ void __launch_bounds__(1024) ce_select_kernel(const int64_t* __restri
   if (scale == nullptr) return;
   if (!per_token) {
     if (tid == 0) {
-      *scale = reduction == kReduceMean ? grad[0] / count[0] : grad[0];
+      // No token has a target: sums are empty, and 1 / 0 (or an infinite grad) times their
+      // zeros would be NaN.
+      *scale = base == 0 ? 0.f : reduction == kReduceMean ? grad[0] / count[0] : grad[0];
       head[1] = 1.f;
     }
     return;
