@@ -499,3 +499,24 @@ def test_no_target_where_the_sums_over_tokens_are_cut(shape, reduction, dtype):
     # the same sizes with one token left
     y[len(y) // 2] = 3
     _check(x, w, y, dtype, reduction)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("go", [1e-45, 1e-40, 5e-39, 1.2e-38, 1e-30])
+def test_vanishing_gradients_of_the_loss(go, dtype):
+    """Per-token gradients down to fp32's smallest number, zeros among them: nothing infinite or
+    NaN on the way, and no gradient above what the definition has.  An element of dx (dW) is at
+    most 2 go max|w| (2 go T max|x|) in magnitude; rounding adds one smallest step of the type."""
+    x, w, y = _make(64, 500, 64, dtype)
+    x.requires_grad_(True), w.requires_grad_(True)
+    loss = ext.linear_cross_entropy(x, w, y, reduction="none")
+    g = torch.full_like(loss, go)
+    g[::3] = 0
+    dx, dw = torch.autograd.grad(loss, (x, w), g)
+    step = {"bf16": 2.0 ** -133, "f16": 2.0 ** -24, "f32": 2.0 ** -149}[dtype]
+    assert (dx.double().abs() <= 2.1 * go * w.double().abs().max() + step).all()
+    assert (dw.double().abs() <= 2.1 * go * 64 * x.double().abs().max() + step).all()
+    assert (dx[::3] == 0).all()
+    if dtype == "f16":
+        assert (dx == 0).all() and (dw == 0).all()

@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(1024) ce_select_kernel(const int64_t* __restri
     if (g > 0.f && g < INFINITY) {
       int ex = 0;
       frexpf(g, &ex);
-      g = ldexpf(1.f, min(ex, 126));
+      g = ldexpf(1.f, max(-126, min(ex, 126)));  // with 1 / g a number too
     } else {
       g = 1.f;
     }
