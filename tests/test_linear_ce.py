@@ -520,3 +520,34 @@ def test_vanishing_gradients_of_the_loss(go, dtype):
     assert (dx[::3] == 0).all()
     if dtype == "f16":
         assert (dx == 0).all() and (dw == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("first", [True, False])
+def test_selection_table_and_workspace(first, monkeypatch):
+    """The fp32 form runs the products that the selection table selects: the first call installs the
+    table, and a later table whose plans take more room changes the workspace with them."""
+    from tilec_b200 import _native, select
+    x, w, y = _make(300, 700, 4096, "f32")
+    split = [[0, 40, 0, 40, 0, 40, _native.VARIANTS["3xtf32"], 16]]
+    small = [[0, 40, 0, 40, 0, 40, _native.VARIANTS["simt"], 0]]
+    try:
+        if first:
+            select.install(small)
+            monkeypatch.setattr(select, "_installed", False)
+            monkeypatch.setattr(select, "load_table", lambda path=None: split)
+            monkeypatch.setattr(ext, "_installed", False)
+            a = ext.linear_cross_entropy(x, w, y)       # installs `split`
+            assert select._installed
+            ext.matrix_mul(x[:, :64].contiguous(), x[:64, :64].contiguous())
+            assert torch.equal(ext.linear_cross_entropy(x, w, y), a)
+        else:
+            select.install(small)
+            _check(x, w, y, "f32")
+        select.install(split)
+        _check(x, w, y, "f32")
+        select.install(small)
+        _check(x, w, y, "f32")
+    finally:
+        monkeypatch.undo()
+        select.install(select.load_table())

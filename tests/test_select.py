@@ -103,3 +103,14 @@ def test_train_ships_a_table_only_when_cross_validation_prefers_it(tmp_path, mon
     doc = tune.train(str(path), str(out))
     assert doc["rows"] and doc["fitted_table_kept"] is True
     assert all(r[6] == "simt" for r in doc["rows"])
+
+
+def test_installing_a_table_forgets_every_cached_workspace_size():
+    """Sizes depend on the plans the table selects: matrix_mul's, and those of the fp32 forms of
+    linear_cross_entropy and matrix_mul_w4."""
+    from tilec_b200 import ext, lm
+    caches = (ext._WS_BYTES, lm._CE_BYTES, lm._W4_BYTES)
+    for c in caches:
+        c["as if from a call under another table"] = 1
+    select.install(select.load_table())
+    assert not any(caches)

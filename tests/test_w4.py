@@ -560,3 +560,21 @@ def _long_bound(x, w64, y, dtype, k, group):
     held = step @ wb.t()
     return (adds * 2.0 ** -24 + 2.0 ** -19) * s + held + 1.001 * U[dtype] * y.abs() + (
         2.0 ** -25 if dtype == "f16" else 0.0)
+
+
+@gpu
+def test_selection_table_and_workspace(monkeypatch):
+    """fp32 x of many rows runs the product that the selection table selects, here too."""
+    from tilec_b200 import _native, select
+    data = _make(40, 300, 4096, 128, "f32")
+    try:
+        monkeypatch.setattr(select, "_installed", False)
+        monkeypatch.setattr(select, "load_table",
+                            lambda path=None: [[0, 40, 0, 40, 0, 40, _native.VARIANTS["simt"], 0]])
+        _check(*data, 128, "f32")
+        assert select._installed
+        select.install([[0, 40, 0, 40, 0, 40, _native.VARIANTS["3xtf32"], 16]])
+        _check(*data, 128, "f32")
+    finally:
+        monkeypatch.undo()
+        select.install(select.load_table())

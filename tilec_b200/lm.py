@@ -12,7 +12,7 @@ missing kernel library raises.  (Packing and quantising are plain torch and run 
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import _native
+from . import _native, select
 
 _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}             # TILEC_REDUCE_*
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # TILEC_DTYPE_*
@@ -36,6 +36,13 @@ def _workspace(nbytes, device):
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
+
+
+def _library():
+    """The kernel library, with the selection table that the fp32 forms' products go by."""
+    if not select._installed:
+        select.ensure_installed()
+    return _native.load()
 
 
 _ext = None   # tilec_b200.ext, which imports this module
@@ -89,7 +96,7 @@ def _ce_workspace(lib, px, pw, dt, t, v, d, ldx, ldw, red, grads, device):
 
 def _ce_forward(x, weight, target, ignore_index, reduction):
     """(loss, statistics for the backward pass)"""
-    lib, fast, dev = _native.load(), _native.fast(), x.device
+    lib, fast, dev = _library(), _native.fast(), x.device
     xr, ldx = _rows(x)
     wr, ldw = _rows(weight)
     t, d = x.shape
@@ -121,7 +128,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad):
         x, weight, target, stats = ctx.saved_tensors
-        lib, fast, dev = _native.load(), _native.fast(), x.device
+        lib, fast, dev = _library(), _native.fast(), x.device
         xr, ldx = _rows(x)
         wr, ldw = _rows(weight)
         t, d = x.shape
@@ -406,7 +413,7 @@ def matrix_mul_w4(x, weight, bias=None, out=None):
         return out
     if bias is not None:
         bias = bias.contiguous()
-    lib = _native.load()
+    lib = _library()
     index = dev.index
     prev = torch.cuda.current_device()
     switch = prev != index
