@@ -551,3 +551,19 @@ def test_selection_table_and_workspace(first, monkeypatch):
     finally:
         monkeypatch.undo()
         select.install(select.load_table())
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_refuses_forward_mode_tangents(grad):
+    """There is no forward-mode derivative: a tangent is refused, not dropped."""
+    fw = torch.autograd.forward_ad
+    x, w, y = torch.randn(4, 8), torch.randn(16, 8), torch.zeros(4, dtype=torch.int64)
+    if grad:
+        x.requires_grad_(True)
+    with fw.dual_level():
+        for a, b in ((fw.make_dual(x, torch.ones_like(x)), w), (x, fw.make_dual(w, torch.ones_like(w)))):
+            for guard in (torch.enable_grad, torch.no_grad):
+                with guard(), pytest.raises(ValueError, match="forward-mode"):
+                    ext.linear_cross_entropy(a, b, y)
+        with pytest.raises(ValueError, match="CUDA"):   # no tangent: on to the next check
+            ext.linear_cross_entropy(x, w, y)

@@ -578,3 +578,18 @@ def test_selection_table_and_workspace(monkeypatch):
     finally:
         monkeypatch.undo()
         select.install(select.load_table())
+
+
+def test_refuses_forward_mode_tangents():
+    """There is no derivative: a tangent of x, bias or out is refused, not dropped."""
+    fw = torch.autograd.forward_ad
+    w = ext.pack_w4(torch.zeros(4, 64, dtype=torch.uint8), torch.ones(4, 2), group_size=32)
+    x, b, out = torch.ones(2, 64), torch.ones(4), torch.ones(2, 4)
+    with fw.dual_level():
+        def dual(t):
+            return fw.make_dual(t, torch.ones_like(t))
+        for args in ((dual(x), w), (x, w, dual(b)), (x, w, None, dual(out))):
+            with torch.no_grad(), pytest.raises(ValueError, match="forward-mode"):
+                ext.matrix_mul_w4(*args)
+        with pytest.raises(ValueError, match="CUDA"):
+            ext.matrix_mul_w4(x, w, b, out)

@@ -10,6 +10,7 @@ Like the rest of the package there is no CPU path for the products: CPU tensors 
 missing kernel library raises.  (Packing and quantising are plain torch and run anywhere.)
 """
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _native, select
@@ -43,6 +44,15 @@ def _library():
     if not select._installed:
         select.ensure_installed()
     return _native.load()
+
+
+def _refuse_tangents(where, *tensors):
+    """Raises for a tensor with a forward-mode tangent, which the kernels would drop."""
+    if getattr(forward_ad, "_current_level", 0) < 0:   # outside every dual level: nothing to look for
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise ValueError(f"{where}: no forward-mode derivative; detach the inputs")
 
 
 _ext = None   # tilec_b200.ext, which imports this module
@@ -156,7 +166,8 @@ def linear_cross_entropy(x, weight, target, ignore_index=-100, reduction="mean")
     x [..., D] and weight [V, D]: CUDA tensors of one dtype, float32, float16 or bfloat16;
     target [...]: int64 class indices with x's leading shape.  reduction: "mean" (over the
     tokens whose target is not ignore_index; NaN when there are none), "sum", or "none".
-    Returns the float32 loss: a scalar, or one value per token for "none".
+    Returns the float32 loss: a scalar, or one value per token for "none".  Gradients are
+    reverse-mode and of first order: forward-mode tangents are refused.
 
     Logits and their softmax are computed in fp32 and never kept: the forward pass keeps two
     floats per token, the backward pass computes the logits again a piece of the vocabulary
@@ -189,6 +200,7 @@ def linear_cross_entropy(x, weight, target, ignore_index=-100, reduction="mean")
                          f"{tuple(x.shape[:-1])}")
     if weight.shape[0] == 0 or weight.shape[1] == 0:
         raise ValueError(f"linear_cross_entropy: weight {tuple(weight.shape)} is empty")
+    _refuse_tangents("linear_cross_entropy", x, weight)
     if not (x.is_cuda and weight.device == x.device and target.device == x.device):
         raise ValueError(f"linear_cross_entropy: inputs must be CUDA tensors on one device (got {x.device}, "
                          f"{weight.device} and {target.device}); tilec_b200 has no CPU path")
@@ -381,7 +393,7 @@ def matrix_mul_w4(x, weight, bias=None, out=None):
     once to x's dtype and multiplied on the tensor cores: up to 256 rows of 16-bit x (and scales
     of its dtype) it is expanded on the way, otherwise into the workspace, at most 256 MiB (or
     256 rows of it) at a time (float32: exact, and the 3xTF32 product of matrix_mul).  Not
-    differentiable."""
+    differentiable: inputs that require a gradient or carry a forward-mode tangent are refused."""
     if not isinstance(weight, W4Weight):
         raise TypeError(f"matrix_mul_w4: weight must be a W4Weight (pack_w4, quantize_w4), got {type(weight).__name__}")
     n, k = weight.shape
@@ -391,6 +403,7 @@ def matrix_mul_w4(x, weight, bias=None, out=None):
     dt = _DTYPES.get(x.dtype)
     if dt is None:
         raise TypeError(f"matrix_mul_w4: x must be float32, float16 or bfloat16, got {x.dtype}")
+    _refuse_tangents("matrix_mul_w4", x, bias, out)
     dev = x.device
     if not (x.is_cuda and weight.device == dev):
         raise ValueError(f"matrix_mul_w4: x and weight must be on one CUDA device (got {dev} and {weight.device}); "
