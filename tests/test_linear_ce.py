@@ -567,3 +567,48 @@ def test_refuses_forward_mode_tangents(grad):
                     ext.linear_cross_entropy(a, b, y)
         with pytest.raises(ValueError, match="CUDA"):   # no tangent: on to the next check
             ext.linear_cross_entropy(x, w, y)
+
+
+@gpu
+@pytest.mark.parametrize("t,v,d,dtype,ignored,reduction", [
+    (1001, 3011, 777, "f16", 0.1, "mean"),      # odd everywhere, dW in slices or padded rows
+    (1001, 3011, 777, "bf16", 0.97, "none"),
+    (4096, 5000, 512, "bf16", 0.6, "sum"),      # most tokens have no target: few live rows of many
+    (4096, 5000, 512, "f16", 0.999, "mean"),
+    (2048, 300, 264, "bf16", 0.5, "mean"),      # long sums over tokens
+    (300, 20000, 136, "f16", 0.3, "sum"),       # long sums over the vocabulary
+    (2048, 9001, 100, "f32", 0.6, "mean")])
+def test_masked_and_ragged_training(t, v, d, dtype, ignored, reduction):
+    x, w, y = _make(t, v, d, dtype, seed=t + v, ignored=ignored)
+    go = None
+    if reduction == "none":
+        go = (torch.rand(t, generator=torch.Generator().manual_seed(4)) + 0.5).cuda()
+    _check(x, w, y, dtype, reduction, go)
+
+
+@gpu
+@pytest.mark.parametrize("dtype,t,d", [("bf16", 40000, 41), ("f16", 40000, 41), ("f32", 20000, 25)])
+def test_several_pieces_of_an_odd_width(dtype, t, d):
+    """Pieces of the vocabulary with gradients whose rows are no whole 16-byte pieces; every other
+    row frozen out by ignore_index, dx and dW asked for apart give what they give together."""
+    v = 9000
+    x, w, y = _make(t, v, d, dtype, ignored=0.5)
+    xg, wg = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    loss = ext.linear_cross_entropy(xg, wg, y)
+    dx, dw = torch.autograd.grad(loss, (xg, wg))
+    live = (y != IGNORE).nonzero()[:, 0]
+    n, w64 = len(live), w.double()
+    dw64, dx64 = torch.zeros_like(w64), torch.zeros(t, d, dtype=torch.float64, device="cuda")
+    for r in live.split(4000):
+        p = torch.softmax(x[r].double() @ w64.t(), 1)
+        p[torch.arange(len(r)), y[r]] -= 1
+        p /= n
+        dw64 += p.t() @ x[r].double()
+        dx64[r] = p @ w64
+    # fp16: gradients are of the order of 1 / n, some below 2^-14, where a step is 2^-24 whatever their size
+    for got, ref in ((dx, dx64), (dw, dw64)):
+        sub = 2.0 ** -25 * math.sqrt(ref.numel()) / ref.norm().item() if dtype == "f16" else 0.0
+        assert _rel(got, ref.cpu()) <= 2.5 * U[dtype] + 3e-5 + sub
+    assert (dx[y == IGNORE] == 0).all()
+    assert torch.equal(torch.autograd.grad(ext.linear_cross_entropy(xg, w, y), xg)[0], dx)
+    assert torch.equal(torch.autograd.grad(ext.linear_cross_entropy(x, wg, y), wg)[0], dw)

@@ -593,3 +593,68 @@ def test_refuses_forward_mode_tangents():
                 ext.matrix_mul_w4(*args)
         with pytest.raises(ValueError, match="CUDA"):
             ext.matrix_mul_w4(x, w, b, out)
+
+
+# (rows, N, K, group, type of x, type of scales).  From 2368 rows of the weight on a CTA has a row
+# tile of its own and takes all of K, so that several rows of a long x come in slabs.
+LONG = [(8, 2500, 14336, 128, "bf16", "bf16"), (8, 2401, 28672, 64, "f16", "f16"),    # 16-bit x in slabs
+        (16, 2500, 8192, 128, "bf16", "f32"), (13, 2400, 11008, 32, "f16", "bf16"),
+        (9, 2370, 4224, 64, "bf16", "f16"), (13, 8192, 8192, 128, "bf16", "bf16"),
+        (1, 2500, 40000, 128, "f32", "f32"), (2, 2500, 30000, 32, "f32", "f32"),      # digits in slabs
+        (3, 2500, 11008, 128, "f32", "f32"), (8, 2400, 8192, 64, "f32", "bf16"),
+        (2, 9000, 16000, 64, "f16", "f16"), (1, 300, 60000, 256, "bf16", "bf16"),
+        (8, 40005, 300, 128, "bf16", "bf16"), (1, 40005, 400, 64, "f16", "f16"),      # many row tiles
+        (5, 70001, 160, 32, "f32", "f32"), (16, 40005, 2700, 64, "f16", "f32"),
+        (17, 2500, 28672, 128, "bf16", "bf16"), (200, 1000, 14336, 64, "f16", "f16"),  # tcgen05
+        (40, 500, 20000, 128, "bf16", "f16"), (20, 500, 20000, 128, "f32", "f32")]
+
+
+@gpu
+@pytest.mark.parametrize("m,n,k,group,dtype,sdtype", LONG)
+def test_long_x_and_many_row_tiles(m, n, k, group, dtype, sdtype):
+    """More of K than the shared copy of x holds at once, and more row tiles than a CTA sums at once;
+    x in rows of a wider tensor, on and off 16-byte boundaries, gives the same bits."""
+    x, codes, scales, zeros, bias = _make(m, n, k, group, dtype, bias=True, sdtype=sdtype)
+    x, codes, scales, zeros, bias = (t.cuda() for t in (x, codes, scales, zeros, bias))
+    w = ext.pack_w4(codes, scales, zeros, group)
+    w64 = _weight64(codes, scales, zeros, group)
+    y = x.double() @ w64.t()
+    if m <= 8 or (m <= 16 and dtype != "f32" and sdtype != dtype):
+        tol = _long_bound(x, w64, y, dtype, k, group)
+    else:   # the weight rounded to x's type; sums of 16 (fp32: 8, three products), 2^-23 off each at worst
+        s = x.double().abs() @ w64.abs().t()
+        rel = 3 * -(-k // 8) * 2.0 ** -23 + 3 * 2.0 ** -20 if dtype == "f32" else -(-k // 16) * 2.0 ** -23 + U[dtype]
+        tol = rel * s + 1.001 * U[dtype] * y.abs() + (2.0 ** -25 if dtype == "f16" else 0.0)
+    y = y + bias.double()
+    tol = tol + U[dtype] * y.abs() + 2.0 ** -23 * bias.double().abs()
+    got = ext.matrix_mul_w4(x, w, bias)
+    err = (got.double() - y).abs()
+    assert torch.isfinite(got).all()
+    assert (err <= tol).all(), f"worst {(err / tol).max():.2f} of the bound"
+    for off in (0, 1, 8):
+        wide = torch.full((m, k + 24), float("nan"), dtype=x.dtype, device="cuda")
+        wide[:, off:off + k] = x
+        view = wide[:, off:off + k]
+        if dtype == "f32" and m > 8:   # the fp32 product picks its kernel by alignment
+            assert ((ext.matrix_mul_w4(view, w, bias).double() - y).abs() <= tol).all()
+        else:
+            assert torch.equal(ext.matrix_mul_w4(view, w, bias), got)
+    assert torch.equal(ext.matrix_mul_w4(x, w, bias), got)
+    ext.check_device()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("m", [1, 2, 5, 8])
+def test_outliers_that_meet_no_weight(m, dtype):
+    """x in digits is held to 2^-30 of its block's largest magnitude, whatever weight that meets:
+    one element of each block is up to 2^20 times the others and its codes are the zero point, so
+    that only what is held of the others counts."""
+    x, codes, scales, zeros, _ = _make(m, 500, 1000, 128, dtype)
+    x[:, 5::128] *= torch.tensor([2.0 ** 14, 2.0 ** 20, 1.0, 2.0 ** 8] * 2)[:len(x[0, 5::128])].to(x.dtype).clamp(
+        max=2.0 ** 12 if dtype == "f16" else 2.0 ** 20)
+    codes[:, 5::128] = zeros[:, :codes[:, 5::128].shape[1]]
+    w64 = _weight64(codes, scales, zeros, 128).cuda()
+    y = x.cuda().double() @ w64.t()
+    got = ext.matrix_mul_w4(x.cuda(), ext.pack_w4(codes, scales, zeros, 128).to("cuda"))
+    assert ((got.double() - y).abs() <= _long_bound(x.cuda(), w64, y, dtype, 1000, 128)).all()
