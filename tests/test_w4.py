@@ -658,3 +658,42 @@ def test_outliers_that_meet_no_weight(m, dtype):
     y = x.cuda().double() @ w64.t()
     got = ext.matrix_mul_w4(x.cuda(), ext.pack_w4(codes, scales, zeros, 128).to("cuda"))
     assert ((got.double() - y).abs() <= _long_bound(x.cuda(), w64, y, dtype, 1000, 128)).all()
+
+
+@gpu
+@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("m,dtype,top", [(1, "f32", 2.0 ** 13), (1, "f32", 2.0 ** 24), (2, "f32", 2.0 ** 20),
+                                         (3, "f32", 2.0 ** 24), (5, "f32", 2.0 ** 40), (8, "f32", 2.0 ** 20),
+                                         (8, "f32", 2.0 ** 100), (1, "bf16", 2.0 ** 15), (1, "f16", 2.0 ** 5),
+                                         (2, "bf16", 2.0 ** 100), (8, "f16", 2.0 ** 12)])
+def test_large_elements_cost_the_others_no_digits(m, dtype, top, group):
+    """Each block of x has an element of `top` times the others' size whose codes are the zero point.
+    The bound is relative to sum |x w|, in which it does not appear: every element of x counts with
+    all its bits (fp32), or all that its output keeps."""
+    x, codes, scales, zeros, _ = _make(m, 300, 2500, group, dtype)
+    x[:, 7::32] = top
+    codes[:, 7::32] = zeros.repeat_interleave(group // 32, 1)[:, :codes[:, 7::32].shape[1]]
+    x, codes, scales, zeros = (t.cuda() for t in (x, codes, scales, zeros))
+    w64 = _weight64(codes, scales, zeros, group)
+    y = x.double() @ w64.t()
+    got = ext.matrix_mul_w4(x, ext.pack_w4(codes, scales, zeros, group))
+    s = x.double().abs() @ w64.abs().t()
+    tol = ((-(-2500 // min(group, 128)) + 40) * 2.0 ** -24 + 2.0 ** -19) * s + 1.001 * U[dtype] * y.abs() + (
+        2.0 ** -25 if dtype == "f16" else 0.0)
+    assert ((got.double() - y).abs() <= tol).all(), f"{((got.double() - y).abs() / tol).max():.1f} of the bound"
+
+
+def _huge(m, dtype, sdtype=None):
+    """One element of x near the type's largest per row and block; with its weight the result is far
+    from it, but codes times x, before the scale, are past fp32."""
+    x, codes, scales, zeros, _ = _make(m, 150, 384, 64, dtype, sdtype=sdtype)
+    x[:, 70::128] = 0.99 * torch.finfo(DT[dtype]).max * (torch.arange(m)[:, None] % 2 * 2 - 1)
+    x[:, 71::128] = -x[:, 70::128] / 2
+    return x, codes, (scales / 64).to(scales.dtype), zeros
+
+
+@gpu
+@pytest.mark.parametrize("m", [1, 2, 3, 8])
+def test_huge_fp32_x_overflows_no_sum(m):
+    x, codes, scales, zeros = _huge(m, "f32")
+    _check(x, codes, scales, zeros, None, 64, "f32")

@@ -41,18 +41,14 @@ int lm_device(DeviceInfo** d, LmInfo** lm) {
     auto w4_attrs = [&](auto gpb, auto wide) {
       constexpr int G = decltype(gpb)::value;
       constexpr bool W = decltype(wide)::value;
-      auto stream = [&](auto sc) {
-        constexpr int C = decltype(sc)::value;
-        w4_attr(w4_stream_kernel<1, G, C, 0>);
-        w4_attr(w4_stream_kernel<2, G, C, 0>);
-        w4_attr(w4_stream_kernel<4, G, C, 0>);
-      };
       if constexpr (W) {
-        stream(std::integral_constant<int, TILEC_DTYPE_F32>{});
+        w4_attr(w4_stream_kernel<1, G, TILEC_DTYPE_F32, 0>);
       } else {
-        stream(std::integral_constant<int, TILEC_DTYPE_F16>{});
-        stream(std::integral_constant<int, TILEC_DTYPE_BF16>{});
+        w4_attr(w4_stream_kernel<1, G, TILEC_DTYPE_F16, 0>);
+        w4_attr(w4_stream_kernel<1, G, TILEC_DTYPE_BF16, 0>);
       }
+      w4_attr(w4_stream_kernel<1, G, W ? 0 : 1, kW4Terms>);
+      w4_attr(w4_stream_kernel<3, G, W ? 0 : 1, kW4Terms>);
       w4_attr(w4_stream_kernel<1, G, W ? 0 : 1, TILEC_DTYPE_F16>);
       w4_attr(w4_stream_kernel<1, G, W ? 0 : 1, TILEC_DTYPE_BF16>);
       w4_attr(w4_stream_kernel<2, G, W ? 0 : 1, TILEC_DTYPE_F16>);
@@ -582,22 +578,19 @@ int64_t w4_stream_fixed_nt(int gpb, bool wide) {
          : gpb == 2 ? (wide ? W4StreamCfg<NT, 2, true, XT>::kFixed : W4StreamCfg<NT, 2, false, XT>::kFixed)
                     : (wide ? W4StreamCfg<NT, 1, true, XT>::kFixed : W4StreamCfg<NT, 1, false, XT>::kFixed);
 }
-int64_t w4_stream_fixed(int nt, int gpb, bool wide, bool x16) {
-  if (x16) return nt == 1 ? w4_stream_fixed_nt<1, 1>(gpb, wide) : w4_stream_fixed_nt<2, 1>(gpb, wide);
-  return nt == 1   ? w4_stream_fixed_nt<1, 0>(gpb, wide)
-         : nt == 2 ? w4_stream_fixed_nt<2, 0>(gpb, wide)
-                   : w4_stream_fixed_nt<4, 0>(gpb, wide);
+int64_t w4_stream_fixed(int nt, int gpb, bool wide, int xt) {
+  if (xt == 0) return w4_stream_fixed_nt<1, 0>(gpb, wide);
+  if (xt == kW4Terms) return nt == 1 ? w4_stream_fixed_nt<1, kW4Terms>(gpb, wide) : w4_stream_fixed_nt<3, kW4Terms>(gpb, wide);
+  return nt == 1 ? w4_stream_fixed_nt<1, TILEC_DTYPE_BF16>(gpb, wide) : w4_stream_fixed_nt<2, TILEC_DTYPE_BF16>(gpb, wide);
 }
 
 struct W4Plan {
   bool stream = false;   // w4_stream_kernel
-  bool x16 = false;      // ... with x in 16-bit values, not digits
+  int xt = 0;            // ... how x enters it: digits, its 16-bit type or three terms
   bool tc = false;       // w4_tc_kernel; otherwise expanded weights and a plain product
   bool pack_x = false;   // x is copied to aligned rows first (expanded weights)
-  int nt = 1, splits = 1, slab = 1, per_cta = 0, ctas = 0;
-  bool cut_before = false;
+  int nt = 1, cols = 1, splits = 1, slab = 1, per_cta = 0, ctas = 0;
   bool polling = false;  // w4_stream_kernel's waits, see W4StreamArgs
-  size_t off_digits = 0, off_sums = 0, off_scale = 0;
   int64_t blocks = 0, kp = 0, piece = 0;
   int slices = 1, kb = 0;
   int64_t ldslab = 0;
@@ -624,14 +617,15 @@ int check_w4_pointers(const W4Call& c) {
   return TILEC_OK;
 }
 
-// How many rows of x run where: one (fp32: up to 8) in digits on w4_stream_kernel; up to 16 of
-// 16-bit x there too, as they are, but for two against a large weight (4096 x 4096: 7.4 us, in
-// digits 9.5; 8192 x 8192: 15.6 and 19.4; 28672 x 8192: 36.7 and 33.0); up to 256 of 16-bit x
+// How many rows of x run where: one of 16-bit x in digits on w4_stream_kernel; up to 16 there too,
+// as they are, but for two against a large weight (4096 x 4096: 7.4 us, in
+// digits 9.5; 8192 x 8192: 15.6 and 19.4; 28672 x 8192: 36.7 and 33.0); up to 8 of fp32 x there
+// as well, in three bf16 terms (three columns a row, which NT = 3 tiles of 8 hold); up to 256 of 16-bit x
 // whose type the scales share on w4_tc_kernel, 128 at a time (8192 x 8192: 128 rows 35 to 39 us,
 // twice that for 256; expanded first, either takes 89); for the rest W is expanded once into the
 // workspace and multiplied on the tcgen05 kernels (fp32: 3xTF32).
-constexpr int64_t kW4MaxCols = 32;  // of digits
 constexpr int64_t kW4Max16 = 16;    // rows of 16-bit x
+constexpr int64_t kW4Max32 = 8;     // rows of fp32 x
 
 void plan_w4(const W4Call& c, const DeviceInfo& d, const LmInfo& lm, W4Plan* p) {
   const bool f32 = c.dtype == TILEC_DTYPE_F32;
@@ -645,7 +639,7 @@ void plan_w4(const W4Call& c, const DeviceInfo& d, const LmInfo& lm, W4Plan* p) 
   };
   const int gpb = c.group == 32 ? 4 : c.group == 64 ? 2 : 1;
   const bool wide = c.sdt == TILEC_DTYPE_F32, two = c.M == 2 && c.N * p->kp >= int64_t(1) << 27;
-  const bool digits = f32 ? c.M * kW4Digits <= kW4MaxCols : c.M == 1 || two;
+  const bool digits = !f32 && (c.M == 1 || two), terms = f32 && c.M <= kW4Max32;
   // Nine to 16 rows: each further slab of x costs w4_stream_kernel some 6 us, w4_tc_kernel is the
   // slower the larger the weight (4096 x 4096, 16 rows in two slabs: 18.0 against 11.3 us;
   // 8192 x 8192, 13 in two: 22.8 against 25.6, 16 in three: 28.0 against 25.6; 28672 x 8192, 16
@@ -653,16 +647,15 @@ void plan_w4(const W4Call& c, const DeviceInfo& d, const LmInfo& lm, W4Plan* p) 
   bool in16 = !f32 && c.M <= kW4Max16;
   if (in16 && c.M > 8 && c.sdt == c.dtype) {
     const int64_t slabs =
-        cdiv(w4_slab16_bytes(p->blocks, c.M), kW4MaxSmem - w4_stream_fixed(2, gpb, wide, true));
+        cdiv(w4_slab16_bytes(p->blocks, c.M), kW4MaxSmem - w4_stream_fixed(2, gpb, wide, c.dtype));
     in16 = c.N * p->kp >= (slabs - 1) << 26;
   }
-  if (digits || in16) {
+  if (digits || in16 || terms) {
     p->stream = true;
     p->polling = d.short_waits;
-    p->x16 = !digits;
-    const int cols = static_cast<int>(p->x16 ? c.M : c.M * kW4Digits);
-    p->nt = cols <= 8 ? 1 : cols <= 16 ? 2 : 4;
-    const int pad = 8 * p->nt;
+    p->xt = digits ? 0 : terms ? kW4Terms : c.dtype;
+    p->cols = static_cast<int>(c.M * (digits ? kW4Digits : terms ? kW4Terms : 1));
+    p->nt = terms ? (c.M <= 2 ? 1 : 3) : p->cols <= 8 ? 1 : 2;
     // One CTA per SM.  With fewer 16-row tiles than SMs, a cluster of CTAs shares each tile's K.
     const int64_t tiles = cdiv(c.N, 16);
     int64_t splits = d.sms / tiles;
@@ -673,19 +666,11 @@ void plan_w4(const W4Call& c, const DeviceInfo& d, const LmInfo& lm, W4Plan* p) 
     p->splits = static_cast<int>(cdiv(p->blocks, p->per_cta));
     const int64_t clusters = d.sms / p->splits;
     p->ctas = static_cast<int>((tiles < clusters ? tiles : clusters) * p->splits);
-    // Two rows are cut in every CTA (a round of some 150 instructions per row and 48 blocks),
-    // more once for all.
-    p->cut_before = !p->x16 && c.M > 2;
-    const int64_t room = kW4MaxSmem - w4_stream_fixed(p->nt, gpb, wide, p->x16);
-    auto slab_bytes = [&](int64_t n) { return p->x16 ? w4_slab16_bytes(n, c.M) : w4_slab_bytes(n, cols, pad, gpb); };
+    const int64_t room = kW4MaxSmem - w4_stream_fixed(p->nt, gpb, wide, p->xt);
+    auto slab_bytes = [&](int64_t n) { return digits ? w4_slab_bytes(n, p->cols, gpb) : w4_slab16_bytes(n, p->cols); };
     int64_t slab = p->per_cta;
     while (slab > 1 && slab_bytes(slab) > room) --slab;
     p->slab = static_cast<int>(cdiv(p->per_cta, cdiv(p->per_cta, slab)));  // slabs of one size
-    if (p->cut_before) {
-      p->off_digits = take(size_t(cols) * p->blocks * kW4Block);
-      p->off_sums = take(size_t(p->blocks) * gpb * pad * 4);
-      p->off_scale = take(size_t(p->blocks) * pad * 4);
-    }
   } else if (!f32 && c.M <= 2 * W4TcCfg<1>::kMaxCols && c.sdt == c.dtype) {
     p->tc = true;
     p->pack_x = !rows_aligned16(c.x, c.ldx);
@@ -734,58 +719,45 @@ void plan_w4(const W4Call& c, const DeviceInfo& d, const LmInfo& lm, W4Plan* p) 
 }
 
 template <int NT, int GPB, int SC, int XT>
-int launch_w4_stream(const W4Args& w, const W4Plan& p, uint8_t* ws, cudaStream_t s) {
+int launch_w4_stream(const W4Args& w, const W4Plan& p, cudaStream_t s) {
   W4StreamArgs a;
   a.w = w;
-  a.d.digits = p.cut_before ? ws + p.off_digits : nullptr;
-  a.d.pitch = p.blocks * kW4Block;
-  a.d.sums = reinterpret_cast<int*>(ws + p.off_sums);
-  a.d.scale = reinterpret_cast<float*>(ws + p.off_scale);
-  a.d.cols_pad = 8 * NT;
-  a.d.gpb = GPB;
   a.row_tiles = static_cast<int>(cdiv(w.N, 16));
   a.per_cta = p.per_cta;
   a.slab = p.slab;
   a.polling = p.polling;
   using Cfg = W4StreamCfg<NT, GPB, SC == 0, XT>;
-  const size_t smem = size_t(Cfg::kFixed + (XT != 0 ? w4_slab16_bytes(p.slab, w.M) : w4_slab_bytes(p.slab, w.cols, 8 * NT, GPB)));
+  const size_t smem =
+      size_t(Cfg::kFixed + (XT != 0 ? w4_slab16_bytes(p.slab, w.cols) : w4_slab_bytes(p.slab, w.cols, GPB)));
   if (int64_t(smem) > kW4MaxSmem) return TILEC_ERR_UNSUPPORTED;
-  if (p.cut_before)
-    TILEC_TRY(launch_k(w4_digits_kernel, dim3(static_cast<unsigned>(cdiv(int64_t(w.M) * p.blocks, 8))), dim3(128), 0, s,
-                       1, w, a.d, static_cast<int>(p.blocks)));
   return launch_k(w4_stream_kernel<NT, GPB, SC, XT>, dim3(static_cast<unsigned>(p.ctas)), dim3(Cfg::kThreads), smem, s,
                   w.splits, a);
 }
 
 // The kernel's variants: by columns, groups per block, type of x and scales.
 template <int GPB, bool WIDE>
-int launch_w4(const W4Args& a, const W4Plan& p, uint8_t* ws, cudaStream_t s) {
-  if (p.x16) {
-    auto by_type = [&](auto nt) {
-      constexpr int NT = decltype(nt)::value;
-      return a.dtype == TILEC_DTYPE_BF16 ? launch_w4_stream<NT, GPB, WIDE ? 0 : 1, TILEC_DTYPE_BF16>(a, p, ws, s)
-                                         : launch_w4_stream<NT, GPB, WIDE ? 0 : 1, TILEC_DTYPE_F16>(a, p, ws, s);
-    };
-    return p.nt == 1 ? by_type(std::integral_constant<int, 1>{}) : by_type(std::integral_constant<int, 2>{});
-  }
-  auto by_columns = [&](auto sc) {
-    constexpr int SC = decltype(sc)::value;
-    return p.nt == 1   ? launch_w4_stream<1, GPB, SC, 0>(a, p, ws, s)
-           : p.nt == 2 ? launch_w4_stream<2, GPB, SC, 0>(a, p, ws, s)
-                       : launch_w4_stream<4, GPB, SC, 0>(a, p, ws, s);
-  };
+int launch_w4(const W4Args& a, const W4Plan& p, cudaStream_t s) {
+  constexpr int SC = WIDE ? 0 : 1;
+  if (p.xt == kW4Terms)
+    return p.nt == 1 ? launch_w4_stream<1, GPB, SC, kW4Terms>(a, p, s) : launch_w4_stream<3, GPB, SC, kW4Terms>(a, p, s);
+  if (p.xt == TILEC_DTYPE_BF16)
+    return p.nt == 1 ? launch_w4_stream<1, GPB, SC, TILEC_DTYPE_BF16>(a, p, s)
+                     : launch_w4_stream<2, GPB, SC, TILEC_DTYPE_BF16>(a, p, s);
+  if (p.xt == TILEC_DTYPE_F16)
+    return p.nt == 1 ? launch_w4_stream<1, GPB, SC, TILEC_DTYPE_F16>(a, p, s)
+                     : launch_w4_stream<2, GPB, SC, TILEC_DTYPE_F16>(a, p, s);
   if constexpr (WIDE)
-    return by_columns(std::integral_constant<int, TILEC_DTYPE_F32>{});
+    return launch_w4_stream<1, GPB, TILEC_DTYPE_F32, 0>(a, p, s);
   else
-    return a.scale_bf16 ? by_columns(std::integral_constant<int, TILEC_DTYPE_BF16>{})
-                        : by_columns(std::integral_constant<int, TILEC_DTYPE_F16>{});
+    return a.scale_bf16 ? launch_w4_stream<1, GPB, TILEC_DTYPE_BF16, 0>(a, p, s)
+                        : launch_w4_stream<1, GPB, TILEC_DTYPE_F16, 0>(a, p, s);
 }
 
 template <bool WIDE>
-int launch_w4(const W4Args& a, const W4Plan& p, int gpb, uint8_t* ws, cudaStream_t s) {
-  return gpb == 4   ? launch_w4<4, WIDE>(a, p, ws, s)
-         : gpb == 2 ? launch_w4<2, WIDE>(a, p, ws, s)
-                    : launch_w4<1, WIDE>(a, p, ws, s);
+int launch_w4(const W4Args& a, const W4Plan& p, int gpb, cudaStream_t s) {
+  return gpb == 4   ? launch_w4<4, WIDE>(a, p, s)
+         : gpb == 2 ? launch_w4<2, WIDE>(a, p, s)
+                    : launch_w4<1, WIDE>(a, p, s);
 }
 
 template <bool BF16, int GPB>
@@ -863,14 +835,14 @@ int run_w4(const W4Call& c, void* workspace, size_t ws_bytes, cudaStream_t s) {
     a.ldx = c.ldx;
     a.dtype = c.dtype;
     a.M = static_cast<int>(c.M);
-    a.cols = static_cast<int>(c.M * (p.stream && !p.x16 ? kW4Digits : 1));
-    a.vec_x = !f32 && rows_aligned16(c.x, c.ldx);
+    a.cols = p.cols;
+    a.vec_x = aligned16(c.x) && c.ldx % (f32 ? 4 : 8) == 0;
     a.out = c.out;
     a.ldo = c.ldo;
     a.bias = c.bias;
     a.splits = p.splits;
     if (p.tc) return run_w4_tc(c, p, a, gpb, ws, *d, s);
-    return a.wide ? launch_w4<true>(a, p, gpb, ws, s) : launch_w4<false>(a, p, gpb, ws, s);
+    return a.wide ? launch_w4<true>(a, p, gpb, s) : launch_w4<false>(a, p, gpb, s);
   }
   const void* x = c.x;
   int64_t ldx = c.ldx;

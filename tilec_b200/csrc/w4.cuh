@@ -39,7 +39,7 @@ struct W4Args {
   const void* x;           // [M][ldx] of type dtype
   int64_t ldx;
   int dtype;               // TILEC_DTYPE_* of x, bias and out
-  int M, cols;             // cols: M, or M times the digits of w4_stream_kernel
+  int M, cols;             // cols: M, or M times the digits or terms of w4_stream_kernel
   int vec_x;               // 16-byte loads of x allowed (16-bit types)
   void* out;               // [M][ldo]
   int64_t ldo;

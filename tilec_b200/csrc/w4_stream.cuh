@@ -1,21 +1,26 @@
-// w4_stream.cuh -- the few-rows product with 4-bit weights on mma.sync: one row of x (fp32:
-// up to 8; two of a large weight) on the integer path, up to 16 rows of 16-bit x on the 16-bit one.
+// w4_stream.cuh -- the few-rows product with 4-bit weights on mma.sync: one row of 16-bit x (two of
+// a large weight) on the integer path, up to 16 rows of 16-bit x and up to 8 of fp32 x on the
+// 16-bit one.
 //
 // One token's product reads N * K / 2 bytes of codes and is bound by memory, if only the
 // arithmetic keeps up: at 6.5 TB/s a quarter SM has about 180 cycles per 1 KB of codes (16
 // rows x 128 k).  As 16-bit floats (multiply16: 0x4300 | code is 128 + code in bf16, 0x6400 |
 // code is 1024 + code in fp16, minus 128 + zero; products are exact, sums fp32, the scale
 // multiplies a group's sum) a code costs 1.4 instructions, most of them on the half-rate integer
-// pipe.  An 8-bit operand (multiply8) needs 3 for 8 codes, and m16n8k32 takes twice the k at the
+// pipe.  fp32 x enters as three bf16 numbers of 8 bits each, which hold all of its 24 (w4_stage32):
+// three columns of the product to a row of x.
+// An 8-bit operand (multiply8) needs 3 for 8 codes, and m16n8k32 takes twice the k at the
 // same rate, for four columns per row of x:
 //
 //   * per 128-k block and row, x becomes whole numbers X = round(x * 2^(29 - e)), 2^e <= the
 //     block's largest magnitude < 2^(e + 1), in four signed 8-bit digits: x is off by at most
 //     2^-30 of 2^e, which is exact for 16-bit types wherever the magnitude is within 2^-22
-//     (bf16) or 2^-19 (fp16) of that, and below the rounding of an fp32 sum;
+//     (bf16) or 2^-19 (fp16) of that;
 //   * each digit is one column of the tensor-core product, so sums over a group are exact
 //     32-bit integers: sum code * X - zero * sum X;
 //   * that times scale * 2^(e - 29) * 256^digit is added in fp32.
+// (fp32 x in digits was as fast, but an element 2^-13 of its block's largest keeps 17 bits, which
+// shows where the largest meets the zero point: 4e-6 off where an fp32 product is 2e-7.)
 //
 // The sums start at 0x4B400000 - zero * sum X: read as a float that is 1.5 * 2^23 + the sum
 // (|sum| < 2^22), which saves the conversions.
@@ -26,18 +31,18 @@
 // copies of four pieces each (two where x needs the room), so that 140 (70) KB are on their way
 // to an SM at any time.  Where a
 // tile is shared by several warps their sums meet in shared memory, in the order of K.
+// Each CTA cuts, splits or copies x for itself (one row is a round of some 150 instructions per 32
+// blocks), a slab of K at a time where it does not fit.
 //
-// x is cut by the CTAs themselves where that is little work (one or two rows), otherwise once,
-// by w4_digits_kernel; w4_stream_kernel then starts its first copies of the weight while x is
-// still being cut: it is launched with programmatic serialisation, and w4_digits_kernel lets
-// it go only after everything before has completed.
-//
-// Measured, 28672 x 8192, one token (125 MB): 27.8 us, 4.5 TB/s; loads alone take 25 in the
-// best of the forms tried.  On the way: rows of codes with the group words apart 35 to 40 us
+// Measured (graph replay), 28672 x 8192, one token (125 MB): 24.7 us, 5.0 TB/s.  On the way, with
+// 27.8 as the best then: rows of codes with the group words apart 35 to 40 us
 // (the words alone cost 6); 24 warps with copies of two pieces 30.5; 12 warps 30.3; CTAs of
-// 128 rows, two waves of them for want of one slot, 40.  8 rows: 34.8 us (a grid of small CTAs
-// with cp.async rings 48), 16 rows, x in three slabs: 52.
+// 128 rows, two waves of them for want of one slot, 40.  8 rows: 33.0 us (a grid of small CTAs
+// with cp.async rings 48), 16 rows, x in three slabs: 50.4.  fp32: one row 32.4, 8 rows of 8192 x
+// 8192 34.0 (in digits 28.3 and 34.4).
 #pragma once
+
+#include <cfloat>
 
 #include "tc2_f16.cuh"
 #include "w4.cuh"
@@ -48,26 +53,27 @@ constexpr int kW4StreamWarps = 16;
 constexpr int kW4Digits = 4;      // columns per row of x
 constexpr int kW4GroupTiles = 16; // row tiles whose sums a CTA holds at a time
 
-// The digits of x, in the workspace or (same layout) in shared memory; zeros past K.
+// The digits of x in shared memory; zeros past K.
 struct W4Digits {
   uint8_t* digits;   // [col][pitch], 128 bytes a block, [t][j][8]: 8 consecutive k in the order 0 4 1 5 2 6 3 7
   int64_t pitch;
-  int* sums;         // [block][group][8 NT]: minus the sum of a column's digits over a group
-  float* scale;      // [block][8 NT]: 2^(e - 29) * 256^digit
-  int cols_pad;      // 8 NT; columns are 4 * row + digit, the smallest first
+  int* sums;         // [block][group][8]: minus the sum of a column's digits over a group
+  float* scale;      // [block][8]: 2^(e - 29) * 256^digit; columns are 4 * row + digit, the smallest first
   int gpb;           // groups per block
 };
 
 struct W4StreamArgs {
-  W4Args w;          // the weight, x (to be cut, and for outputs that are not finite), bias and out
-  W4Digits d;        // workspace; digits == nullptr: the CTAs cut x themselves
+  W4Args w;          // the weight, x, bias and out
   int row_tiles;
   int per_cta;       // blocks of K a CTA takes; a cluster's CTAs follow one another along K
   int slab;          // blocks of x in shared memory at a time
   int polling;       // the device's wait limit is shortened (w4_wait_on)
 };
 
-// XT: how x enters: 0 in digits, else as 16-bit values of that TILEC_DTYPE_*.
+// XT: how x enters: 0 in digits (one or two 16-bit rows), TILEC_DTYPE_F16 or _BF16 as it is,
+// kW4Terms (fp32) in three bf16 terms.
+constexpr int kW4Terms = 3;
+
 template <int NT, int GPB, bool WIDE, int XT>
 struct W4StreamCfg {
   static constexpr int kThreads = 32 * kW4StreamWarps;
@@ -78,7 +84,14 @@ struct W4StreamCfg {
   static constexpr int kStage = kRun * kPiece;
   static constexpr int kStages = 2;
   static constexpr int kRingBytes = kW4StreamWarps * kStages * kStage;
-  static constexpr int kPart = (XT == 0 ? 2 : 8) * NT * 16;  // floats: the sums of a row tile, [row of x][16]
+  static constexpr bool kSummed = XT == 0 || XT == kW4Terms;  // several columns to a row of x
+  static_assert(!(XT == 0 && NT != 1) && !(XT == kW4Terms && NT != 1 && NT != 3), "columns of several to a row");
+  static constexpr int kRows = kSummed && NT == 1 ? 2 : kSummed ? 8 : 8 * NT;  // rows of x
+  static constexpr int kPart = kRows * 16;  // floats: the sums of a row tile, [row of x][16]
+  // Chains of MMAs per group and column: one of eight dependent MMAs is what a warp would wait for
+  // (28672 x 8192, 8 rows: 38.9 us, in two parts 34.8, in four 37.7); three tiles of columns are
+  // three chains already.
+  static constexpr int kChains = NT == 3 ? 1 : 2;
   static constexpr int kSumBytes = kW4GroupTiles * kPart * 4;
   static constexpr int kPartBytes = 2 * kW4StreamWarps * kPart * 4;
   static constexpr int kBarBytes = 1024;     // a barrier per warp and stage, the abort flag
@@ -86,10 +99,10 @@ struct W4StreamCfg {
   static_assert(kStage % 128 == 0 && (kW4StreamWarps * kStages + 1) * 8 <= kBarBytes, "shared memory layout");
 };
 // Bytes of `slab` blocks of x: digits (16 bytes more a column: conflict-free reads), sums, scales.
-__host__ __device__ inline int64_t w4_slab_bytes(int64_t slab, int cols, int cols_pad, int gpb) {
-  return cols * (slab * kW4Block + 16) + slab * cols_pad * 4 * (gpb + 1);
+__host__ __device__ inline int64_t w4_slab_bytes(int64_t slab, int cols, int gpb) {
+  return cols * (slab * kW4Block + 16) + slab * 8 * 4 * (gpb + 1);
 }
-// The same in 16-bit values (64 bytes more a row: conflict-free reads).
+// The same in 16-bit values (64 bytes more a row: conflict-free reads); fp32: three such rows.
 __host__ __device__ inline int64_t w4_slab16_bytes(int64_t slab, int64_t rows) {
   return rows * (slab * (2 * kW4Block) + 64);
 }
@@ -101,31 +114,25 @@ __device__ __forceinline__ void w4_cut(const W4Args& p, const W4Digits& d, bool 
   const int j = l >> 2, t = l & 3;
   const int k0 = blk * kW4Block + 8 * l;
   float v[8];
-  if (p.dtype == 0) {
-    const float* s = static_cast<const float*>(p.x) + m * p.ldx + k0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = live && k0 + i < p.K ? s[i] : 0.f;
+  const unsigned short* s = static_cast<const unsigned short*>(p.x) + m * p.ldx + k0;
+  uint32_t w[4] = {0, 0, 0, 0};
+  if (live && p.vec_x && k0 + 8 <= p.K) {
+    const uint4 h = *reinterpret_cast<const uint4*>(s);
+    w[0] = h.x; w[1] = h.y; w[2] = h.z; w[3] = h.w;
   } else {
-    const unsigned short* s = static_cast<const unsigned short*>(p.x) + m * p.ldx + k0;
-    uint32_t w[4] = {0, 0, 0, 0};
-    if (live && p.vec_x && k0 + 8 <= p.K) {
-      const uint4 h = *reinterpret_cast<const uint4*>(s);
-      w[0] = h.x; w[1] = h.y; w[2] = h.z; w[3] = h.w;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (live && k0 + i < p.K) w[i >> 1] |= uint32_t(s[i]) << (16 * (i & 1));
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (p.dtype == 2) {
+      v[2 * i] = __uint_as_float(w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
     } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (live && k0 + i < p.K) w[i >> 1] |= uint32_t(s[i]) << (16 * (i & 1));
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (p.dtype == 2) {
-        v[2 * i] = __uint_as_float(w[i] << 16);
-        v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
-      } else {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
-      }
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
     }
   }
   uint32_t top = 0;  // the largest magnitude, as bits: infinities and NaN come out on top
@@ -164,23 +171,14 @@ __device__ __forceinline__ void w4_cut(const W4Args& p, const W4Digits& d, bool 
     const int col = m * kW4Digits + part;
     *reinterpret_cast<uint2*>(d.digits + col * d.pitch + at * kW4Block + t * 32 + j * 8) = make_uint2(d0, d1);
     if (t == 0 && j % (4 / d.gpb) == 0)
-      d.sums[(at * d.gpb + j / (4 / d.gpb)) * d.cols_pad + col] = -sum;
-    if (l == 0) d.scale[at * d.cols_pad + col] = down * __uint_as_float(static_cast<uint32_t>(127 + 8 * part) << 23);
+      d.sums[(at * d.gpb + j / (4 / d.gpb)) * 8 + col] = -sum;
+    if (l == 0) d.scale[at * 8 + col] = down * __uint_as_float(static_cast<uint32_t>(127 + 8 * part) << 23);
   }
 }
 
-// Cuts all of x, 8 blocks a CTA.
-__global__ void __launch_bounds__(128) w4_digits_kernel(const __grid_constant__ W4Args p,
-                                                        const __grid_constant__ W4Digits d, int nblocks) {
-  pdl_wait();
-  pdl_launch_dependents();
-  const int task = static_cast<int>(blockIdx.x) * 8 + (threadIdx.x >> 4);
-  const bool live = task < p.M * nblocks;
-  const int m = live ? task / nblocks : 0, blk = live ? task - m * nblocks : 0;
-  w4_cut(p, d, live, m, blk, blk, threadIdx.x & 15);
-}
-
-// One output from its definition, in fp32 and k order.
+// One output from its definition, in fp32 and k order: where sums are not finite because x is not,
+// or because codes times an x of 2^117 or more are past fp32's range before the scale brings them
+// back.  Slow: some 0.5 to 5 ms for a weight's outputs.
 __device__ __noinline__ float w4_output(const W4Args& p, int gpb, int n, int m) {
   float v = 0.f;
   const int wb = w4_word_bytes(gpb, p.wide);
@@ -253,6 +251,44 @@ __device__ __forceinline__ void w4_stage16(const W4Args& p, uint8_t* xs, int pit
   cp_async_wait<0>();
 }
 
+// fp32 rows of x, blocks s0 .. s0 + n, as three bf16 numbers each: x = high + middle + low, 8 bits
+// of its 24 each, cut off and not rounded (nothing overflows, nothing is lost down to 2^-133).
+// [term][row][pitch], zeros past K.  Infinities and NaN are their own high term.
+__device__ __forceinline__ void w4_stage32(const W4Args& p, uint8_t* xs, int pitch, int s0, int n) {
+  const int per_row = n * (kW4Block / 8);
+  for (int i = threadIdx.x; i < p.M * per_row; i += 32 * kW4StreamWarps) {
+    const int m = i / per_row, c = i - m * per_row, k = s0 * kW4Block + 8 * c;
+    const float* s = static_cast<const float*>(p.x) + m * p.ldx + k;
+    float v[8];
+    if (p.vec_x && k + 8 <= p.K) {
+      const float4 a = reinterpret_cast<const float4*>(s)[0], b = reinterpret_cast<const float4*>(s)[1];
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = k + j < p.K ? s[j] : 0.f;
+    }
+#pragma unroll
+    for (int term = 0; term < kW4Terms; ++term) {
+      uint32_t h[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t bits = __float_as_uint(v[j]);
+        h[j] = bits & 0xFFFF0000u;
+        if ((bits & 0x7F800000u) == 0x7F800000u) {
+          if ((bits & 0x007FFFFFu) != 0) h[j] = 0x7FC00000u;  // a NaN whose high half may say infinity
+          v[j] = 0.f;
+        } else {
+          v[j] -= __uint_as_float(h[j]);
+        }
+      }
+      *reinterpret_cast<uint4*>(xs + (term * p.M + m) * pitch + 16 * c) =
+          make_uint4(__byte_perm(h[0], h[1], 0x7632), __byte_perm(h[2], h[3], 0x7632),
+                     __byte_perm(h[4], h[5], 0x7632), __byte_perm(h[6], h[7], 0x7632));
+    }
+  }
+}
+
 // What a warp does when a copy has not landed after one try (mbar_wait's loop, out of line).
 // `polling`: the device's limit is shortened (failure tests).  The suspending form of the test
 // sleeps for longer than a copy takes, so with it no limit below that would ever run out.
@@ -281,13 +317,14 @@ __device__ __noinline__ bool w4_wait_on(uint32_t bar, uint32_t parity, volatile 
   }
 }
 
-// SC: type of the scales (TILEC_DTYPE_*); with 16-bit x (XT != 0) 0, or 1 for either 16-bit type.
+// SC: type of the scales (TILEC_DTYPE_*); where x is not in digits (XT != 0) 0, or 1 for either 16-bit type.
 // Grid: x = CTAs (clusters of `splits`, whose CTAs share their row tiles and split K).
 template <int NT, int GPB, int SC, int XT>
 __global__ void __launch_bounds__(32 * kW4StreamWarps, 1) w4_stream_kernel(const __grid_constant__ W4StreamArgs a) {
   constexpr bool WIDE = SC == 0;
   using Cfg = W4StreamCfg<NT, GPB, WIDE, XT>;
-  constexpr int COLS = 8 * NT, WB = w4_word_bytes(GPB, WIDE), T = Cfg::kThreads, S = Cfg::kStages, W = kW4StreamWarps;
+  constexpr int WB = w4_word_bytes(GPB, WIDE), T = Cfg::kThreads, S = Cfg::kStages, W = kW4StreamWarps;
+  constexpr bool BF = XT == TILEC_DTYPE_BF16 || XT == kW4Terms;  // bf16 operands (where x is not in digits)
   extern __shared__ __align__(128) uint8_t w4_smem[];
   const W4Args& p = a.w;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -297,35 +334,41 @@ __global__ void __launch_bounds__(32 * kW4StreamWarps, 1) w4_stream_kernel(const
   uint64_t* bars = reinterpret_cast<uint64_t*>(w4_smem + Cfg::kFixed - Cfg::kBarBytes) + warp * S;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(w4_smem + Cfg::kFixed - 8);
   const int pitch = XT == 0 ? a.slab * kW4Block + 16 : a.slab * (2 * kW4Block) + 64;
-  W4Digits d = a.d;                                // the slab in shared memory
+  W4Digits d;                                      // the slab of x
   d.digits = w4_smem + Cfg::kFixed;
   d.pitch = pitch;
   d.sums = reinterpret_cast<int*>(d.digits + p.cols * pitch);
-  d.scale = reinterpret_cast<float*>(d.sums + a.slab * GPB * COLS);
+  d.scale = reinterpret_cast<float*>(d.sums + a.slab * GPB * 8);
+  d.gpb = GPB;
   const int g = lane >> 2, t = lane & 3;
   const int rank = p.splits > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   const int cluster = static_cast<int>(blockIdx.x) / p.splits, clusters = static_cast<int>(gridDim.x) / p.splits;
   const int b_begin = min(p.blocks, rank * a.per_cta), b_end = min(p.blocks, b_begin + a.per_cta);
   const int tile_begin = static_cast<int>(int64_t(a.row_tiles) * cluster / clusters);
   const int tile_end = static_cast<int>(int64_t(a.row_tiles) * (cluster + 1) / clusters);
-  const bool cut_here = a.d.digits == nullptr;
   if (lane == 0) {
     for (int i = 0; i < S; ++i) mbar_init(&bars[i], 1);
     if (warp == 0) *abort_flag = 0;
     fence_barrier_init();
   }
   __syncthreads();
-  if (cut_here) pdl_wait();  // otherwise w4_digits_kernel has: what came before it is complete
+  pdl_wait();
+  pdl_launch_dependents();
 
   float total[NT][4];
   // 32-bit shared addresses; columns past the last one repeat it, their sums are never read.
   const uint32_t ring_at = smem_u32(ring), lane_codes = 16 * WB + lane * 16, lane_words = g * WB;
   uint32_t x_col[NT];
 #pragma unroll
-  for (int i = 0; i < NT; ++i)
-    x_col[i] = smem_u32(d.digits) + min(8 * i + g, p.cols - 1) * pitch + (XT == 0 ? 32 : 16) * t;
+  for (int i = 0; i < NT; ++i) {
+    // Three terms to a row: columns 4 * row + term (the fourth is not read), or a tile of columns per term.
+    const int row = XT != kW4Terms ? min(8 * i + g, p.cols - 1)
+                    : NT == 1      ? min(g & 3, 2) * p.M + min(g >> 2, p.M - 1)
+                                   : i * p.M + min(g, p.M - 1);
+    x_col[i] = smem_u32(d.digits) + row * pitch + (XT == 0 ? 32 : 16) * t;
+  }
   uint32_t magic = 0;  // in a register: the logic instruction takes one immediate
-  if constexpr (XT != 0) asm volatile("mov.b32 %0, %1;" : "=r"(magic) : "n"(XT == 2 ? 0x43004300u : 0x64006400u));
+  if constexpr (XT != 0) asm volatile("mov.b32 %0, %1;" : "=r"(magic) : "n"(BF ? 0x43004300u : 0x64006400u));
   const uint32_t sums_at = smem_u32(d.sums) + 8 * t, scale_at = smem_u32(d.scale) + 8 * t;
 
   auto multiply16 = [&](uint32_t piece, int blk) {
@@ -333,9 +376,8 @@ __global__ void __launch_bounds__(32 * kW4StreamWarps, 1) w4_stream_kernel(const
     uint32_t wa[WB / 4], wb[WB / 4];
     lds_words(wa, piece + lane_words);
     lds_words(wb, piece + lane_words + 8 * WB);
-    // A group's sum in two parts: one chain of eight dependent MMAs is what a warp would wait for
-    // (28672 x 8192, 8 rows: 38.9 us, in two parts 34.8, in four 37.7).
-    float acc[NT][2][4], sa = 0.f, sb = 0.f;
+    constexpr int CH = Cfg::kChains;
+    float acc[NT][CH][4], sa = 0.f, sb = 0.f;
     uint32_t za = 0, zb = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -358,26 +400,27 @@ __global__ void __launch_bounds__(32 * kW4StreamWarps, 1) w4_stream_kernel(const
       uint32_t u[4], v[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        u[i] = w4_pair<XT == 2>(ca, i, magic, za);
-        v[i] = w4_pair<XT == 2>(cb, i, magic, zb);
+        u[i] = w4_pair<BF>(ca, i, magic, za);
+        v[i] = w4_pair<BF>(cb, i, magic, zb);
       }
 #pragma unroll
       for (int i = 0; i < NT; ++i) {
         const uint4 xv = lds128(x_col[i] + blk * (2 * kW4Block) + 64 * j);
-        if (j % kSteps == 0) {
-          mma_16816_zero<XT == 2>(acc[i][0], u[0], v[0], u[1], v[1], xv.x, xv.y);
-          mma_16816_zero<XT == 2>(acc[i][1], u[2], v[2], u[3], v[3], xv.z, xv.w);
-        } else {
-          mma_16816<XT == 2>(acc[i][0], u[0], v[0], u[1], v[1], xv.x, xv.y);
-          mma_16816<XT == 2>(acc[i][1], u[2], v[2], u[3], v[3], xv.z, xv.w);
-        }
+        if (j % kSteps == 0)
+          mma_16816_zero<BF>(acc[i][0], u[0], v[0], u[1], v[1], xv.x, xv.y);
+        else
+          mma_16816<BF>(acc[i][0], u[0], v[0], u[1], v[1], xv.x, xv.y);
+        if (j % kSteps == 0 && CH == 2)
+          mma_16816_zero<BF>(acc[i][CH - 1], u[2], v[2], u[3], v[3], xv.z, xv.w);
+        else
+          mma_16816<BF>(acc[i][CH - 1], u[2], v[2], u[3], v[3], xv.z, xv.w);
       }
       if ((j + 1) % kSteps == 0) {
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
 #pragma unroll
           for (int c = 0; c < 4; ++c)
-            total[i][c] = fmaf(acc[i][0][c] + acc[i][1][c], c < 2 ? sa : sb, total[i][c]);
+            total[i][c] = fmaf(CH == 2 ? acc[i][0][c] + acc[i][CH - 1][c] : acc[i][0][c], c < 2 ? sa : sb, total[i][c]);
         }
       }
     }
@@ -393,7 +436,7 @@ __global__ void __launch_bounds__(32 * kW4StreamWarps, 1) w4_stream_kernel(const
     for (int i = 0; i < NT; ++i) {
       x[i][0] = lds128(x_col[i] + blk * kW4Block);
       x[i][1] = lds128(x_col[i] + blk * kW4Block + 16);
-      xs[i] = lds64(scale_at + blk * (COLS * 4) + 32 * i);
+      xs[i] = lds64(scale_at + blk * 32);
     }
     int acc[NT][4];
     float sa = 0.f, sb = 0.f;
@@ -413,7 +456,7 @@ __global__ void __launch_bounds__(32 * kW4StreamWarps, 1) w4_stream_kernel(const
         }
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-          const uint2 sx = lds64(sums_at + (blk * GPB + k) * (COLS * 4) + 32 * i);
+          const uint2 sx = lds64(sums_at + (blk * GPB + k) * 32);
           acc[i][0] = 0x4B400000 + za * static_cast<int>(sx.x);
           acc[i][1] = 0x4B400000 + za * static_cast<int>(sx.y);
           acc[i][2] = 0x4B400000 + zb * static_cast<int>(sx.x);
@@ -453,7 +496,7 @@ __global__ void __launch_bounds__(32 * kW4StreamWarps, 1) w4_stream_kernel(const
 
   int stage = 0;
   uint32_t phase = 0;
-  bool ok = true, waited = false;
+  bool ok = true;
   const bool whole_x = b_end - b_begin <= a.slab;
   for (int group = tile_begin; group < tile_end; group += kW4GroupTiles) {
     const int ntiles = min(kW4GroupTiles, tile_end - group);
@@ -488,32 +531,18 @@ __global__ void __launch_bounds__(32 * kW4StreamWarps, 1) w4_stream_kernel(const
       };
 #pragma unroll
       for (int i = 0; i < S; ++i) fetch();
-      if (!waited) {
-        pdl_wait();
-        pdl_launch_dependents();
-        waited = true;
-      }
       if (!whole_x || (group == tile_begin && s0 == b_begin)) {
-        if constexpr (XT != 0) {
+        if constexpr (XT == kW4Terms) {
+          w4_stage32(p, d.digits, pitch, s0, n);
+        } else if constexpr (XT != 0) {
           w4_stage16(p, d.digits, pitch, s0, n);
-        } else if (cut_here) {
+        } else {
           for (int base = 0; base < p.M * n; base += T / 16) {
             const int task = base + (threadIdx.x >> 4);
             const bool live = task < p.M * n;
             const int m = live ? task / n : 0, at = live ? task - m * n : 0;
             w4_cut(p, d, live, m, s0 + at, at, threadIdx.x & 15);
           }
-        } else {
-          for (int c = warp; c < p.cols; c += W) {
-            const uint8_t* src = a.d.digits + c * a.d.pitch + static_cast<int64_t>(s0) * kW4Block;
-            for (int k = lane * 16; k < n * kW4Block; k += 512) cp_async_16(d.digits + c * pitch + k, src + k, 16);
-          }
-          const int* src_sums = a.d.sums + static_cast<int64_t>(s0) * GPB * COLS;
-          for (int i = threadIdx.x * 4; i < n * GPB * COLS; i += T * 4) cp_async_16(d.sums + i, src_sums + i, 16);
-          const float* src_scale = a.d.scale + static_cast<int64_t>(s0) * COLS;
-          for (int i = threadIdx.x * 4; i < n * COLS; i += T * 4) cp_async_16(d.scale + i, src_scale + i, 16);
-          cp_async_commit();
-          cp_async_wait<0>();
         }
       }
       if (s0 == b_begin)
@@ -523,29 +552,32 @@ __global__ void __launch_bounds__(32 * kW4StreamWarps, 1) w4_stream_kernel(const
       // A row tile's sums are complete, or as far as this warp goes.
       auto leave = [&](int tile, bool whole, int which) {
         float* dst = whole ? tile_sums + tile * Cfg::kPart : parts + (2 * warp + which) * Cfg::kPart;
+        if constexpr (Cfg::kSummed && NT == 1) {
+          // A row of x: two columns here, two (three terms: one) in the neighbouring lane.
+          const bool both = XT == 0 || (t & 1) == 0;
+          float v0 = total[0][0] + (both ? total[0][1] : 0.f), v1 = total[0][2] + (both ? total[0][3] : 0.f);
+          v0 += __shfl_xor_sync(0xffffffffu, v0, 1);
+          v1 += __shfl_xor_sync(0xffffffffu, v1, 1);
+          if ((t & 1) == 0) {
+            float* r = dst + (t >> 1) * 16 + g;
+            r[0] = whole ? r[0] + v0 : v0;
+            r[8] = whole ? r[8] + v1 : v1;
+          }
+        } else {
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          if constexpr (XT != 0) {
+          for (int i = 0; i < (Cfg::kSummed ? 1 : NT); ++i) {
             float* r = dst + (8 * i + 2 * t) * 16 + g;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               float* at = r + (j & 1) * 16 + (j >> 1) * 8;
-              *at = whole ? *at + total[i][j] : total[i][j];
-              total[i][j] = 0.f;
+              float v = total[i][j];
+              if constexpr (Cfg::kSummed) v = (total[2][j] + total[1][j]) + total[0][j];
+              *at = whole ? *at + v : v;
             }
-            continue;
           }
-          // Digits of one row of x: two columns here, two in the neighbouring lane.
-          float v0 = total[i][0] + total[i][1], v1 = total[i][2] + total[i][3];
-          v0 += __shfl_xor_sync(0xffffffffu, v0, 1);
-          v1 += __shfl_xor_sync(0xffffffffu, v1, 1);
-          if ((t & 1) == 0) {
-            float* r = dst + (2 * i + (t >> 1)) * 16 + g;
-            r[0] = whole ? r[0] + v0 : v0;
-            r[8] = whole ? r[8] + v1 : v1;
-          }
-          total[i][0] = total[i][1] = total[i][2] = total[i][3] = 0.f;
         }
+#pragma unroll
+        for (int i = 0; i < NT; ++i) total[i][0] = total[i][1] = total[i][2] = total[i][3] = 0.f;
       };
 #pragma unroll
       for (int i = 0; i < NT; ++i) total[i][0] = total[i][1] = total[i][2] = total[i][3] = 0.f;
@@ -627,8 +659,8 @@ __global__ void __launch_bounds__(32 * kW4StreamWarps, 1) w4_stream_kernel(const
           v += u;
         }
       }
-      if constexpr (XT == 0) {
-        if (v != v) v = w4_output(p, GPB, row, m);
+      if constexpr (Cfg::kSummed) {
+        if (!(fabsf(v) <= FLT_MAX)) v = w4_output(p, GPB, row, m);
       }
       if (p.bias != nullptr) v += load_as_float(p.bias, row, p.dtype);
       store_from_float(p.out, int64_t(m) * p.ldo + row, p.dtype, v);
