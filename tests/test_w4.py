@@ -697,3 +697,11 @@ def _huge(m, dtype, sdtype=None):
 def test_huge_fp32_x_overflows_no_sum(m):
     x, codes, scales, zeros = _huge(m, "f32")
     _check(x, codes, scales, zeros, None, 64, "f32")
+
+
+@gpu
+@pytest.mark.parametrize("m,sdtype", [(1, "bf16"), (2, "bf16"), (3, "f32"), (8, "bf16"), (16, "f32"), (17, "bf16"),
+                                      (40, "f32")])
+def test_huge_bf16_x_overflows_no_sum(m, sdtype):
+    x, codes, scales, zeros = _huge(m, "bf16", sdtype)
+    _check(x, codes, scales, zeros, None, 64, "bf16")

@@ -191,6 +191,7 @@ __device__ __noinline__ float w4_output(const W4Args& p, int gpb, int n, int m) 
     const float s = p.wide ? __uint_as_float(w[1]) : w4_scale16(w[0], p.scale_bf16);
     const float q = float((code >> (4 * (kk >> 1 & 3) + 16 * (kk & 1))) & 15u) - float(w[0] & 15u);
     v += load_as_float(p.x, m * p.ldx + k, p.dtype) * (q * s);
+    if (v != v) break;  // it stays NaN
   }
   return v;
 }
@@ -659,7 +660,7 @@ __global__ void __launch_bounds__(32 * kW4StreamWarps, 1) w4_stream_kernel(const
           v += u;
         }
       }
-      if constexpr (Cfg::kSummed) {
+      if constexpr (XT != TILEC_DTYPE_F16) {  // fp16 times codes stays in range, and is not finite by itself
         if (!(fabsf(v) <= FLT_MAX)) v = w4_output(p, GPB, row, m);
       }
       if (p.bias != nullptr) v += load_as_float(p.bias, row, p.dtype);
