@@ -317,9 +317,7 @@ TILEC_API size_t tilec_linear_ce_workspace_bytes(const void* x, const void* w, i
  *   0..7 of the block, k = 2i in bits 4i..4i+3 and k = 2i + 1 in bits 4i+16..4i+19 (i = 0..3).
  *   Rows past N and k past K: any codes, finite scales.
  * Up to 8 rows (many 16-bit calls of up to 16), x, codes, zero points and scales enter exactly and
- * sums are fp32; one 16-bit row of x (two of a large weight) enters as whole multiples of
- * 2^-29 of the power of two at or below the largest magnitude of its block of 128 k.  With more
- * rows the weight (code - zero) * scale is rounded once to dtype and multiplied on the tensor
+ * sums are fp32.  With more rows the weight (code - zero) * scale is rounded once to dtype and multiplied on the tensor
  * cores (fp32: the 3xTF32 product).  out shares no memory with x or bias.
  * Workspace: tilec_mm_w4_workspace_bytes (at most 256 MiB of expanded weights or 256 rows). */
 TILEC_API int tilec_mm_w4(const void* x, int32_t dtype, int64_t M, int64_t ldx, const void* weight,

@@ -705,3 +705,32 @@ def test_huge_fp32_x_overflows_no_sum(m):
 def test_huge_bf16_x_overflows_no_sum(m, sdtype):
     x, codes, scales, zeros = _huge(m, "bf16", sdtype)
     _check(x, codes, scales, zeros, None, 64, "bf16")
+
+
+@gpu
+@pytest.mark.parametrize("m,n,k,dtype,top", [(1, 300, 2500, "bf16", 2.0 ** 30), (1, 300, 2500, "bf16", 2.0 ** 110),
+                                             (1, 40005, 2500, "f16", 2.0 ** 15), (1, 2500, 40000, "bf16", 2.0 ** 23),
+                                             (2, 9000, 16000, "bf16", 2.0 ** 40), (2, 9000, 16000, "f16", 2.0 ** 13),
+                                             (1, 37, 300, "bf16", 2.0 ** 127)])
+@pytest.mark.parametrize("few", [True, False])
+def test_large_elements_beside_small_ones_in_16_bits(m, n, k, dtype, top, few):
+    """The digits of one or two 16-bit rows hold 30 bits below a block's largest magnitude; what they
+    leave out of a few elements, or of all, counts all the same.  Repeats give the same bits."""
+    x, codes, scales, zeros, _ = _make(m, n, k, 64, dtype)
+    if few:      # one block in five, most of whose elements are zeros, with a large one
+        x.view(-1)[torch.rand(m * k, generator=torch.Generator().manual_seed(8)) < 0.97] = 0
+    x[:, 7::640 if few else 32] = top
+    x[:, 9::64] *= 2.0 ** -10
+    codes[:, 7::32] = zeros.repeat_interleave(2, 1)[:, :codes[:, 7::32].shape[1]]
+    x, codes, scales, zeros = (t.cuda() for t in (x, codes, scales, zeros))
+    w64 = _weight64(codes, scales, zeros, 64)
+    y = x.double() @ w64.t()
+    w = ext.pack_w4(codes, scales, zeros, 64)
+    got = ext.matrix_mul_w4(x, w)
+    s = x.double().abs() @ w64.abs().t()
+    # group sums (and, one by one, elements) added in fp32 in any order, 2^-24 S each at worst
+    tol = ((k if not few else -(-k // 64) + 110) * 2.0 ** -24 + 2.0 ** -19) * s + 1.001 * U[dtype] * y.abs() + (
+        2.0 ** -25 if dtype == "f16" else 0.0)
+    assert ((got.double() - y).abs() <= tol).all(), f"{((got.double() - y).abs() / tol).max():.1f} of the bound"
+    for _ in range(3):
+        assert torch.equal(ext.matrix_mul_w4(x, w), got)

@@ -618,12 +618,11 @@ int check_w4_pointers(const W4Call& c) {
 }
 
 // How many rows of x run where: one of 16-bit x in digits on w4_stream_kernel; up to 16 there too,
-// as they are, but for two against a large weight (4096 x 4096: 7.4 us, in
-// digits 9.5; 8192 x 8192: 15.6 and 19.4; 28672 x 8192: 36.7 and 33.0); up to 8 of fp32 x there
-// as well, in three bf16 terms (three columns a row, which NT = 3 tiles of 8 hold); up to 256 of 16-bit x
-// whose type the scales share on w4_tc_kernel, 128 at a time (8192 x 8192: 128 rows 35 to 39 us,
-// twice that for 256; expanded first, either takes 89); for the rest W is expanded once into the
-// workspace and multiplied on the tcgen05 kernels (fp32: 3xTF32).
+// as they are; up to 8 of fp32 x there as well, in three bf16 terms (three columns a row, which
+// NT = 3 tiles of 8 hold); up to 256 of 16-bit x whose type the scales share on w4_tc_kernel, 128
+// at a time (8192 x 8192: 128 rows 35 to 39 us, twice that for 256; expanded first, either takes
+// 89); for the rest W is expanded once into the workspace and multiplied on the tcgen05 kernels
+// (fp32: 3xTF32).
 constexpr int64_t kW4Max16 = 16;    // rows of 16-bit x
 constexpr int64_t kW4Max32 = 8;     // rows of fp32 x
 
@@ -638,8 +637,8 @@ void plan_w4(const W4Call& c, const DeviceInfo& d, const LmInfo& lm, W4Plan* p) 
     return o;
   };
   const int gpb = c.group == 32 ? 4 : c.group == 64 ? 2 : 1;
-  const bool wide = c.sdt == TILEC_DTYPE_F32, two = c.M == 2 && c.N * p->kp >= int64_t(1) << 27;
-  const bool digits = !f32 && (c.M == 1 || two), terms = f32 && c.M <= kW4Max32;
+  const bool wide = c.sdt == TILEC_DTYPE_F32;
+  const bool digits = !f32 && c.M == 1, terms = f32 && c.M <= kW4Max32;
   // Nine to 16 rows: each further slab of x costs w4_stream_kernel some 6 us, w4_tc_kernel is the
   // slower the larger the weight (4096 x 4096, 16 rows in two slabs: 18.0 against 11.3 us;
   // 8192 x 8192, 13 in two: 22.8 against 25.6, 16 in three: 28.0 against 25.6; 28672 x 8192, 16
@@ -654,7 +653,7 @@ void plan_w4(const W4Call& c, const DeviceInfo& d, const LmInfo& lm, W4Plan* p) 
     p->stream = true;
     p->polling = d.short_waits;
     p->xt = digits ? 0 : terms ? kW4Terms : c.dtype;
-    p->cols = static_cast<int>(c.M * (digits ? kW4Digits : terms ? kW4Terms : 1));
+    p->cols = static_cast<int>(digits ? kW4Digits : terms ? kW4Terms * c.M : c.M);
     p->nt = terms ? (c.M <= 2 ? 1 : 3) : p->cols <= 8 ? 1 : 2;
     // One CTA per SM.  With fewer 16-row tiles than SMs, a cluster of CTAs shares each tile's K.
     const int64_t tiles = cdiv(c.N, 16);
@@ -667,7 +666,7 @@ void plan_w4(const W4Call& c, const DeviceInfo& d, const LmInfo& lm, W4Plan* p) 
     const int64_t clusters = d.sms / p->splits;
     p->ctas = static_cast<int>((tiles < clusters ? tiles : clusters) * p->splits);
     const int64_t room = kW4MaxSmem - w4_stream_fixed(p->nt, gpb, wide, p->xt);
-    auto slab_bytes = [&](int64_t n) { return digits ? w4_slab_bytes(n, p->cols, gpb) : w4_slab16_bytes(n, p->cols); };
+    auto slab_bytes = [&](int64_t n) { return digits ? w4_slab_bytes(n, gpb) : w4_slab16_bytes(n, p->cols); };
     int64_t slab = p->per_cta;
     while (slab > 1 && slab_bytes(slab) > room) --slab;
     p->slab = static_cast<int>(cdiv(p->per_cta, cdiv(p->per_cta, slab)));  // slabs of one size
@@ -728,7 +727,7 @@ int launch_w4_stream(const W4Args& w, const W4Plan& p, cudaStream_t s) {
   a.polling = p.polling;
   using Cfg = W4StreamCfg<NT, GPB, SC == 0, XT>;
   const size_t smem =
-      size_t(Cfg::kFixed + (XT != 0 ? w4_slab16_bytes(p.slab, w.cols) : w4_slab_bytes(p.slab, w.cols, GPB)));
+      size_t(Cfg::kFixed + (XT != 0 ? w4_slab16_bytes(p.slab, w.cols) : w4_slab_bytes(p.slab, GPB)));
   if (int64_t(smem) > kW4MaxSmem) return TILEC_ERR_UNSUPPORTED;
   return launch_k(w4_stream_kernel<NT, GPB, SC, XT>, dim3(static_cast<unsigned>(p.ctas)), dim3(Cfg::kThreads), smem, s,
                   w.splits, a);

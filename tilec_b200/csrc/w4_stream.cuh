@@ -1,6 +1,5 @@
-// w4_stream.cuh -- the few-rows product with 4-bit weights on mma.sync: one row of 16-bit x (two of
-// a large weight) on the integer path, up to 16 rows of 16-bit x and up to 8 of fp32 x on the
-// 16-bit one.
+// w4_stream.cuh -- the few-rows product with 4-bit weights on mma.sync: one row of 16-bit x on the
+// integer path, up to 16 rows of 16-bit x and up to 8 of fp32 x on the 16-bit one.
 //
 // One token's product reads N * K / 2 bytes of codes and is bound by memory, if only the
 // arithmetic keeps up: at 6.5 TB/s a quarter SM has about 180 cycles per 1 KB of codes (16
@@ -10,17 +9,17 @@
 // pipe.  fp32 x enters as three bf16 numbers of 8 bits each, which hold all of its 24 (w4_stage32):
 // three columns of the product to a row of x.
 // An 8-bit operand (multiply8) needs 3 for 8 codes, and m16n8k32 takes twice the k at the
-// same rate, for four columns per row of x:
+// same rate, for the eight columns that one row of x then has:
 //
-//   * per 128-k block and row, x becomes whole numbers X = round(x * 2^(29 - e)), 2^e <= the
-//     block's largest magnitude < 2^(e + 1), in four signed 8-bit digits: x is off by at most
-//     2^-30 of 2^e, which is exact for 16-bit types wherever the magnitude is within 2^-22
-//     (bf16) or 2^-19 (fp16) of that;
+//   * per 128-k block, x becomes pairs of whole numbers X 2^(e - 29) + Y 2^(e - 60), 2^e <= the
+//     block's largest magnitude < 2^(e + 1), in four signed 8-bit digits each.  That is all of a
+//     16-bit number down to 2^-53 (bf16; fp16: always) of the largest.  What they leave out of
+//     smaller ones is kept in a list (W4Rest, normally empty) and added by itself: x enters exactly;
 //   * each digit is one column of the tensor-core product, so sums over a group are exact
-//     32-bit integers: sum code * X - zero * sum X;
-//   * that times scale * 2^(e - 29) * 256^digit is added in fp32.
-// (fp32 x in digits was as fast, but an element 2^-13 of its block's largest keeps 17 bits, which
-// shows where the largest meets the zero point: 4e-6 off where an fp32 product is 2e-7.)
+//     32-bit integers: sum code * digit - zero * sum digit;
+//   * that times scale * the digit's power of two is added in fp32.
+// (With X alone an fp32 element 2^-13 of its block's largest keeps 17 bits, which shows where the
+// largest meets the zero point: 4e-6 off where an fp32 product is 2e-7.)
 //
 // The sums start at 0x4B400000 - zero * sum X: read as a float that is 1.5 * 2^23 + the sum
 // (|sum| < 2^22), which saves the conversions.
@@ -31,15 +30,16 @@
 // copies of four pieces each (two where x needs the room), so that 140 (70) KB are on their way
 // to an SM at any time.  Where a
 // tile is shared by several warps their sums meet in shared memory, in the order of K.
-// Each CTA cuts, splits or copies x for itself (one row is a round of some 150 instructions per 32
-// blocks), a slab of K at a time where it does not fit.
+// Each CTA cuts, splits or copies x for itself, a slab of K at a time where it does not fit (one
+// row: from K = 10368 or less on).
 //
-// Measured (graph replay), 28672 x 8192, one token (125 MB): 24.7 us, 5.0 TB/s.  On the way, with
-// 27.8 as the best then: rows of codes with the group words apart 35 to 40 us
+// Measured (graph replay), 28672 x 8192, one token (125 MB): 26.2 us, 4.8 TB/s; four digits
+// instead of eight 25.4, but eight are what holds x, and the other four columns of the MMA would be
+// idle.  On the way, with 27.8 as the best then: rows of codes with the group words apart 35 to 40 us
 // (the words alone cost 6); 24 warps with copies of two pieces 30.5; 12 warps 30.3; CTAs of
-// 128 rows, two waves of them for want of one slot, 40.  8 rows: 33.0 us (a grid of small CTAs
-// with cp.async rings 48), 16 rows, x in three slabs: 50.4.  fp32: one row 32.4, 8 rows of 8192 x
-// 8192 34.0 (in digits 28.3 and 34.4).
+// 128 rows, two waves of them for want of one slot, 40.  8 rows: 33.2 us (a grid of small CTAs
+// with cp.async rings 48), 16 rows, x in three slabs: 50.4.  fp32: one row 32.3, 8 rows of 8192 x
+// 8192 34.1 (in digits 28.4 and 34.4).
 #pragma once
 
 #include <cfloat>
@@ -50,7 +50,7 @@
 namespace tilec {
 
 constexpr int kW4StreamWarps = 16;
-constexpr int kW4Digits = 4;      // columns per row of x
+constexpr int kW4Digits = 8;      // columns of the one row of x
 constexpr int kW4GroupTiles = 16; // row tiles whose sums a CTA holds at a time
 
 // The digits of x in shared memory; zeros past K.
@@ -58,9 +58,18 @@ struct W4Digits {
   uint8_t* digits;   // [col][pitch], 128 bytes a block, [t][j][8]: 8 consecutive k in the order 0 4 1 5 2 6 3 7
   int64_t pitch;
   int* sums;         // [block][group][8]: minus the sum of a column's digits over a group
-  float* scale;      // [block][8]: 2^(e - 29) * 256^digit; columns are 4 * row + digit, the smallest first
+  float* scale;      // [block][8]: 2^(e - 60) * 256^digit for the lower four, 2^(e - 29) * 256^(digit - 4)
   int gpb;           // groups per block
+  int* rest_count;   // elements of the slab that the digits do not hold in full ...
+  struct W4Rest* rest;  // ... and by how much, kW4MaxRest at most
 };
+
+// An element of x beyond what its digits hold: its k, and the exact difference.
+struct W4Rest {
+  int k;
+  float value;
+};
+constexpr int kW4MaxRest = 64;
 
 struct W4StreamArgs {
   W4Args w;          // the weight, x, bias and out
@@ -70,8 +79,8 @@ struct W4StreamArgs {
   int polling;       // the device's wait limit is shortened (w4_wait_on)
 };
 
-// XT: how x enters: 0 in digits (one or two 16-bit rows), TILEC_DTYPE_F16 or _BF16 as it is,
-// kW4Terms (fp32) in three bf16 terms.
+// XT: how x enters: 0 in digits (one 16-bit row), TILEC_DTYPE_F16 or _BF16 as it is, kW4Terms
+// (fp32) in three bf16 terms.
 constexpr int kW4Terms = 3;
 
 template <int NT, int GPB, bool WIDE, int XT>
@@ -86,7 +95,7 @@ struct W4StreamCfg {
   static constexpr int kRingBytes = kW4StreamWarps * kStages * kStage;
   static constexpr bool kSummed = XT == 0 || XT == kW4Terms;  // several columns to a row of x
   static_assert(!(XT == 0 && NT != 1) && !(XT == kW4Terms && NT != 1 && NT != 3), "columns of several to a row");
-  static constexpr int kRows = kSummed && NT == 1 ? 2 : kSummed ? 8 : 8 * NT;  // rows of x
+  static constexpr int kRows = XT == 0 ? 1 : kSummed && NT == 1 ? 2 : kSummed ? 8 : 8 * NT;  // rows of x
   static constexpr int kPart = kRows * 16;  // floats: the sums of a row tile, [row of x][16]
   // Chains of MMAs per group and column: one of eight dependent MMAs is what a warp would wait for
   // (28672 x 8192, 8 rows: 38.9 us, in two parts 34.8, in four 37.7); three tiles of columns are
@@ -94,35 +103,36 @@ struct W4StreamCfg {
   static constexpr int kChains = NT == 3 ? 1 : 2;
   static constexpr int kSumBytes = kW4GroupTiles * kPart * 4;
   static constexpr int kPartBytes = 2 * kW4StreamWarps * kPart * 4;
-  static constexpr int kBarBytes = 1024;     // a barrier per warp and stage, the abort flag
+  static constexpr int kBarBytes = 1024;     // a barrier per warp and stage, W4Rest, the abort flag
+  static constexpr int kRestAt = 512 - 16;   // two counts, then the entries
   static constexpr int kFixed = kRingBytes + kSumBytes + kPartBytes + kBarBytes;
-  static_assert(kStage % 128 == 0 && (kW4StreamWarps * kStages + 1) * 8 <= kBarBytes, "shared memory layout");
+  static_assert(kStage % 128 == 0 && kW4StreamWarps * kStages * 8 <= kRestAt, "shared memory layout");
+  static_assert(kRestAt + 8 + kW4MaxRest * 8 <= kBarBytes - 8, "shared memory layout");
 };
 // Bytes of `slab` blocks of x: digits (16 bytes more a column: conflict-free reads), sums, scales.
-__host__ __device__ inline int64_t w4_slab_bytes(int64_t slab, int cols, int gpb) {
-  return cols * (slab * kW4Block + 16) + slab * 8 * 4 * (gpb + 1);
+__host__ __device__ inline int64_t w4_slab_bytes(int64_t slab, int gpb) {
+  return kW4Digits * (slab * kW4Block + 16) + slab * kW4Digits * 4 * (gpb + 1);
 }
 // The same in 16-bit values (64 bytes more a row: conflict-free reads); fp32: three such rows.
 __host__ __device__ inline int64_t w4_slab16_bytes(int64_t slab, int64_t rows) {
   return rows * (slab * (2 * kW4Block) + 64);
 }
 
-// Sixteen lanes (l = 0 .. 15) cut one 128-k block of one row of x; all lanes of a warp call.
+// Sixteen lanes (l = 0 .. 15) cut one 128-k block of the row x; all lanes of a warp call.
 // `at`: where the block goes in d.
-__device__ __forceinline__ void w4_cut(const W4Args& p, const W4Digits& d, bool live, int m, int blk, int at, int l) {
-  constexpr int shift = 29;
+__device__ __forceinline__ void w4_cut(const W4Args& p, const W4Digits& d, bool live, int blk, int at, int l) {
   const int j = l >> 2, t = l & 3;
   const int k0 = blk * kW4Block + 8 * l;
   float v[8];
-  const unsigned short* s = static_cast<const unsigned short*>(p.x) + m * p.ldx + k0;
+  const unsigned short* src = static_cast<const unsigned short*>(p.x) + k0;
   uint32_t w[4] = {0, 0, 0, 0};
   if (live && p.vec_x && k0 + 8 <= p.K) {
-    const uint4 h = *reinterpret_cast<const uint4*>(s);
+    const uint4 h = *reinterpret_cast<const uint4*>(src);
     w[0] = h.x; w[1] = h.y; w[2] = h.z; w[3] = h.w;
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (live && k0 + i < p.K) w[i >> 1] |= uint32_t(s[i]) << (16 * (i & 1));
+      if (live && k0 + i < p.K) w[i >> 1] |= uint32_t(src[i]) << (16 * (i & 1));
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -140,21 +150,42 @@ __device__ __forceinline__ void w4_cut(const W4Args& p, const W4Digits& d, bool 
   for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
 #pragma unroll
   for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-  // 2^-90 and below share one step (2^(shift + 90) still is a float).
-  const int e = max(static_cast<int>(top >> 23) - 127, -90);
-  const float up = __uint_as_float(static_cast<uint32_t>(127 + shift - e) << 23);
-  uint32_t y[8];  // X + 0x80 in every byte: bytes, less 0x80 each, are the digits
+  // Powers of two as bits.  2^-60 and below share one step, so that all of them are normal numbers.
+  const int e = max(static_cast<int>(top >> 23) - 127, -60);
+  auto pow2 = [](int n) { return __uint_as_float(static_cast<uint32_t>(127 + n) << 23); };
+  // x = X 2^(e - 29) + Y 2^(e - 60), |X|, |Y| <= 2^30, and what neither holds.
+  uint32_t x_hi[8], x_lo[8];  // with 0x80 in every byte: bytes, less 0x80 each, are the digits
+  auto cut = [&](uint32_t (&y)[8], float up, float down) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float s = v[i] * up;
-    y[i] = static_cast<uint32_t>(__float2int_rn(s)) + 0x80808080u;
+    for (int i = 0; i < 8; ++i) {
+      const int whole = __float2int_rn(v[i] * up);
+      y[i] = static_cast<uint32_t>(whole) + 0x80808080u;
+      v[i] = fmaf(-__int2float_rn(whole), down, v[i]);  // exact: few bits of x are left below a step
+    }
+  };
+  cut(x_hi, pow2(29 - e), pow2(e - 29));
+  cut(x_lo, pow2(60 - e), pow2(e - 60));
+  bool rest = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) rest |= v[i] != 0.f;
+  if (rest && top < 0x7F800000u) {
+#pragma unroll 1
+    for (int i = 0; i < 8; ++i) {
+      float value = 0.f;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) value = c == i ? v[c] : value;
+      if (value == 0.f) continue;
+      const int n = atomicAdd(d.rest_count, 1);
+      if (n < kW4MaxRest) d.rest[n] = W4Rest{k0 + i, value};
+    }
   }
-  // 2^(e - shift) * 256^part; a block with anything not finite makes its sums NaN, and the
-  // outputs are then computed one by one (w4_output).
-  const float down = top >= 0x7F800000u ? __int_as_float(0x7fc00000)
-                                        : __uint_as_float(static_cast<uint32_t>(127 + e - shift) << 23);
+  // A block with anything not finite makes its sums NaN, and the outputs are then computed one by
+  // one (w4_output).
+  const bool finite = top < 0x7F800000u;
 #pragma unroll
-  for (int part = 0; part < kW4Digits; ++part) {
+  for (int col = 0; col < kW4Digits; ++col) {
+    const int part = col & 3;
+    const uint32_t(&y)[8] = col < 4 ? x_lo : x_hi;
     const uint32_t sel = part | (4 + part) << 4;
     auto gather = [&](int a, int b, int c, int e) {
       return __byte_perm(__byte_perm(y[a], y[b], sel), __byte_perm(y[c], y[e], sel), 0x5410) ^ 0x80808080u;
@@ -168,12 +199,27 @@ __device__ __forceinline__ void w4_cut(const W4Args& p, const W4Digits& d, bool 
     other = __shfl_xor_sync(0xffffffffu, sum, 8);
     if (d.gpb == 1) sum += other;
     if (!live) continue;
-    const int col = m * kW4Digits + part;
     *reinterpret_cast<uint2*>(d.digits + col * d.pitch + at * kW4Block + t * 32 + j * 8) = make_uint2(d0, d1);
-    if (t == 0 && j % (4 / d.gpb) == 0)
-      d.sums[(at * d.gpb + j / (4 / d.gpb)) * 8 + col] = -sum;
-    if (l == 0) d.scale[at * 8 + col] = down * __uint_as_float(static_cast<uint32_t>(127 + 8 * part) << 23);
+    if (t == 0 && j % (4 / d.gpb) == 0) d.sums[(at * d.gpb + j / (4 / d.gpb)) * kW4Digits + col] = -sum;
+    if (l == 0)
+      d.scale[at * kW4Digits + col] = finite ? pow2(e - (col < 4 ? 60 : 29) + 8 * part) : __int_as_float(0x7fc00000);
   }
+}
+
+__device__ __forceinline__ float w4_weight(const W4Args& p, int gpb, int n, int k) {
+  const int wb = w4_word_bytes(gpb, p.wide), b = k / kW4Block, kk = k % kW4Block;
+  const uint8_t* piece = p.data + (int64_t(n >> 4) * p.blocks + b) * w4_piece_bytes(gpb, p.wide);
+  const uint32_t code = reinterpret_cast<const uint32_t*>(piece + 16 * wb + (n & 15) * 64)[(kk >> 3 & 3) * 4 + (kk >> 5)];
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(piece + (n & 15) * wb) + (kk * gpb / kW4Block) * (p.wide ? 2 : 1);
+  const float s = p.wide ? __uint_as_float(w[1]) : w4_scale16(w[0], p.scale_bf16);
+  return (float((code >> (4 * (kk >> 1 & 3) + 16 * (kk & 1))) & 15u) - float(w[0] & 15u)) * s;
+}
+
+// What x's digits left out, in order of k: the sum over `n` entries for one output.
+__device__ __noinline__ float w4_rest(const W4Args& p, int gpb, int row, const W4Rest* list, int n) {
+  float v = 0.f;
+  for (int i = 0; i < n; ++i) v += list[i].value * w4_weight(p, gpb, row, list[i].k);
+  return v;
 }
 
 // One output from its definition, in fp32 and k order: where sums are not finite because x is not,
@@ -181,16 +227,8 @@ __device__ __forceinline__ void w4_cut(const W4Args& p, const W4Digits& d, bool 
 // back.  Slow: some 0.5 to 5 ms for a weight's outputs.
 __device__ __noinline__ float w4_output(const W4Args& p, int gpb, int n, int m) {
   float v = 0.f;
-  const int wb = w4_word_bytes(gpb, p.wide);
   for (int k = 0; k < p.K; ++k) {
-    const int b = k / kW4Block, kk = k % kW4Block;
-    const uint8_t* piece = p.data + (int64_t(n >> 4) * p.blocks + b) * w4_piece_bytes(gpb, p.wide);
-    const uint32_t code =
-        reinterpret_cast<const uint32_t*>(piece + 16 * wb + (n & 15) * 64)[(kk >> 3 & 3) * 4 + (kk >> 5)];
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(piece + (n & 15) * wb) + (kk * gpb / kW4Block) * (p.wide ? 2 : 1);
-    const float s = p.wide ? __uint_as_float(w[1]) : w4_scale16(w[0], p.scale_bf16);
-    const float q = float((code >> (4 * (kk >> 1 & 3) + 16 * (kk & 1))) & 15u) - float(w[0] & 15u);
-    v += load_as_float(p.x, m * p.ldx + k, p.dtype) * (q * s);
+    v += load_as_float(p.x, m * p.ldx + k, p.dtype) * w4_weight(p, gpb, n, k);
     if (v != v) break;  // it stays NaN
   }
   return v;
@@ -341,6 +379,8 @@ __global__ void __launch_bounds__(32 * kW4StreamWarps, 1) w4_stream_kernel(const
   d.sums = reinterpret_cast<int*>(d.digits + p.cols * pitch);
   d.scale = reinterpret_cast<float*>(d.sums + a.slab * GPB * 8);
   d.gpb = GPB;
+  int* rest_counts = reinterpret_cast<int*>(w4_smem + Cfg::kFixed - Cfg::kBarBytes + Cfg::kRestAt);  // of slabs in turn
+  d.rest = reinterpret_cast<W4Rest*>(rest_counts + 2);
   const int g = lane >> 2, t = lane & 3;
   const int rank = p.splits > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   const int cluster = static_cast<int>(blockIdx.x) / p.splits, clusters = static_cast<int>(gridDim.x) / p.splits;
@@ -349,7 +389,7 @@ __global__ void __launch_bounds__(32 * kW4StreamWarps, 1) w4_stream_kernel(const
   const int tile_end = static_cast<int>(int64_t(a.row_tiles) * (cluster + 1) / clusters);
   if (lane == 0) {
     for (int i = 0; i < S; ++i) mbar_init(&bars[i], 1);
-    if (warp == 0) *abort_flag = 0;
+    if (warp == 0) *abort_flag = rest_counts[0] = rest_counts[1] = 0;
     fence_barrier_init();
   }
   __syncthreads();
@@ -498,6 +538,7 @@ __global__ void __launch_bounds__(32 * kW4StreamWarps, 1) w4_stream_kernel(const
   int stage = 0;
   uint32_t phase = 0;
   bool ok = true;
+  int turn = 1, n_rest = 0;  // digits: the slab's count of W4Rest, and how many
   const bool whole_x = b_end - b_begin <= a.slab;
   for (int group = tile_begin; group < tile_end; group += kW4GroupTiles) {
     const int ntiles = min(kW4GroupTiles, tile_end - group);
@@ -532,34 +573,56 @@ __global__ void __launch_bounds__(32 * kW4StreamWarps, 1) w4_stream_kernel(const
       };
 #pragma unroll
       for (int i = 0; i < S; ++i) fetch();
-      if (!whole_x || (group == tile_begin && s0 == b_begin)) {
+      const bool stage_x = !whole_x || (group == tile_begin && s0 == b_begin);
+      if (stage_x) {
+        turn ^= 1;
+        d.rest_count = rest_counts + turn;
         if constexpr (XT == kW4Terms) {
           w4_stage32(p, d.digits, pitch, s0, n);
         } else if constexpr (XT != 0) {
           w4_stage16(p, d.digits, pitch, s0, n);
         } else {
-          for (int base = 0; base < p.M * n; base += T / 16) {
-            const int task = base + (threadIdx.x >> 4);
-            const bool live = task < p.M * n;
-            const int m = live ? task / n : 0, at = live ? task - m * n : 0;
-            w4_cut(p, d, live, m, s0 + at, at, threadIdx.x & 15);
+          for (int base = 0; base < n; base += T / 16) {
+            const int at = base + (threadIdx.x >> 4);
+            w4_cut(p, d, at < n, s0 + at, at, threadIdx.x & 15);
           }
         }
       }
       if (s0 == b_begin)
         for (int i = threadIdx.x; i < ntiles * Cfg::kPart; i += T) tile_sums[i] = 0.f;
       __syncthreads();
+      if constexpr (XT == 0) {
+        if (stage_x) {
+          n_rest = rest_counts[turn];
+          if (threadIdx.x == 0) rest_counts[turn ^ 1] = 0;  // last read before the slab's first barrier
+          if (n_rest > 1 && n_rest <= kW4MaxRest) {  // in order of k, whoever came first
+            W4Rest mine = {};
+            int rank = 0;
+            if (static_cast<int>(threadIdx.x) < n_rest) {
+              mine = d.rest[threadIdx.x];
+              for (int i = 0; i < n_rest; ++i) rank += d.rest[i].k < mine.k;
+            }
+            __syncthreads();
+            if (static_cast<int>(threadIdx.x) < n_rest) d.rest[rank] = mine;
+            __syncthreads();
+          }
+        }
+      }
 
       // A row tile's sums are complete, or as far as this warp goes.
       auto leave = [&](int tile, bool whole, int which) {
         float* dst = whole ? tile_sums + tile * Cfg::kPart : parts + (2 * warp + which) * Cfg::kPart;
         if constexpr (Cfg::kSummed && NT == 1) {
-          // A row of x: two columns here, two (three terms: one) in the neighbouring lane.
+          // A row of x: its digits in all four lanes t, or its terms in two of them (three of four columns).
           const bool both = XT == 0 || (t & 1) == 0;
           float v0 = total[0][0] + (both ? total[0][1] : 0.f), v1 = total[0][2] + (both ? total[0][3] : 0.f);
           v0 += __shfl_xor_sync(0xffffffffu, v0, 1);
           v1 += __shfl_xor_sync(0xffffffffu, v1, 1);
-          if ((t & 1) == 0) {
+          if constexpr (XT == 0) {
+            v0 += __shfl_xor_sync(0xffffffffu, v0, 2);
+            v1 += __shfl_xor_sync(0xffffffffu, v1, 2);
+          }
+          if (XT == 0 ? t == 0 : (t & 1) == 0) {
             float* r = dst + (t >> 1) * 16 + g;
             r[0] = whole ? r[0] + v0 : v0;
             r[8] = whole ? r[8] + v1 : v1;
@@ -640,6 +703,14 @@ __global__ void __launch_bounds__(32 * kW4StreamWarps, 1) w4_stream_kernel(const
         if (last_tile != first_tile) gather(last_tile);
       }
       __syncthreads();
+      if constexpr (XT == 0) {
+        if (n_rest > 0) {  // rare; more than the list holds: the outputs are computed one by one
+          for (int i = threadIdx.x; i < ntiles * 16; i += T)
+            tile_sums[i] += n_rest > kW4MaxRest ? __int_as_float(0x7fc00000)
+                                                : w4_rest(p, GPB, group * 16 + i, d.rest, n_rest);
+          __syncthreads();
+        }
+      }
     }
 
     // Outputs of the group's tiles, from all CTAs' sums of a cluster.

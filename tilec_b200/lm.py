@@ -387,9 +387,7 @@ def matrix_mul_w4(x, weight, bias=None, out=None):
     `out`, [..., N] with unit column stride, sharing no memory with x or bias) x's dtype.
 
     Up to 8 rows of x, the decoding case (many 16-bit calls of up to 16), the codes are read once
-    and enter exactly, as x does: sums are fp32, with one rounding at the end.  (One 16-bit row,
-    or two of a large weight, goes through the integer tensor path, where x is held in steps of
-    2^-29 of the power of two at or below the largest magnitude of its block of 128.)  With more
+    and enter exactly, as x does: sums are fp32, with one rounding at the end.  With more
     rows the weight is rounded once to x's dtype and multiplied on the tensor cores: up to 256 rows of 16-bit x (and scales
     of its dtype) it is expanded on the way, otherwise into the workspace, at most 256 MiB (or
     256 rows of it) at a time (float32: exact, and the 3xTF32 product of matrix_mul).  Not
