@@ -734,3 +734,58 @@ def test_large_elements_beside_small_ones_in_16_bits(m, n, k, dtype, top, few):
     assert ((got.double() - y).abs() <= tol).all(), f"{((got.double() - y).abs() / tol).max():.1f} of the bound"
     for _ in range(3):
         assert torch.equal(ext.matrix_mul_w4(x, w), got)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("m", [1, 2, 4, 8, 13])
+def test_not_finite_rows_follow_the_formula(m, dtype):
+    """x infinite at one place gives the sign of that weight (NaN where it is zero), NaN gives NaN, and
+    a huge finite row beside them its product."""
+    if m > 8 and dtype == "f32":
+        pytest.skip("from 9 rows on the fp32 product splits infinities")
+    x, codes, scales, zeros = _huge(max(m, 4), dtype, "f32")
+    w64 = _weight64(codes, scales, zeros, 64)
+    w = ext.pack_w4(codes, scales, zeros, 64).to("cuda")
+    nan, inf = x[1:2].clone(), _make(1, 150, 384, 64, dtype)[0]
+    nan[0, 200], inf[0, 77] = float("nan"), float("-inf")
+    for batch in ([nan, inf, x[:1], x[2:3]] * 4, [x[:1], inf, nan, x[3:4]] * 4, [inf] * 16, [nan] * 16):
+        batch = torch.cat(batch)[:m]
+        got = ext.matrix_mul_w4(batch.cuda(), w).cpu().double()
+        for row, out in zip(batch, got):
+            if torch.isnan(row).any():
+                assert torch.isnan(out).all()
+            elif torch.isinf(row).any():
+                sign = -torch.sign(w64[:, 77])
+                assert torch.equal(torch.isnan(out), sign == 0) and (out[sign != 0] == sign[sign != 0] * float("inf")).all()
+            else:
+                y = w64 @ row.double()
+                tol = _bound(row[None], w64, y[None], dtype, 1)[0] if m <= 8 else 2.0 ** -13 * y.abs() + _bound(
+                    row[None], w64, y[None], dtype, 9)[0]
+                assert ((out - y).abs() <= tol).all()
+
+
+@gpu
+def test_a_nan_row_costs_the_batch_little():
+    """A row of a batch that is not finite (a padded one, say) is not computed one output at a time:
+    the call takes less than eight times the finite one (one at a time: some twenty times)."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    codes = torch.randint(0, 16, (8192, 8192), device="cuda", generator=g, dtype=torch.uint8)
+    w = ext.pack_w4(codes, torch.rand(8192, 64, device="cuda", generator=g).bfloat16())
+    x = torch.randn(8, 8192, device="cuda", generator=g).bfloat16()
+    bad = x.clone()
+    bad[3, 4000] = float("nan")
+
+    def best(t):
+        times = []
+        for _ in range(20):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            for _ in range(4):
+                ext.matrix_mul_w4(t, w)
+            b.record()
+            b.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times)
+
+    assert best(bad) <= 8 * best(x)

@@ -94,6 +94,7 @@ struct W4StreamCfg {
   static constexpr int kStages = 2;
   static constexpr int kRingBytes = kW4StreamWarps * kStages * kStage;
   static constexpr bool kSummed = XT == 0 || XT == kW4Terms;  // several columns to a row of x
+  static_assert(kW4GroupTiles * 16 * 8 * NT <= 32 * kThreads, "a bit per output of a thread");
   static_assert(!(XT == 0 && NT != 1) && !(XT == kW4Terms && NT != 1 && NT != 3), "columns of several to a row");
   static constexpr int kRows = XT == 0 ? 1 : kSummed && NT == 1 ? 2 : kSummed ? 8 : 8 * NT;  // rows of x
   static constexpr int kPart = kRows * 16;  // floats: the sums of a row tile, [row of x][16]
@@ -103,10 +104,12 @@ struct W4StreamCfg {
   static constexpr int kChains = NT == 3 ? 1 : 2;
   static constexpr int kSumBytes = kW4GroupTiles * kPart * 4;
   static constexpr int kPartBytes = 2 * kW4StreamWarps * kPart * 4;
-  static constexpr int kBarBytes = 1024;     // a barrier per warp and stage, W4Rest, the abort flag
+  static constexpr int kBarBytes = 1024;     // a barrier per warp and stage, rows' states, W4Rest, the abort flag
+  static constexpr int kStatesAt = 256;      // w4_row_states of 16 rows, and whether they are wanted
   static constexpr int kRestAt = 512 - 16;   // two counts, then the entries
   static constexpr int kFixed = kRingBytes + kSumBytes + kPartBytes + kBarBytes;
-  static_assert(kStage % 128 == 0 && kW4StreamWarps * kStages * 8 <= kRestAt, "shared memory layout");
+  static_assert(kStage % 128 == 0 && kW4StreamWarps * kStages * 8 <= kStatesAt, "shared memory layout");
+  static_assert(kStatesAt + 17 * 4 <= kRestAt, "shared memory layout");
   static_assert(kRestAt + 8 + kW4MaxRest * 8 <= kBarBytes - 8, "shared memory layout");
 };
 // Bytes of `slab` blocks of x: digits (16 bytes more a column: conflict-free reads), sums, scales.
@@ -222,9 +225,9 @@ __device__ __noinline__ float w4_rest(const W4Args& p, int gpb, int row, const W
   return v;
 }
 
-// One output from its definition, in fp32 and k order: where sums are not finite because x is not,
-// or because codes times an x of 2^117 or more are past fp32's range before the scale brings them
-// back.  Slow: some 0.5 to 5 ms for a weight's outputs.
+// One output from its definition, in fp32 and k order: where the digits'
+// sums are not finite because x is not, or where codes times an x of 2^117 or more are past fp32's
+// range before the scale brings them back.  Slow: some 0.5 to 5 ms for a weight's outputs.
 __device__ __noinline__ float w4_output(const W4Args& p, int gpb, int n, int m) {
   float v = 0.f;
   for (int k = 0; k < p.K; ++k) {
@@ -232,6 +235,24 @@ __device__ __noinline__ float w4_output(const W4Args& p, int gpb, int n, int m) 
     if (v != v) break;  // it stays NaN
   }
   return v;
+}
+
+// Whether rows of x hold infinities (bit 0 of states[m]) or NaN (bit 1).  All threads of a CTA call;
+// asked only where an output is not finite.
+__device__ __noinline__ void w4_row_states(const W4Args& p, int* states) {
+  const bool wide = p.dtype == TILEC_DTYPE_F32;
+  const uint32_t top = wide ? 0x7F800000u : p.dtype == TILEC_DTYPE_BF16 ? 0x7F80u : 0x7C00u;
+  for (int m = 0; m < p.M; ++m) {
+    int state = 0;
+    for (int k = threadIdx.x; k < p.K; k += 32 * kW4StreamWarps) {
+      const int64_t at = m * p.ldx + k;
+      const uint32_t bits = wide ? static_cast<const uint32_t*>(p.x)[at] & 0x7FFFFFFFu
+                                 : static_cast<const unsigned short*>(p.x)[at] & 0x7FFFu;
+      if (bits >= top) state |= bits == top ? 1 : 2;
+    }
+    if (state != 0) atomicOr(&states[m], state);
+  }
+  __syncthreads();
 }
 
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -381,6 +402,8 @@ __global__ void __launch_bounds__(32 * kW4StreamWarps, 1) w4_stream_kernel(const
   d.gpb = GPB;
   int* rest_counts = reinterpret_cast<int*>(w4_smem + Cfg::kFixed - Cfg::kBarBytes + Cfg::kRestAt);  // of slabs in turn
   d.rest = reinterpret_cast<W4Rest*>(rest_counts + 2);
+  int* row_states = reinterpret_cast<int*>(w4_smem + Cfg::kFixed - Cfg::kBarBytes + Cfg::kStatesAt);
+  volatile int* again_flag = row_states + 16;  // some output was not finite
   const int g = lane >> 2, t = lane & 3;
   const int rank = p.splits > 1 ? static_cast<int>(cluster_ctarank()) : 0;
   const int cluster = static_cast<int>(blockIdx.x) / p.splits, clusters = static_cast<int>(gridDim.x) / p.splits;
@@ -392,6 +415,7 @@ __global__ void __launch_bounds__(32 * kW4StreamWarps, 1) w4_stream_kernel(const
     if (warp == 0) *abort_flag = rest_counts[0] = rest_counts[1] = 0;
     fence_barrier_init();
   }
+  if (threadIdx.x <= 16) row_states[threadIdx.x] = 0;
   __syncthreads();
   pdl_wait();
   pdl_launch_dependents();
@@ -539,6 +563,7 @@ __global__ void __launch_bounds__(32 * kW4StreamWarps, 1) w4_stream_kernel(const
   uint32_t phase = 0;
   bool ok = true;
   int turn = 1, n_rest = 0;  // digits: the slab's count of W4Rest, and how many
+  bool have_states = false;
   const bool whole_x = b_end - b_begin <= a.slab;
   for (int group = tile_begin; group < tile_end; group += kW4GroupTiles) {
     const int ntiles = min(kW4GroupTiles, tile_end - group);
@@ -716,10 +741,16 @@ __global__ void __launch_bounds__(32 * kW4StreamWarps, 1) w4_stream_kernel(const
     // Outputs of the group's tiles, from all CTAs' sums of a cluster.
     if (p.splits > 1) cluster_sync();
     const int count = ntiles * 16 * p.M;
-    for (int i = rank * T + threadIdx.x; i < count; i += p.splits * T) {
+    auto put = [&](int i, float v) {
+      const int row = group * 16 + (i >> 4) / p.M * 16 + (i & 15), m = (i >> 4) % p.M;
+      if (p.bias != nullptr) v += load_as_float(p.bias, row, p.dtype);
+      store_from_float(p.out, int64_t(m) * p.ldo + row, p.dtype, v);
+    };
+    uint32_t again = 0;  // this thread's outputs that are not finite, one bit each
+    int turn_out = 0;
+    for (int i = rank * T + threadIdx.x; i < count; i += p.splits * T, ++turn_out) {
       const int r = i & 15, m = (i >> 4) % p.M, tl = (i >> 4) / p.M, at = tl * Cfg::kPart + m * 16 + r;
-      const int row = (group + tl) * 16 + r;
-      if (row >= p.N) continue;
+      if ((group + tl) * 16 + r >= p.N) continue;
       float v = 0.f;
       if (p.splits == 1) {
         v = tile_sums[at];
@@ -731,14 +762,25 @@ __global__ void __launch_bounds__(32 * kW4StreamWarps, 1) w4_stream_kernel(const
           v += u;
         }
       }
-      if constexpr (XT != TILEC_DTYPE_F16) {  // fp16 times codes stays in range, and is not finite by itself
-        if (!(fabsf(v) <= FLT_MAX)) v = w4_output(p, GPB, row, m);
-      }
-      if (p.bias != nullptr) v += load_as_float(p.bias, row, p.dtype);
-      store_from_float(p.out, int64_t(m) * p.ldo + row, p.dtype, v);
+      if (XT != TILEC_DTYPE_F16 && !(fabsf(v) <= FLT_MAX)) again |= 1u << turn_out;
+      put(i, v);
     }
+    if (again) *again_flag = 1;
     if (p.splits > 1) cluster_sync();  // every CTA's sums have been read
     else __syncthreads();
+    // Sums that are not finite though x is have left fp32's range (fp16 cannot), or were given up;
+    // an x in digits that is not finite has none.
+    if constexpr (XT != TILEC_DTYPE_F16) {
+      if (*again_flag) {
+        if (!have_states) w4_row_states(p, row_states);
+        have_states = true;
+        for (; again; again &= again - 1) {
+          const int i = rank * T + threadIdx.x + (__ffs(again) - 1) * p.splits * T, m = (i >> 4) % p.M;
+          if (XT == 0 ? (row_states[m] & 2) == 0 : row_states[m] == 0)
+            put(i, w4_output(p, GPB, group * 16 + (i >> 4) / p.M * 16 + (i & 15), m));
+        }
+      }
+    }
   }
 }
 
