@@ -9,6 +9,8 @@ The kernels are behind the C ABI (tilec_linear_ce_*, tilec_mm_w4 in include/tile
 Like the rest of the package there is no CPU path for the products: CPU tensors raise, and a
 missing kernel library raises.  (Packing and quantising are plain torch and run anywhere.)
 """
+from types import SimpleNamespace
+
 import torch
 from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
@@ -46,10 +48,12 @@ def _library():
     return _native.load()
 
 
+# torch's count of forward-mode levels: below 0 outside all of them, where no tensor has a tangent.
+_levels = forward_ad if hasattr(forward_ad, "_current_level") else SimpleNamespace(_current_level=0)
+
+
 def _refuse_tangents(where, *tensors):
     """Raises for a tensor with a forward-mode tangent, which the kernels would drop."""
-    if getattr(forward_ad, "_current_level", 0) < 0:   # outside every dual level: nothing to look for
-        return
     for t in tensors:
         if t is not None and forward_ad.unpack_dual(t).tangent is not None:
             raise ValueError(f"{where}: no forward-mode derivative; detach the inputs")
@@ -200,7 +204,8 @@ def linear_cross_entropy(x, weight, target, ignore_index=-100, reduction="mean")
                          f"{tuple(x.shape[:-1])}")
     if weight.shape[0] == 0 or weight.shape[1] == 0:
         raise ValueError(f"linear_cross_entropy: weight {tuple(weight.shape)} is empty")
-    _refuse_tangents("linear_cross_entropy", x, weight)
+    if _levels._current_level >= 0:
+        _refuse_tangents("linear_cross_entropy", x, weight)
     if not (x.is_cuda and weight.device == x.device and target.device == x.device):
         raise ValueError(f"linear_cross_entropy: inputs must be CUDA tensors on one device (got {x.device}, "
                          f"{weight.device} and {target.device}); tilec_b200 has no CPU path")
@@ -401,7 +406,8 @@ def matrix_mul_w4(x, weight, bias=None, out=None):
     dt = _DTYPES.get(x.dtype)
     if dt is None:
         raise TypeError(f"matrix_mul_w4: x must be float32, float16 or bfloat16, got {x.dtype}")
-    _refuse_tangents("matrix_mul_w4", x, bias, out)
+    if _levels._current_level >= 0:
+        _refuse_tangents("matrix_mul_w4", x, bias, out)
     dev = x.device
     if not (x.is_cuda and weight.device == dev):
         raise ValueError(f"matrix_mul_w4: x and weight must be on one CUDA device (got {dev} and {weight.device}); "
@@ -424,7 +430,9 @@ def matrix_mul_w4(x, weight, bias=None, out=None):
         return out
     if bias is not None:
         bias = bias.contiguous()
-    lib = _library()
+    if not select._installed:
+        select.ensure_installed()
+    fast = _native.fast()
     index = dev.index
     prev = torch.cuda.current_device()
     switch = prev != index
@@ -437,13 +445,12 @@ def matrix_mul_w4(x, weight, bias=None, out=None):
         key = (dt, m, ldx, sdt, n, k, group, ldo, px & 15, po & 15, index)
         nbytes = _W4_BYTES.get(key)
         if nbytes is None:
-            nbytes = lib.tilec_mm_w4_workspace_bytes(px, dt, m, ldx, sdt, n, k, group, po, ldo)
+            nbytes = _native.load().tilec_mm_w4_workspace_bytes(px, dt, m, ldx, sdt, n, k, group, po, ldo)
             if len(_W4_BYTES) >= 4096:  # a process that sees many shapes: start over
                 _W4_BYTES.clear()
             _W4_BYTES[key] = nbytes
         ws = _workspace(nbytes, dev)
-        fast = _native.fast()
-        rc = (fast.w4 if fast is not None else lib.tilec_mm_w4)(
+        rc = (fast.w4 if fast is not None else _native.load().tilec_mm_w4)(
             px, dt, m, ldx, weight.data.data_ptr(), sdt, n, k, group, _ptr(bias), po, ldo, _ptr(ws), nbytes, stream)
         _native.check(rc, "tilec_mm_w4")
         _check_device(stream)
