@@ -279,7 +279,8 @@ TILEC_API int tilec_mm_f32_splitk_noalloc(const float* A, const float* B, float*
  *   loss:  T floats (TILEC_REDUCE_NONE) or one float.
  *   stats: 2 * T + 1 floats, 8-byte aligned, for the backward pass: per token (m, s) with
  *          sum_v exp(logit) = s * 2^m, then (SUM / MEAN) the number of tokens with a target.
- * Workspace: tilec_linear_ce_workspace_bytes(..., grads = 0). */
+ * Workspace: tilec_linear_ce_workspace_bytes(..., grads = 0): 16 bytes per token and 256 entries of
+ * the vocabulary, copies of operands, and for fp32 a piece of the logits. */
 TILEC_API int tilec_linear_ce_forward(const void* x, const void* w, const int64_t* target, int32_t dtype, int64_t T,
                                       int64_t V, int64_t D, int64_t ldx, int64_t ldw, int64_t ignore_index,
                                       int32_t reduction, float* loss, float* stats, void* workspace,
@@ -317,8 +318,9 @@ TILEC_API size_t tilec_linear_ce_workspace_bytes(const void* x, const void* w, i
  *   0..7 of the block, k = 2i in bits 4i..4i+3 and k = 2i + 1 in bits 4i+16..4i+19 (i = 0..3).
  *   Rows past N and k past K: any codes, finite scales.
  * Up to 8 rows (many 16-bit calls of up to 16), x, codes, zero points and scales enter exactly and
- * sums are fp32.  With more rows the weight (code - zero) * scale is rounded once to dtype and multiplied on the tensor
- * cores (fp32: the 3xTF32 product).  out shares no memory with x or bias.
+ * sums are fp32.  With more rows the weight (code - zero) * scale is rounded once to dtype (fp16:
+ * infinite past 65504) and multiplied on the tensor cores (fp32: the 3xTF32 product).  So a row's
+ * bits depend on how many rows it comes with.  out shares no memory with x or bias.
  * Workspace: tilec_mm_w4_workspace_bytes (at most 256 MiB of expanded weights or 256 rows). */
 TILEC_API int tilec_mm_w4(const void* x, int32_t dtype, int64_t M, int64_t ldx, const void* weight,
                           int32_t scale_dtype, int64_t N, int64_t K, int64_t group, const void* bias, void* out,

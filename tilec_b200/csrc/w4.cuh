@@ -15,7 +15,10 @@
 //   scale << 16 (16-bit scales), or two, zero and the fp32 scale.  Groups longer than 128 have
 //   theirs in every block.
 //
-// Up to 256 rows of x the product streams the codes once (K/2 bytes a row of W).  At full
+// The codes are streamed once (K/2 bytes a row of W) for up to 16 rows of 16-bit x and 8 of fp32 x,
+// and once per 128 rows for up to 256 rows of 16-bit x whose type the scales share; for the rest W
+// is expanded in memory first (w4_expand_kernel, 5 times the codes' bytes in 16 bits, 9 in fp32,
+// written and read again).  At full
 // bandwidth an SM has under three lane-instructions per weight, too few to convert and multiply
 // each weight on the FMA pipe, so the sums run on tensor cores: mma.sync, 16 rows of W against 8
 // columns at a time, for up to 16 rows of x (w4_stream.cuh), tcgen05 with the weight expanded in
@@ -82,7 +85,8 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// The pair of codes i of a word, minus the zero point (zm = the magic number | zero, twice).
+// The pair of codes i of a word, minus the zero point (zm = the magic number | zero, twice): the
+// well-known way to a 16-bit float, a small number in the low bits of the mantissa of a power of two.
 // The and-or is one three-input logic instruction; left to the compiler it became two, and
 // the integer pipe is what this kernel's arithmetic runs into first.
 template <bool BF16>

@@ -1,8 +1,8 @@
 // w4_tc.cuh -- products of some tens of rows with 4-bit weights on the 5th-generation tensor
 // cores (tcgen05, fp32 accumulators in TMEM), the weight expanded on the way.
 //
-// From some 9 to 17 rows of x on (see plan_w4), mma.sync's share of the work grows with the rows while the weight still
-// has to be read once; expanding it in HBM first (w4_expand_kernel) costs five times its bytes.
+// From some 9 to 17 rows of x on (see plan_w4), mma.sync's share of the work grows with the rows
+// while the weight still has to be read once (129 to 256 rows: twice, 128 rows at a time); expanding it in HBM first (w4_expand_kernel) costs five times its bytes.
 // Here a CTA takes 128 rows of W as the M side of the product and up to 128 rows of x as its N
 // side (swapped, so that the few rows of x pad to 16 and not to 128 or 256):
 //   * one warp fetches codes (bulk copies of four blocks per 16-row tile, a run of memory each,

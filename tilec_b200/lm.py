@@ -173,16 +173,24 @@ def linear_cross_entropy(x, weight, target, ignore_index=-100, reduction="mean")
     Returns the float32 loss: a scalar, or one value per token for "none".  Gradients are
     reverse-mode and of first order: forward-mode tangents are refused.
 
-    Logits and their softmax are computed in fp32 and never kept: the forward pass keeps two
-    floats per token, the backward pass computes the logits again a piece of the vocabulary
-    at a time.  Its workspace is at most 512 MiB for a piece (or 4096 vocabulary entries, for
-    very many tokens), a copy of x, fp32 sums of x's shape, and a copy of `weight` when its
-    rows are not 16-byte aligned.  The gradients are sums in fp32 rounded once to x's dtype;
-    the logits' gradient is rounded to the operands' dtype on the way (float32: not at all).
+    Logits and their softmax are computed in fp32 and never kept whole: the forward pass keeps
+    two floats per token, the backward pass computes the logits again a piece of the vocabulary
+    at a time.  The gradients are sums in fp32 rounded once to x's dtype; the logits' gradient is
+    rounded to the operands' dtype on the way (float32: not at all).
 
-    A token whose target is ignore_index has loss 0 and gradient 0 whatever its row holds; a
-    16-bit call does no products for it.  Any other target outside [0, V) makes the token's
-    loss and the gradients NaN and sets a device status bit (ext.check_device raises it).
+    Workspace of a forward pass: 16 bytes per token and 256 vocabulary entries (512 MiB for 65536
+    tokens and 131072 entries); of 16-bit operands a copy of x above 256 tokens; of float32 ones a
+    piece of the logits.  Of a backward pass: a piece of the logits' gradient and a copy of x,
+    fp32 sums of x's shape where there are several pieces, at most 20 MB of partial sums, and,
+    where D is no multiple of 8, a 16-bit copy of a piece's gradient (of the whole weight's, where
+    one piece is all of the vocabulary).  Of either: a copy of `weight` when its 16-bit rows are
+    not 16-byte aligned, and what the float32 products take (operands that are not aligned,
+    partial sums).  A piece is at most 512 MiB, or 4096 vocabulary entries for very many tokens.
+
+    A token whose target is ignore_index has loss 0 and gradient 0 whatever its row holds; with
+    16-bit operands a backward pass, and a forward pass of more than 256 tokens, do no products
+    for it.  Any other target outside [0, V) makes the token's loss and the gradients NaN and
+    sets a device status bit (ext.check_device raises it).
 
     Forward and backward can be captured into a CUDA graph.  As with any torch operator, drop
     the losses of eager calls on the same leaves before capturing a backward() (or capture
@@ -392,11 +400,18 @@ def matrix_mul_w4(x, weight, bias=None, out=None):
     `out`, [..., N] with unit column stride, sharing no memory with x or bias) x's dtype.
 
     Up to 8 rows of x, the decoding case (many 16-bit calls of up to 16), the codes are read once
-    and enter exactly, as x does: sums are fp32, with one rounding at the end.  With more
-    rows the weight is rounded once to x's dtype and multiplied on the tensor cores: up to 256 rows of 16-bit x (and scales
-    of its dtype) it is expanded on the way, otherwise into the workspace, at most 256 MiB (or
-    256 rows of it) at a time (float32: exact, and the 3xTF32 product of matrix_mul).  Not
-    differentiable: inputs that require a gradient or carry a forward-mode tangent are refused."""
+    and enter exactly, as x does: sums are fp32, with one rounding at the end.  With more rows the
+    weight is rounded once to x's dtype (float16: what is past 65504 becomes infinite) and
+    multiplied on the tensor cores: up to 256 rows of 16-bit x with scales of its dtype it is
+    expanded on the way, once per 128 rows; otherwise into the workspace, at most 256 MiB (or
+    256 rows of it) at a time (float32: exact, and the 3xTF32 product of matrix_mul).  So a token's
+    bits depend on how many rows it comes with.
+
+    Infinities and NaN in x stay in their rows, as in the formula (float32 from 9 rows on: NaN).
+    Up to 16 rows, outputs whose sums leave float32's range before the scales bring them back (x of
+    2^117 or more), and those of a single 16-bit row with infinities, are computed one at a time,
+    which takes 0.5 to 5 ms.  Not differentiable: inputs that require a gradient or carry a
+    forward-mode tangent are refused."""
     if not isinstance(weight, W4Weight):
         raise TypeError(f"matrix_mul_w4: weight must be a W4Weight (pack_w4, quantize_w4), got {type(weight).__name__}")
     n, k = weight.shape
